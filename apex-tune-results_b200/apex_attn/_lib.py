@@ -76,6 +76,31 @@ class BwdVarlenArgs(ctypes.Structure):
                 ("strides", ctypes.c_longlong * 16)]
 
 
+class KVPlanArgs(ctypes.Structure):
+    """Mirror of apex_attn_kv_plan_args (include/apex_attn.h)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "block_table", "seq_lens", "new_lens", "finished", "free_blocks", "free_count", "slots", "cu_seqlens",
+        "seq_lens_out", "free_count_out", "placed")] + [("table_stride", ctypes.c_longlong)] + [
+        (n, ctypes.c_int) for n in ("batch", "table_width", "free_capacity", "block_size", "max_new_tokens")]
+
+
+class KVAppendArgs(ctypes.Structure):
+    """Mirror of apex_attn_kv_append_args (include/apex_attn.h)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_cache", "v_cache", "k_scale", "v_scale", "slots")] + [
+        (n, ctypes.c_int) for n in ("total", "heads_kv", "head_dim", "dtype", "num_blocks", "block_size")] + [
+        ("strides", ctypes.c_longlong * 10)]
+
+
+class PagedArgs(ctypes.Structure):
+    """Mirror of apex_attn_paged_args (include/apex_attn.h)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "q", "k_cache", "v_cache", "k_scale", "v_scale", "block_table", "seq_lens", "cu_seqlens_q", "o", "lse")] + [
+        ("table_stride", ctypes.c_longlong), ("strides", ctypes.c_longlong * 10)] + [
+        (n, ctypes.c_int) for n in (
+            "batch", "heads_q", "heads_kv", "total_q", "max_seqlen_q", "head_dim", "dtype", "num_blocks",
+            "block_size", "table_width", "causal", "window_left", "zero_rest")] + [("sm_scale", ctypes.c_float)]
+
+
 # Every symbol the header declares: (name, restype, argtypes).
 _c_ll_p = ctypes.POINTER(ctypes.c_longlong)
 SYMBOLS = {
@@ -104,6 +129,12 @@ SYMBOLS = {
                                           ctypes.c_size_t, ctypes.c_void_p]),
     "apex_attn_bwd_varlen_mode": (ctypes.c_int, [ctypes.POINTER(BwdVarlenArgs), ctypes.c_int,
                                                  ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "apex_attn_kv_plan": (ctypes.c_int, [ctypes.POINTER(KVPlanArgs), ctypes.c_void_p]),
+    "apex_attn_kv_release": (ctypes.c_int, [ctypes.POINTER(KVPlanArgs), ctypes.c_void_p]),
+    "apex_attn_kv_append": (ctypes.c_int, [ctypes.POINTER(KVAppendArgs), ctypes.c_void_p]),
+    "apex_attn_fwd_paged_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 4),
+    "apex_attn_fwd_paged": (ctypes.c_int, [ctypes.POINTER(PagedArgs), ctypes.c_void_p, ctypes.c_size_t,
+                                           ctypes.c_void_p]),
     "apex_attn_num_sms_hint": (ctypes.c_int, [ctypes.c_int]),
     "apex_attn_set_forward_kernel": (ctypes.c_int, [ctypes.c_int]),
     "apex_attn_forward_kernel_for": (ctypes.c_int, [ctypes.c_int] * 7),

@@ -1,8 +1,10 @@
 """Builds libapex_attn.so in-tree (next to the apex_attn package) with nvcc for sm_100a.
 
 Usage: python apex-tune-results_b200/build.py [--verbose]
-The library links the CUDA runtime statically and resolves cuTensorMapEncodeTiled through
-cudaGetDriverEntryPoint, so it needs no -lcuda and loads on a machine without a GPU.
+Each source is compiled to an object under _build/ (side by side, and only when it or a
+header changed), then linked. The library links the CUDA runtime statically and resolves
+cuTensorMapEncodeTiled through cudaGetDriverEntryPoint, so it needs no -lcuda and loads on
+a machine without a GPU.
 """
 from __future__ import annotations
 
@@ -15,10 +17,18 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
+OBJ = os.path.join(HERE, "_build")
 OUT = os.path.join(HERE, "apex_attn", "libapex_attn.so")
-SOURCES = [os.path.join(CSRC, "attn_fwd.cu")]
-HEADERS = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))] + [
-    os.path.join(ROOT, "include", "apex_attn.h")]
+SOURCES = [os.path.join(CSRC, "attn_fwd.cu"), os.path.join(CSRC, "paged.cu")]
+API = os.path.join(ROOT, "include", "apex_attn.h")
+# Headers each source includes (a change in one recompiles only the sources that list it).
+_SHARED = [API, *(os.path.join(CSRC, f) for f in ("runtime.h", "sm100_ptx.cuh", "attn_fwd_kernel.cuh"))]
+HEADERS = {
+    SOURCES[0]: _SHARED + [os.path.join(CSRC, f) for f in ("attn_fwd_tile_kernel.cuh", "attn_bwd_kernel.cuh")],
+    SOURCES[1]: _SHARED + [os.path.join(CSRC, f) for f in ("attn_paged_kernel.cuh", "kv_cache_kernels.cuh")],
+}
+FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo", "-Xptxas", "-v",
+         "-Xcompiler", "-fPIC", "-I", os.path.join(ROOT, "include"), "-I", CSRC]
 
 
 def nvcc_path() -> str:
@@ -28,30 +38,50 @@ def nvcc_path() -> str:
     raise RuntimeError("nvcc not found")
 
 
-def command(out: str = OUT) -> list[str]:
-    return [nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17",
-            "-lineinfo", "-Xptxas", "-v", "-Xcompiler", "-fPIC", "-shared",
-            "-I", os.path.join(ROOT, "include"), "-I", CSRC, "-o", out, *SOURCES]
+def object_of(source: str) -> str:
+    return os.path.join(OBJ, os.path.splitext(os.path.basename(source))[0] + ".o")
+
+
+def newer(target: str, inputs: list[str]) -> bool:
+    return os.path.exists(target) and all(os.path.getmtime(f) <= os.path.getmtime(target) for f in inputs)
+
+
+def stale_sources() -> list[str]:
+    return [s for s in SOURCES if not newer(object_of(s), [s, *HEADERS[s], __file__])]
 
 
 def up_to_date() -> bool:
-    if not os.path.exists(OUT):
-        return False
-    t = os.path.getmtime(OUT)
-    return all(os.path.getmtime(f) <= t for f in SOURCES + HEADERS + [__file__])
+    inputs = [f for s in SOURCES for f in (s, *HEADERS[s])] + [__file__]
+    return newer(OUT, inputs)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and up_to_date():
         return OUT
+    os.makedirs(OBJ, exist_ok=True)
+    nvcc = nvcc_path()
+    jobs = []
+    for source in SOURCES if force else stale_sources():
+        cmd = [nvcc, *FLAGS, "-c", "-o", object_of(source) + ".tmp", source]
+        jobs.append((source, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    failed = []
+    for source, job in jobs:
+        log = job.communicate()[0]
+        if job.returncode != 0:
+            sys.stderr.write(log)
+            failed.append(os.path.basename(source))
+            continue
+        if verbose:
+            sys.stdout.write(log)
+        os.replace(object_of(source) + ".tmp", object_of(source))
+    if failed:
+        raise RuntimeError("nvcc failed building libapex_attn.so: " + ", ".join(failed))
     tmp = OUT + ".tmp"
-    proc = subprocess.run(command(tmp), capture_output=True, text=True)
+    proc = subprocess.run([nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-Xcompiler", "-fPIC",
+                           "-o", tmp, *map(object_of, SOURCES)], capture_output=True, text=True)
     if proc.returncode != 0:
         sys.stderr.write(proc.stdout + proc.stderr)
-        raise RuntimeError("nvcc failed building libapex_attn.so")
-    log = proc.stdout + proc.stderr
-    if verbose:
-        sys.stdout.write(log)
+        raise RuntimeError("nvcc failed linking libapex_attn.so")
     os.replace(tmp, OUT)
     return OUT
 

@@ -24,10 +24,14 @@
 #include "attn_bwd_kernel.cuh"
 #include "attn_fwd_kernel.cuh"
 #include "attn_fwd_tile_kernel.cuh"
+#include "runtime.h"
 
 namespace {
 
 using apex::AttnParams;
+using apex::host::aligned16;
+using apex::host::DeviceGuard;
+using apex::host::kMaxDevices;
 
 constexpr int kVersion = 300;  // 0.3.0
 
@@ -66,7 +70,6 @@ constexpr int kEmuTile = D == 64 ? APEX_TILE_EMU64 : APEX_TILE_EMU128;
 // two-sub-tile kernel for every call, 2 = the tile kernel wherever it applies.
 std::atomic<int> g_fwd_kind{0};
 
-constexpr int kMaxDevices = 64;
 // Per-device scratch of the kernel: int[64]. Word 0 is the status word; words
 // [kCounterBase, kCounterBase + kCounterSlots) are work-item counters. Each call takes the
 // next slot (round robin) and zeroes it on its stream before the launch, so calls that
@@ -304,8 +307,6 @@ int launch(DeviceState& ds, unsigned attr_bit, const CUtensorMap& mq, const CUte
              : launch_one<D, T, false, false>(ds, attr_bit, mq, mk, mv, p, grid, stream);
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 int item_rows(int head_dim) {
   switch (head_dim) {
     case 64: return apex::Cfg<64>::kItemRows;
@@ -313,21 +314,6 @@ int item_rows(int head_dim) {
     default: return apex::Cfg<256>::kItemRows;
   }
 }
-
-struct DeviceGuard {
-  int prev = -1;
-  explicit DeviceGuard(int dev) {
-    if (cudaGetDevice(&prev) != cudaSuccess) {
-      (void)cudaGetLastError();
-      prev = -1;
-    }
-    if (prev != dev) cudaSetDevice(dev);
-  }
-  ~DeviceGuard() {
-    int cur = -1;
-    if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
-  }
-};
 
 __global__ void wait_timeout_selftest_kernel(int* status, int* host_flag, unsigned long long timeout_ns) {
   __shared__ __align__(8) uint64_t bar;
@@ -925,6 +911,28 @@ int backward_varlen(const apex_attn_bwd_varlen_args* a, int mode, void* workspac
 }
 
 }  // namespace
+
+namespace apex {
+namespace host {
+
+int device_of(const void* ptr) { return ::device_of(ptr); }
+
+int acquire(int dev, Device* out) {
+  DeviceState* ds = nullptr;
+  int rc = init_device(dev, &ds);
+  if (rc != APEX_ATTN_OK || (rc = sticky_error(*ds)) != APEX_ATTN_OK) return rc;
+  out->status = ds->status;
+  out->host_flag_dev = ds->host_flag_dev;
+  out->num_sms = ds->num_sms;
+  return APEX_ATTN_OK;
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() { return g_encode; }
+
+unsigned long long wait_timeout_ns() { return ::wait_timeout_ns(); }
+
+}  // namespace host
+}  // namespace apex
 
 extern "C" {
 

@@ -1,0 +1,305 @@
+// Host side of the paged 8-bit K/V cache operators: argument validation and launches behind
+// the C ABI declared in include/apex_attn.h.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <climits>
+#include <cmath>
+#include <cstdint>
+
+#include "apex_attn.h"
+#include "attn_paged_kernel.cuh"
+#include "kv_cache_kernels.cuh"
+#include "runtime.h"
+
+namespace {
+
+using apex::host::aligned16;
+using apex::host::device_of;
+using apex::host::DeviceGuard;
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+int launched() {
+  if (cudaGetLastError() != cudaSuccess) return APEX_ATTN_ERR_LAUNCH;
+  return APEX_ATTN_OK;
+}
+
+// 16, 32, 64 or 128 -> its logarithm; -1 otherwise.
+int block_shift_of(int block_size) {
+  for (int s = 4; s <= 7; ++s)
+    if (block_size == 1 << s) return s;
+  return -1;
+}
+
+// Every pointer of a call lives on the device of the first; nulls are skipped.
+int common_device(const void* const* ptrs, int n) {
+  const int dev = device_of(ptrs[0]);
+  if (dev < 0) return -1;
+  for (int i = 1; i < n; ++i)
+    if (ptrs[i] != nullptr && device_of(ptrs[i]) != dev) return -1;
+  return dev;
+}
+
+// Raises a kernel's dynamic shared-memory limit once per device.
+template <typename K>
+int allow_smem(K kern, int bytes, std::atomic<unsigned long long>& done, int dev) {
+  const unsigned long long bit = 1ull << dev;
+  if (done.load(std::memory_order_acquire) & bit) return APEX_ATTN_OK;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return APEX_ATTN_ERR_LAUNCH;
+  }
+  done.fetch_or(bit, std::memory_order_release);
+  return APEX_ATTN_OK;
+}
+static_assert(apex::host::kMaxDevices <= 64, "one bit per device");
+
+// ------------------------------------------------------------------ bookkeeping --
+constexpr int kPlanSmem = (3 * apex::kPlanMaxBatch + 1) * (int)sizeof(int);
+std::atomic<unsigned long long> g_plan_smem{0}, g_release_smem{0};
+
+int plan(const apex_attn_kv_plan_args* a, bool release, void* stream) {
+  if (!a || !a->block_table || !a->seq_lens || !a->free_blocks || !a->free_count || !a->seq_lens_out ||
+      !a->free_count_out)
+    return APEX_ATTN_ERR_INVALID_ARGUMENT;
+  if (release ? !a->finished : (!a->new_lens || !a->slots || !a->cu_seqlens || !a->placed))
+    return APEX_ATTN_ERR_INVALID_ARGUMENT;
+  if (a->batch <= 0 || a->table_width <= 0 || a->free_capacity <= 0 || (!release && a->max_new_tokens <= 0))
+    return APEX_ATTN_ERR_INVALID_ARGUMENT;
+  const int shift = block_shift_of(a->block_size);
+  if (shift < 0) return APEX_ATTN_ERR_INVALID_ARGUMENT;
+  if (a->batch > apex::kPlanMaxBatch || (long long)a->table_width * a->block_size > INT_MAX ||
+      a->free_capacity > (1 << 30) || a->max_new_tokens > (1 << 30))
+    return APEX_ATTN_ERR_TOO_LARGE;
+  if (a->table_stride < a->table_width) return APEX_ATTN_ERR_BAD_LAYOUT;
+  const void* ptrs[] = {a->block_table, a->seq_lens,     a->free_blocks, a->free_count,
+                        a->seq_lens_out, a->free_count_out, release ? a->finished : a->new_lens,
+                        release ? nullptr : a->slots, release ? nullptr : a->cu_seqlens,
+                        release ? nullptr : a->placed};
+  for (const void* ptr : ptrs)
+    if (!aligned(ptr, 4)) return APEX_ATTN_ERR_BAD_LAYOUT;
+  if (!release && !aligned(a->slots, 8)) return APEX_ATTN_ERR_BAD_LAYOUT;
+  // The CTAs read all inputs independently of one another's writes.
+  if (a->seq_lens_out == a->seq_lens || a->free_count_out == a->free_count) return APEX_ATTN_ERR_INVALID_ARGUMENT;
+
+  const int dev = common_device(ptrs, 10);
+  if (dev < 0) return APEX_ATTN_ERR_NO_DEVICE;
+  DeviceGuard guard(dev);
+  apex::host::Device d;
+  int rc = apex::host::acquire(dev, &d);
+  if (rc != APEX_ATTN_OK) return rc;
+  rc = release ? allow_smem(apex::kv_release_kernel, kPlanSmem, g_release_smem, dev)
+               : allow_smem(apex::kv_plan_kernel, kPlanSmem, g_plan_smem, dev);
+  if (rc != APEX_ATTN_OK) return rc;
+
+  apex::PlanParams p{};
+  p.block_table = a->block_table;
+  p.table_stride = a->table_stride;
+  p.seq_lens = a->seq_lens;
+  p.new_lens = release ? a->finished : a->new_lens;
+  p.free_blocks = a->free_blocks;
+  p.free_count = a->free_count;
+  p.slots = a->slots;
+  p.cu_seqlens = a->cu_seqlens;
+  p.seq_lens_out = a->seq_lens_out;
+  p.free_count_out = a->free_count_out;
+  p.placed = a->placed;
+  p.batch = a->batch;
+  p.table_width = a->table_width;
+  p.free_capacity = a->free_capacity;
+  p.block_shift = shift;
+  p.max_new = a->max_new_tokens;
+  const int threads = a->batch <= 256 ? 256 : 1024;
+  const long long entries = release ? (long long)a->batch * 4 : std::max(a->max_new_tokens, a->batch);
+  const int grid = (int)std::min<long long>((entries + threads - 1) / threads, d.num_sms);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (release)
+    apex::kv_release_kernel<<<grid, threads, a->batch * (int)sizeof(int), s>>>(p);
+  else
+    apex::kv_plan_kernel<<<grid, threads, (3 * a->batch + 1) * (int)sizeof(int), s>>>(p);
+  return launched();
+}
+
+// ----------------------------------------------------------------------- append --
+int append(const apex_attn_kv_append_args* a, void* stream) {
+  if (!a || !a->k || !a->v || !a->k_cache || !a->v_cache || !a->k_scale || !a->v_scale || !a->slots)
+    return APEX_ATTN_ERR_INVALID_ARGUMENT;
+  if (a->total <= 0 || a->heads_kv <= 0 || a->num_blocks <= 0) return APEX_ATTN_ERR_INVALID_ARGUMENT;
+  const int shift = block_shift_of(a->block_size);
+  if (shift < 0) return APEX_ATTN_ERR_INVALID_ARGUMENT;
+  if (!apex_attn_supports_head_dim(a->head_dim)) return APEX_ATTN_ERR_UNSUPPORTED_HEAD_DIM;
+  if (a->dtype != APEX_ATTN_BF16 && a->dtype != APEX_ATTN_FP16) return APEX_ATTN_ERR_UNSUPPORTED_DTYPE;
+  if (a->total > (1 << 30) || a->heads_kv > 65535) return APEX_ATTN_ERR_TOO_LARGE;
+  for (int i = 0; i < 4; ++i)
+    if (a->strides[i] < 0 || (a->strides[i] & 7) != 0 || a->strides[i] >= (1LL << 38)) return APEX_ATTN_ERR_BAD_LAYOUT;
+  for (int i = 4; i < 10; ++i)
+    if (a->strides[i] < 0 || (a->strides[i] & 15) != 0 || a->strides[i] >= (1LL << 38)) return APEX_ATTN_ERR_BAD_LAYOUT;
+  if (a->strides[6] < a->head_dim || a->strides[9] < a->head_dim) return APEX_ATTN_ERR_BAD_LAYOUT;
+  if (!aligned16(a->k) || !aligned16(a->v) || !aligned16(a->k_cache) || !aligned16(a->v_cache) ||
+      !aligned(a->k_scale, 4) || !aligned(a->v_scale, 4) || !aligned(a->slots, 8))
+    return APEX_ATTN_ERR_BAD_LAYOUT;
+
+  const void* ptrs[] = {a->k, a->v, a->k_cache, a->v_cache, a->k_scale, a->v_scale, a->slots};
+  const int dev = common_device(ptrs, 7);
+  if (dev < 0) return APEX_ATTN_ERR_NO_DEVICE;
+  DeviceGuard guard(dev);
+  apex::host::Device d;
+  int rc = apex::host::acquire(dev, &d);
+  if (rc != APEX_ATTN_OK) return rc;
+
+  apex::AppendParams p{};
+  p.x[0] = a->k;
+  p.x[1] = a->v;
+  p.codes[0] = static_cast<unsigned char*>(a->k_cache);
+  p.codes[1] = static_cast<unsigned char*>(a->v_cache);
+  p.scale[0] = a->k_scale;
+  p.scale[1] = a->v_scale;
+  p.slots = a->slots;
+  for (int i = 0; i < 2; ++i) {
+    p.x_st[i] = a->strides[2 * i];
+    p.x_sh[i] = a->strides[2 * i + 1];
+    p.c_sb[i] = a->strides[4 + 3 * i];
+    p.c_sh[i] = a->strides[5 + 3 * i];
+    p.c_st[i] = a->strides[6 + 3 * i];
+  }
+  p.num_slots = (long long)a->num_blocks * a->block_size;
+  p.total = a->total;
+  p.heads = a->heads_kv;
+  p.head_dim = a->head_dim;
+  p.block_shift = shift;
+  // One token per CTA while all CTAs fit the device at once (decode: every token is a run of
+  // its own); longer windows, up to the smallest block, once there are more.
+  const long long ctas = 2LL * a->heads_kv * a->total;
+  p.window = (int)std::max(1LL, std::min(16LL, ctas / (16LL * d.num_sms)));
+  const dim3 grid((unsigned)((a->total + p.window - 1) / p.window), (unsigned)a->heads_kv, 2);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (a->dtype == APEX_ATTN_BF16)
+    apex::kv_append_kernel<__nv_bfloat16><<<grid, apex::kAppendThreads, 0, s>>>(p);
+  else
+    apex::kv_append_kernel<__half><<<grid, apex::kAppendThreads, 0, s>>>(p);
+  return launched();
+}
+
+// -------------------------------------------------------------------- attention --
+size_t workspace_bytes(int heads_q, int heads_kv, int max_seqlen_q, int head_dim) {
+  if (heads_q <= 0 || heads_kv <= 0 || max_seqlen_q <= 0 || head_dim <= 0) return 0;
+  return 16;
+}
+
+template <typename T>
+int launch_simple(const apex::PagedParams& p, int head_dim, cudaStream_t s) {
+  const dim3 grid((unsigned)p.max_q, (unsigned)p.heads_q, (unsigned)p.batch);
+  switch (head_dim) {
+    case 64: apex::attn_paged_simple_kernel<T, 64><<<grid, 128, 0, s>>>(p); break;
+    case 128: apex::attn_paged_simple_kernel<T, 128><<<grid, 128, 0, s>>>(p); break;
+    default: apex::attn_paged_simple_kernel<T, 256><<<grid, 128, 0, s>>>(p);
+  }
+  return launched();
+}
+
+int forward_paged(const apex_attn_paged_args* a, void* workspace, size_t bytes, void* stream) {
+  // ---- argument validation (no CUDA calls) ----
+  if (!a || !a->q || !a->k_cache || !a->v_cache || !a->k_scale || !a->v_scale || !a->block_table || !a->seq_lens ||
+      !a->o || !workspace)
+    return APEX_ATTN_ERR_INVALID_ARGUMENT;
+  if (a->batch <= 0 || a->heads_q <= 0 || a->heads_kv <= 0 || a->heads_q % a->heads_kv != 0 || a->total_q <= 0 ||
+      a->max_seqlen_q <= 0 || a->num_blocks <= 0 || a->table_width <= 0)
+    return APEX_ATTN_ERR_INVALID_ARGUMENT;
+  if (!a->cu_seqlens_q && (a->total_q % a->batch != 0 || a->total_q / a->batch != a->max_seqlen_q))
+    return APEX_ATTN_ERR_INVALID_ARGUMENT;
+  if (a->window_left < -1 || (a->window_left >= 0 && !a->causal)) return APEX_ATTN_ERR_INVALID_ARGUMENT;
+  const int shift = block_shift_of(a->block_size);
+  if (shift < 0) return APEX_ATTN_ERR_INVALID_ARGUMENT;
+  if (!apex_attn_supports_head_dim(a->head_dim)) return APEX_ATTN_ERR_UNSUPPORTED_HEAD_DIM;
+  if (a->dtype != APEX_ATTN_BF16 && a->dtype != APEX_ATTN_FP16) return APEX_ATTN_ERR_UNSUPPORTED_DTYPE;
+  if (!std::isfinite(a->sm_scale) || !(a->sm_scale > 0.f)) return APEX_ATTN_ERR_BAD_SCALE;
+  if (a->total_q > (1 << 30) || a->batch > 65535 || a->heads_q > 65535 ||
+      (long long)a->max_seqlen_q * a->heads_q > (1 << 30) || (long long)a->table_width * a->block_size > (1 << 30))
+    return APEX_ATTN_ERR_TOO_LARGE;
+  for (int i = 0; i < 4; ++i)
+    if (a->strides[i] < 0 || (a->strides[i] & 7) != 0 || a->strides[i] >= (1LL << 38)) return APEX_ATTN_ERR_BAD_LAYOUT;
+  for (int i = 4; i < 10; ++i)
+    if (a->strides[i] < 0 || (a->strides[i] & 15) != 0 || a->strides[i] >= (1LL << 38)) return APEX_ATTN_ERR_BAD_LAYOUT;
+  if (a->strides[1] < a->head_dim || a->strides[3] < a->head_dim || a->strides[6] < a->head_dim ||
+      a->strides[9] < a->head_dim || a->table_stride < a->table_width)
+    return APEX_ATTN_ERR_BAD_LAYOUT;
+  if (!aligned16(a->q) || !aligned16(a->k_cache) || !aligned16(a->v_cache) || !aligned16(a->o) || !aligned16(workspace))
+    return APEX_ATTN_ERR_BAD_LAYOUT;
+  if (!aligned(a->k_scale, 4) || !aligned(a->v_scale, 4) || !aligned(a->block_table, 4) || !aligned(a->seq_lens, 4) ||
+      !aligned(a->cu_seqlens_q, 4) || !aligned(a->lse, 4))
+    return APEX_ATTN_ERR_BAD_LAYOUT;
+  if (bytes < workspace_bytes(a->heads_q, a->heads_kv, a->max_seqlen_q, a->head_dim))
+    return APEX_ATTN_ERR_INVALID_ARGUMENT;
+
+  // ---- device ----
+  const void* ptrs[] = {a->q,           a->k_cache,  a->v_cache,      a->k_scale, a->v_scale,
+                        a->block_table, a->seq_lens, a->cu_seqlens_q, a->o,       a->lse, workspace};
+  const int dev = common_device(ptrs, 11);
+  if (dev < 0) return APEX_ATTN_ERR_NO_DEVICE;
+  DeviceGuard guard(dev);
+  apex::host::Device d;
+  int rc = apex::host::acquire(dev, &d);
+  if (rc != APEX_ATTN_OK) return rc;
+
+  apex::PagedParams p{};
+  p.q = a->q;
+  p.o = a->o;
+  p.lse = a->lse;
+  p.k_codes = static_cast<const unsigned char*>(a->k_cache);
+  p.v_codes = static_cast<const unsigned char*>(a->v_cache);
+  p.k_scale = a->k_scale;
+  p.v_scale = a->v_scale;
+  p.block_table = a->block_table;
+  p.seq_lens = a->seq_lens;
+  p.cu_seqlens_q = a->cu_seqlens_q;
+  p.table_stride = a->table_stride;
+  p.q_st = a->strides[0];
+  p.q_sh = a->strides[1];
+  p.o_st = a->strides[2];
+  p.o_sh = a->strides[3];
+  p.k_sb = a->strides[4];
+  p.k_sh = a->strides[5];
+  p.k_st = a->strides[6];
+  p.v_sb = a->strides[7];
+  p.v_sh = a->strides[8];
+  p.v_st = a->strides[9];
+  p.batch = a->batch;
+  p.heads_q = a->heads_q;
+  p.heads_kv = a->heads_kv;
+  p.group = a->heads_q / a->heads_kv;
+  p.total_q = a->total_q;
+  p.max_q = a->max_seqlen_q;
+  p.num_blocks = a->num_blocks;
+  p.block_shift = shift;
+  p.table_width = a->table_width;
+  p.causal = a->causal ? 1 : 0;
+  p.window = a->window_left;
+  p.zero_rest = a->zero_rest ? 1 : 0;
+  p.scale_log2 = a->sm_scale * 1.4426950408889634f;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return a->dtype == APEX_ATTN_BF16 ? launch_simple<__nv_bfloat16>(p, a->head_dim, s)
+                                    : launch_simple<__half>(p, a->head_dim, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int apex_attn_kv_plan(const apex_attn_kv_plan_args* args, void* stream) { return plan(args, false, stream); }
+
+int apex_attn_kv_release(const apex_attn_kv_plan_args* args, void* stream) { return plan(args, true, stream); }
+
+int apex_attn_kv_append(const apex_attn_kv_append_args* args, void* stream) { return append(args, stream); }
+
+size_t apex_attn_fwd_paged_workspace_bytes(int heads_q, int heads_kv, int max_seqlen_q, int head_dim) {
+  return workspace_bytes(heads_q, heads_kv, max_seqlen_q, head_dim);
+}
+
+int apex_attn_fwd_paged(const apex_attn_paged_args* args, void* workspace, size_t workspace_bytes, void* stream) {
+  return forward_paged(args, workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

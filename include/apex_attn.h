@@ -343,6 +343,149 @@ int apex_attn_bwd_varlen(const apex_attn_bwd_varlen_args* args, void* workspace,
 int apex_attn_bwd_varlen_mode(const apex_attn_bwd_varlen_args* args, int mode, void* workspace,
                               size_t workspace_bytes, void* stream);
 
+/*
+ * A paged K/V cache held in 8 bits, and attention over it (serving).
+ *
+ * The cache is a pool of blocks of `block_size` tokens (16, 32, 64 or 128). K and V are e4m3
+ * codes, logically [num_blocks, heads_kv, block_size, D], each with one fp32 scale per (block,
+ * K/V head), contiguous [num_blocks, heads_kv]; a cached value is code * scale. Request b's
+ * token at position t is row t % block_size of block block_table[b][t / block_size], that is
+ * slot block * block_size + t % block_size. Strides are (block, head, token) byte strides,
+ * multiples of 16, with unit stride along D, so storage of [num_blocks, block_size, heads_kv,
+ * D] needs no copy. A block belongs to one request. Nothing here synchronises or takes a
+ * length from the host, so a step of plan, append and attention can be captured into a graph.
+ * No counterpart in the reference.
+ *
+ * apex_attn_kv_plan: one scheduling step. Request b holds seq_lens[b] tokens and brings
+ * new_lens[b] more (negative counts as 0). Blocks for them come off the top of the stack
+ * free_blocks[0 .. *free_count), in request order, and their ids go into the request's table
+ * row after the ones it holds. Written: block_table (those entries only), slots [max_new_tokens]
+ * (the slot of each new token, requests one after another; -1 past the last), cu_seqlens
+ * [batch + 1] (offsets of the requests' new tokens), seq_lens_out [batch], *free_count_out
+ * (free_blocks itself is not changed), and placed [batch]. A request that the stack, its table
+ * row (table_width entries) or the slot array has no room for is not placed: 0 in placed, -1 in
+ * its slots, its length as it was, no block taken; a later request that needs no block can
+ * still be placed. batch at most 8192.
+ *
+ * apex_attn_kv_release: finished [batch]; the blocks of each request with a non-zero entry are
+ * pushed on the stack (free_blocks from *free_count on, in request order; at most
+ * free_capacity entries), its length becomes 0, its table row stays as it is.
+ * new_lens, slots, cu_seqlens, placed and max_new_tokens are not read.
+ *
+ * Both: seq_lens_out and free_count_out must not be the input buffers
+ * (APEX_ATTN_ERR_INVALID_ARGUMENT) nor overlap them.
+ */
+typedef struct apex_attn_kv_plan_args {
+  int* block_table;
+  const int* seq_lens;
+  const int* new_lens;
+  const int* finished;
+  int* free_blocks;
+  const int* free_count;
+  long long* slots;
+  int* cu_seqlens;
+  int* seq_lens_out;
+  int* free_count_out;
+  int* placed;
+  long long table_stride; /* row stride of block_table, in entries */
+  int batch;
+  int table_width;
+  int free_capacity;
+  int block_size;
+  int max_new_tokens;
+} apex_attn_kv_plan_args;
+
+int apex_attn_kv_plan(const apex_attn_kv_plan_args* args, void* stream);
+int apex_attn_kv_release(const apex_attn_kv_plan_args* args, void* stream);
+
+/*
+ * Quantises new tokens k, v [total, heads_kv, D] (bf16 or fp16) into their slots of the cache.
+ * Tokens with consecutive slots inside one block are a run. Its scale (per head, K and V apart)
+ * is the smallest power of two 2^e, e >= -100, with max |x| <= 448 * 2^e over the run; a run
+ * that starts inside a block keeps the block's tokens before it, so its scale is at least the
+ * block's old one, and where the scale grows their codes are divided by the growth (exact
+ * but for codes that leave e4m3's normal range). Codes are x / scale rounded to nearest even.
+ * Values that are not finite do not count for the scale and are stored as NaN. Slots
+ * outside [0, num_blocks * block_size) are skipped; rows of the block after the run stay as
+ * they were. At most one run may go to a block in one call (what apex_attn_kv_plan gives).
+ *
+ * strides: k token, head; v token, head (elements, multiples of 8); k_cache block, head,
+ * token; v_cache block, head, token (bytes, multiples of 16). Pointers 16-byte aligned.
+ */
+typedef struct apex_attn_kv_append_args {
+  const void* k;
+  const void* v;
+  void* k_cache;
+  void* v_cache;
+  float* k_scale;
+  float* v_scale;
+  const long long* slots;
+  int total;
+  int heads_kv;
+  int head_dim;
+  int dtype;
+  int num_blocks;
+  int block_size;
+  long long strides[10];
+} apex_attn_kv_append_args;
+
+int apex_attn_kv_append(const apex_attn_kv_append_args* args, void* stream);
+
+/*
+ * Attention of new query tokens over the cache.
+ *   q, o          [total_q, heads_q, D], bf16 or fp16; query head h reads K/V head
+ *                 h / (heads_q / heads_kv)
+ *   cu_seqlens_q  device int32 [batch + 1], offsets of the requests' query rows as for
+ *                 apex_attn_fwd_varlen; null: total_q / batch = max_seqlen_q rows each
+ *   seq_lens      device int32 [batch]: cached tokens of each request, the query tokens' own
+ *                 among them (append first). Clamped to [0, table_width * block_size].
+ *   causal        query row i of n stands at position seq_len - n + i and sees positions up to
+ *                 its own; 0: every cached token
+ *   window_left   -1: no window. >= 0 (causal only): from its own position - window_left on
+ *   lse           nullable, fp32 [heads_q, total_q], natural logarithm
+ *   zero_rest     non-zero: rows of o (and lse) outside every request are set to zero;
+ *                 0: they are not written
+ *   strides       q token, head; o token, head (elements, multiples of 8); k_cache block, head,
+ *                 token; v_cache block, head, token (bytes, multiples of 16)
+ * A row that sees nothing (an empty request, a position before the cache) gives o = 0 and
+ * lse = -infinity. Table entries outside [0, num_blocks) read as zeros; entries of blocks that
+ * no row of a request sees are not read, and what the cache holds there or behind the last
+ * token (NaN codes too) does not matter. Scores, softmax statistics and sums are fp32.
+ * workspace: device memory of at least apex_attn_fwd_paged_workspace_bytes(...) bytes, 16-byte
+ * aligned, used only during the call; calls that can overlap need one each.
+ */
+typedef struct apex_attn_paged_args {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  const float* k_scale;
+  const float* v_scale;
+  const int* block_table;
+  const int* seq_lens;
+  const int* cu_seqlens_q;
+  void* o;
+  float* lse;
+  long long table_stride; /* row stride of block_table, in entries */
+  long long strides[10];
+  int batch;
+  int heads_q;
+  int heads_kv;
+  int total_q;
+  int max_seqlen_q;
+  int head_dim;
+  int dtype;
+  int num_blocks;
+  int block_size;
+  int table_width;
+  int causal;
+  int window_left;
+  int zero_rest;
+  float sm_scale;
+} apex_attn_paged_args;
+
+size_t apex_attn_fwd_paged_workspace_bytes(int heads_q, int heads_kv, int max_seqlen_q, int head_dim);
+int apex_attn_fwd_paged(const apex_attn_paged_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Number of SMs of `device` (the persistent kernels' grid is min(work items, this)), or a
  * negative status: APEX_ATTN_ERR_NO_DEVICE for a bad ordinal or no device,
  * APEX_ATTN_ERR_UNSUPPORTED_ARCH if it is not sm_100. Lets a caller size its own batching
