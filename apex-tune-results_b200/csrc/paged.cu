@@ -184,20 +184,101 @@ int append(const apex_attn_kv_append_args* a, void* stream) {
 }
 
 // -------------------------------------------------------------------- attention --
+constexpr int kMaxSms = 160;  // the workspace holds what this many SMs' CTAs may write
+
+// Query rows per tile: the smallest tile that holds all rows of a request's K/V head, else the
+// largest. d = 256 stops at 64 rows (shared memory).
+int query_tile(int rows, int head_dim) {
+  if (rows <= 16) return 16;
+  if (rows <= 32) return 32;
+  return rows <= 64 || head_dim == 256 ? 64 : 128;
+}
+
+struct Workspace {
+  size_t share, lse, o, bytes;  // offsets and size
+};
+
+Workspace workspace_plan(int query_rows, int head_dim) {
+  const size_t parts = 2 * 2 * kMaxSms;  // two per CTA, at most two CTAs per SM
+  Workspace w;
+  w.share = 0;
+  w.lse = parts * apex::kShareInts * sizeof(int);
+  w.o = w.lse + parts * query_rows * sizeof(float);
+  w.bytes = w.o + parts * query_rows * head_dim * sizeof(float);
+  return w;
+}
+
 size_t workspace_bytes(int heads_q, int heads_kv, int max_seqlen_q, int head_dim) {
   if (heads_q <= 0 || heads_kv <= 0 || max_seqlen_q <= 0 || head_dim <= 0) return 0;
-  return 16;
+  const long long rows = (long long)((heads_q + heads_kv - 1) / heads_kv) * max_seqlen_q;
+  return workspace_plan(query_tile((int)std::min(rows, 1LL << 30), head_dim), head_dim).bytes;
+}
+
+// 4-D map over the cache [num_blocks, H_kv, block, D], dims ordered (D, block, H_kv, blocks); a
+// box is one block of one head, up to 128 columns, swizzled by its row size.
+int encode_cache(CUtensorMap* m, const void* ptr, const apex_attn_paged_args& a, const long long* st) {
+  const cuuint64_t sh = a.heads_kv > 1 ? st[1] : (cuuint64_t)a.block_size * st[2];
+  const cuuint64_t sb = a.num_blocks > 1 ? st[0] : (cuuint64_t)a.heads_kv * sh;
+  const cuuint64_t dims[4] = {(cuuint64_t)a.head_dim, (cuuint64_t)a.block_size, (cuuint64_t)a.heads_kv,
+                              (cuuint64_t)a.num_blocks};
+  const cuuint64_t strides[3] = {(cuuint64_t)st[2], sh, sb};
+  const cuuint32_t box[4] = {(cuuint32_t)std::min(a.head_dim, 128), (cuuint32_t)a.block_size, 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = apex::host::tensor_map_encoder()(
+      m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(ptr), dims, strides, box, estr,
+      CU_TENSOR_MAP_INTERLEAVE_NONE, a.head_dim >= 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? APEX_ATTN_OK : APEX_ATTN_ERR_TENSOR_MAP;
+}
+
+template <typename T, int D, int NQ>
+int launch_paged(const apex::PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, int dev, int num_sms,
+                 cudaStream_t s) {
+  using C = apex::PagedCfg<T, D, NQ>;
+  static std::atomic<unsigned long long> done{0};
+  const int rc = allow_smem(apex::attn_paged_kernel<T, D, NQ>, C::kBytes, done, dev);
+  if (rc != APEX_ATTN_OK) return rc;
+  const int grid = C::kCtas * std::min(num_sms, kMaxSms);
+  apex::attn_paged_kernel<T, D, NQ><<<grid, C::kThreads, C::kBytes, s>>>(mk, mv, p);
+  if (launched() != APEX_ATTN_OK) return APEX_ATTN_ERR_LAUNCH;
+  // The join may be set up while the last CTAs of the kernel before it run.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(apex::kCombineThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, apex::attn_paged_combine_kernel<T, D, NQ>, p) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return APEX_ATTN_ERR_LAUNCH;
+  }
+  return APEX_ATTN_OK;
+}
+
+template <typename T, int D>
+int launch_tile(int tile, const apex::PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, int dev,
+                int num_sms, cudaStream_t s) {
+  switch (tile) {
+    case 16: return launch_paged<T, D, 16>(p, mk, mv, dev, num_sms, s);
+    case 32: return launch_paged<T, D, 32>(p, mk, mv, dev, num_sms, s);
+    case 64: return launch_paged<T, D, 64>(p, mk, mv, dev, num_sms, s);
+    default:
+      if constexpr (D <= 128) return launch_paged<T, D, 128>(p, mk, mv, dev, num_sms, s);
+      return APEX_ATTN_ERR_INVALID_ARGUMENT;
+  }
 }
 
 template <typename T>
-int launch_simple(const apex::PagedParams& p, int head_dim, cudaStream_t s) {
-  const dim3 grid((unsigned)p.max_q, (unsigned)p.heads_q, (unsigned)p.batch);
+int launch_dim(int head_dim, int tile, const apex::PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv,
+               int dev, int num_sms, cudaStream_t s) {
   switch (head_dim) {
-    case 64: apex::attn_paged_simple_kernel<T, 64><<<grid, 128, 0, s>>>(p); break;
-    case 128: apex::attn_paged_simple_kernel<T, 128><<<grid, 128, 0, s>>>(p); break;
-    default: apex::attn_paged_simple_kernel<T, 256><<<grid, 128, 0, s>>>(p);
+    case 64: return launch_tile<T, 64>(tile, p, mk, mv, dev, num_sms, s);
+    case 128: return launch_tile<T, 128>(tile, p, mk, mv, dev, num_sms, s);
+    default: return launch_tile<T, 256>(tile, p, mk, mv, dev, num_sms, s);
   }
-  return launched();
 }
 
 int forward_paged(const apex_attn_paged_args* a, void* workspace, size_t bytes, void* stream) {
@@ -244,44 +325,51 @@ int forward_paged(const apex_attn_paged_args* a, void* workspace, size_t bytes, 
   int rc = apex::host::acquire(dev, &d);
   if (rc != APEX_ATTN_OK) return rc;
 
+  const long long* st = a->strides;
+  CUtensorMap mk, mv;
+  if ((rc = encode_cache(&mk, a->k_cache, *a, st + 4)) || (rc = encode_cache(&mv, a->v_cache, *a, st + 7))) return rc;
+
+  const int group = a->heads_q / a->heads_kv;
+  const int tile = query_tile(group * a->max_seqlen_q, a->head_dim);
+  const Workspace w = workspace_plan(tile, a->head_dim);
+  char* ws = static_cast<char*>(workspace);
   apex::PagedParams p{};
   p.q = a->q;
   p.o = a->o;
   p.lse = a->lse;
-  p.k_codes = static_cast<const unsigned char*>(a->k_cache);
-  p.v_codes = static_cast<const unsigned char*>(a->v_cache);
   p.k_scale = a->k_scale;
   p.v_scale = a->v_scale;
   p.block_table = a->block_table;
   p.seq_lens = a->seq_lens;
   p.cu_seqlens_q = a->cu_seqlens_q;
+  p.share = reinterpret_cast<int*>(ws + w.share);
+  p.part_lse = reinterpret_cast<float*>(ws + w.lse);
+  p.part_o = reinterpret_cast<float*>(ws + w.o);
+  p.status = d.status;
+  p.host_flag = d.host_flag_dev;
+  p.timeout_ns = apex::host::wait_timeout_ns();
   p.table_stride = a->table_stride;
-  p.q_st = a->strides[0];
-  p.q_sh = a->strides[1];
-  p.o_st = a->strides[2];
-  p.o_sh = a->strides[3];
-  p.k_sb = a->strides[4];
-  p.k_sh = a->strides[5];
-  p.k_st = a->strides[6];
-  p.v_sb = a->strides[7];
-  p.v_sh = a->strides[8];
-  p.v_st = a->strides[9];
+  p.q_st = st[0];
+  p.q_sh = st[1];
+  p.o_st = st[2];
+  p.o_sh = st[3];
   p.batch = a->batch;
-  p.heads_q = a->heads_q;
   p.heads_kv = a->heads_kv;
-  p.group = a->heads_q / a->heads_kv;
+  p.group = group;
   p.total_q = a->total_q;
   p.max_q = a->max_seqlen_q;
   p.num_blocks = a->num_blocks;
   p.block_shift = shift;
   p.table_width = a->table_width;
   p.causal = a->causal ? 1 : 0;
-  p.window = a->window_left;
-  p.zero_rest = a->zero_rest ? 1 : 0;
+  // A window that reaches past every table hides nothing.
+  p.window = a->window_left < a->table_width * a->block_size ? a->window_left : -1;
+  p.zero_rest = a->zero_rest && a->cu_seqlens_q ? 1 : 0;
+  p.stream_once = group * a->max_seqlen_q <= tile ? 1 : 0;
   p.scale_log2 = a->sm_scale * 1.4426950408889634f;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return a->dtype == APEX_ATTN_BF16 ? launch_simple<__nv_bfloat16>(p, a->head_dim, s)
-                                    : launch_simple<__half>(p, a->head_dim, s);
+  return a->dtype == APEX_ATTN_BF16 ? launch_dim<__nv_bfloat16>(a->head_dim, tile, p, mk, mv, dev, d.num_sms, s)
+                                    : launch_dim<__half>(a->head_dim, tile, p, mk, mv, dev, d.num_sms, s);
 }
 
 }  // namespace

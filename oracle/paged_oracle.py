@@ -93,8 +93,8 @@ def attend(q, k_codes, v_codes, k_scale, v_scale, table, lens, cu, block, causal
     bounds on what the kernels' documented roundings may move them by (before o is rounded
     to its type):
 
-    * a weight p * v_scale is held in two e4m3 terms: 2^-8 of itself (half a step of four
-      bits, twice) plus 2^-16 of the row's largest (e4m3's spacing 2^-9 below 2^-6, halved, with
+    * a weight p * v_scale is rounded to fp16 (2^-12 covers half a step of 11 bits) and held in
+      two e4m3 terms: 2^-8 of itself (half a step of four bits, twice) plus 2^-16 of the row's largest (e4m3's spacing 2^-9 below 2^-6, halved, with
       the largest at 2^6);
     * a query value in two terms (three for fp16): exact, or off by 2^-10 / 224 of the largest
       of the tile's, taken here as the largest of the request's rows;
@@ -132,6 +132,6 @@ def attend(q, k_codes, v_codes, k_scale, v_scale, table, lens, cu, block, causal
                 off = off.max().item() + 2.0 ** -20 * (1 + abs(lse[h, r].item()))
                 lse_bound[h, r] = off
                 mass = p @ v.abs()
-                o_bound[r, h] = mass * (2.0 ** -8 + 2 * off + 2.0 ** -19) \
+                o_bound[r, h] = mass * (2.0 ** -8 + 2.0 ** -12 + 2 * off + 2.0 ** -19) \
                     + 2.0 ** -16 * (p * vs[lo:hi]).max() * vc[lo:hi].abs().sum(0)
     return o, lse, o_bound, lse_bound
