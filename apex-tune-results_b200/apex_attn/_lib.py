@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 LIB_NAME = "libapex_attn.so"
@@ -81,14 +82,15 @@ class KVPlanArgs(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in (
         "block_table", "seq_lens", "new_lens", "finished", "free_blocks", "free_count", "slots", "cu_seqlens",
         "seq_lens_out", "free_count_out", "placed")] + [("table_stride", ctypes.c_longlong)] + [
-        (n, ctypes.c_int) for n in ("batch", "table_width", "free_capacity", "block_size", "max_new_tokens")]
+        (n, ctypes.c_int) for n in ("batch", "table_width", "free_capacity", "block_size", "max_new_tokens",
+                                    "known_device")]
 
 
 class KVAppendArgs(ctypes.Structure):
     """Mirror of apex_attn_kv_append_args (include/apex_attn.h)."""
     _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_cache", "v_cache", "k_scale", "v_scale", "slots")] + [
         (n, ctypes.c_int) for n in ("total", "heads_kv", "head_dim", "dtype", "num_blocks", "block_size")] + [
-        ("strides", ctypes.c_longlong * 10)]
+        ("strides", ctypes.c_longlong * 10), ("known_device", ctypes.c_int)]
 
 
 class PagedArgs(ctypes.Structure):
@@ -98,7 +100,15 @@ class PagedArgs(ctypes.Structure):
         ("table_stride", ctypes.c_longlong), ("strides", ctypes.c_longlong * 10)] + [
         (n, ctypes.c_int) for n in (
             "batch", "heads_q", "heads_kv", "total_q", "max_seqlen_q", "head_dim", "dtype", "num_blocks",
-            "block_size", "table_width", "causal", "window_left", "zero_rest")] + [("sm_scale", ctypes.c_float)]
+            "block_size", "table_width", "causal", "window_left", "zero_rest")] + [("sm_scale", ctypes.c_float),
+                                                                             ("known_device", ctypes.c_int)]
+
+
+# The same structs as struct.Struct layouts: packing one takes the host a fifth of the time that
+# filling a ctypes.Structure does. Pointers are unsigned 64-bit, null is 0.
+KV_PLAN_ARGS = struct.Struct("@11Qq6i")
+KV_APPEND_ARGS = struct.Struct("@7Q6i10qi")
+PAGED_ARGS = struct.Struct("@10Qq10q13ifi")
 
 
 # Every symbol the header declares: (name, restype, argtypes).
@@ -129,11 +139,11 @@ SYMBOLS = {
                                           ctypes.c_size_t, ctypes.c_void_p]),
     "apex_attn_bwd_varlen_mode": (ctypes.c_int, [ctypes.POINTER(BwdVarlenArgs), ctypes.c_int,
                                                  ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
-    "apex_attn_kv_plan": (ctypes.c_int, [ctypes.POINTER(KVPlanArgs), ctypes.c_void_p]),
-    "apex_attn_kv_release": (ctypes.c_int, [ctypes.POINTER(KVPlanArgs), ctypes.c_void_p]),
-    "apex_attn_kv_append": (ctypes.c_int, [ctypes.POINTER(KVAppendArgs), ctypes.c_void_p]),
+    "apex_attn_kv_plan": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "apex_attn_kv_release": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "apex_attn_kv_append": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "apex_attn_fwd_paged_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 4),
-    "apex_attn_fwd_paged": (ctypes.c_int, [ctypes.POINTER(PagedArgs), ctypes.c_void_p, ctypes.c_size_t,
+    "apex_attn_fwd_paged": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
                                            ctypes.c_void_p]),
     "apex_attn_num_sms_hint": (ctypes.c_int, [ctypes.c_int]),
     "apex_attn_set_forward_kernel": (ctypes.c_int, [ctypes.c_int]),

@@ -23,7 +23,7 @@ status text otherwise.
 """
 from __future__ import annotations
 
-import ctypes
+import functools
 import math
 from typing import NamedTuple
 
@@ -33,8 +33,17 @@ from . import _lib
 from .ops import _DTYPES
 
 _E4M3 = torch.float8_e4m3fn
+_INT32 = torch.int32
 _HEAD_DIMS = (64, 128, 256)
 _BLOCK_SIZES = (16, 32, 64, 128)
+
+# A decode step's kernels are short, so the host's share counts: these functions ask each tensor
+# for a property once and pack the arguments in one go.
+try:
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+except AttributeError:  # a build of torch without CUDA, or one that names it otherwise
+    def _raw_stream(device):
+        return torch.cuda.current_stream(device).cuda_stream
 
 
 class KVCachePlan(NamedTuple):
@@ -47,36 +56,46 @@ class KVCachePlan(NamedTuple):
 
 
 def _int32(t, name, numel, device):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != numel or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor of {numel} values on {device}, got {t.dtype} "
-                         f"{tuple(t.shape)} on {t.device}")
+    """The address of a contiguous int32 vector."""
+    if t.dtype is not _INT32 or t.shape != (numel,) or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {numel} values on the CUDA device {device}, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
 
 
 def _table(block_table):
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
-        raise ValueError(f"block_table must be int32 [batch, width] with unit stride along a row, got "
-                         f"{block_table.dtype} {tuple(block_table.shape)}")
-    if not block_table.is_cuda:
-        raise ValueError("block_table must be a CUDA tensor")
+    """(batch, width, row stride) of a block table."""
+    if block_table.dtype is not _INT32 or block_table.dim() != 2:
+        raise ValueError(f"block_table must be int32 [batch, width], got {block_table.dtype} "
+                         f"{tuple(block_table.shape)}")
     batch, width = block_table.shape
-    return batch, width, max(block_table.stride(0), width) if batch > 1 else width
+    row, unit = block_table.stride()
+    if width > 1 and unit != 1 or batch > 1 and row < width:
+        raise ValueError("block_table needs unit stride along its rows, and rows that do not overlap")
+    return batch, width, row if batch > 1 else width
 
 
-def _bookkeeping(block_table, seq_lens, free_blocks, free_count, block_size):
+def _bookkeeping(call, name, block_table, seq_lens, new_lens, finished, free_blocks, free_count, block_size,
+                 slots, cu_at, lens_at, count_at, placed_at, max_new):
+    """Checks what plan and release share and runs `call`, writing to the given addresses."""
+    device = block_table.get_device()
+    if device < 0:
+        raise ValueError("block_table must be a CUDA tensor")
     batch, width, stride = _table(block_table)
-    device = block_table.device
-    _int32(seq_lens, "seq_lens", batch, device)
-    _int32(free_count, "free_count", 1, device)
-    _int32(free_blocks, "free_blocks", free_blocks.numel(), device)
+    if batch == 0 or width == 0:
+        raise ValueError(f"block_table has no entries: {tuple(block_table.shape)}")
     if block_size not in _BLOCK_SIZES:
         raise ValueError(f"block_size must be one of {_BLOCK_SIZES}, got {block_size}")
-    out = torch.empty(batch + 1, dtype=torch.int32, device=device)  # lengths, then the count
-    args = _lib.KVPlanArgs(block_table=block_table.data_ptr(), seq_lens=seq_lens.data_ptr(),
-                           free_blocks=free_blocks.data_ptr(), free_count=free_count.data_ptr(),
-                           seq_lens_out=out.data_ptr(), free_count_out=out.data_ptr() + 4 * batch,
-                           table_stride=stride, batch=batch, table_width=width,
-                           free_capacity=free_blocks.numel(), block_size=block_size)
-    return args, out, batch, device
+    capacity = free_blocks.numel()
+    args = _lib.KV_PLAN_ARGS.pack(
+        block_table.data_ptr(), _int32(seq_lens, "seq_lens", batch, device),
+        0 if new_lens is None else _int32(new_lens, "new_lens", batch, device),
+        0 if finished is None else _int32(finished, "finished", batch, device),
+        _int32(free_blocks, "free_blocks", capacity, device), _int32(free_count, "free_count", 1, device), slots,
+        cu_at, lens_at, count_at, placed_at, stride, batch, width, capacity, block_size, max_new, device + 1)
+    rc = call(args, _raw_stream(device))
+    if rc:
+        _lib.check(rc, name)
 
 
 def kv_cache_plan(block_table, seq_lens, new_lens, free_blocks, free_count, block_size,
@@ -96,20 +115,18 @@ def kv_cache_plan(block_table, seq_lens, new_lens, free_blocks, free_count, bloc
       array had no room for. It takes no block, keeps its length, and its slots are -1.
 
     At most 8192 requests. Asynchronous on the current CUDA stream of the table's device."""
-    args, out, batch, device = _bookkeeping(block_table, seq_lens, free_blocks, free_count, block_size)
-    _int32(new_lens, "new_lens", batch, device)
     if max_new_tokens < 1:
         raise ValueError("max_new_tokens must be positive")
-    slots = torch.empty(max_new_tokens, dtype=torch.int64, device=device)
-    more = torch.empty(2 * batch + 1, dtype=torch.int32, device=device)
-    args.new_lens = new_lens.data_ptr()
-    args.slots = slots.data_ptr()
-    args.cu_seqlens = more.data_ptr()
-    args.placed = more.data_ptr() + 4 * (batch + 1)
-    args.max_new_tokens = max_new_tokens
-    stream = torch.cuda.current_stream(device).cuda_stream
-    _lib.check(_lib.load().apex_attn_kv_plan(ctypes.byref(args), stream), "kv_cache_plan")
-    return KVCachePlan(slots, more[:batch + 1], out[:batch], out[batch:], more[batch + 1:])
+    batch = seq_lens.numel()
+    where = block_table.device
+    slots = torch.empty(max_new_tokens, dtype=torch.int64, device=where)
+    out = torch.empty(3 * batch + 2, dtype=_INT32, device=where)
+    at = out.data_ptr()
+    _bookkeeping(_lib.load().apex_attn_kv_plan, "kv_cache_plan", block_table, seq_lens, new_lens, None, free_blocks,
+                 free_count, block_size, slots.data_ptr(), at, at + 4 * batch + 4, at + 12 * batch + 4,
+                 at + 8 * batch + 4, max_new_tokens)
+    cu, lens, placed, count = out.split_with_sizes((batch + 1, batch, batch, 1))
+    return KVCachePlan(slots, cu, lens, count, placed)
 
 
 def kv_cache_release(block_table, seq_lens, finished, free_blocks, free_count,
@@ -118,52 +135,63 @@ def kv_cache_release(block_table, seq_lens, finished, free_blocks, free_count,
     ``[batch]``) back on the stack ``free_blocks`` (behind its first ``free_count`` entries, in
     request order). Returns the lengths (0 for those requests) and the count after it, as
     new tensors; the table rows stay as they are. Arguments as for kv_cache_plan."""
-    args, out, batch, device = _bookkeeping(block_table, seq_lens, free_blocks, free_count, block_size)
-    _int32(finished, "finished", batch, device)
-    args.finished = finished.data_ptr()
-    stream = torch.cuda.current_stream(device).cuda_stream
-    _lib.check(_lib.load().apex_attn_kv_release(ctypes.byref(args), stream), "kv_cache_release")
-    return out[:batch], out[batch:]
+    lens, count = torch.empty_like(seq_lens), torch.empty_like(free_count)
+    _bookkeeping(_lib.load().apex_attn_kv_release, "kv_cache_release", block_table, seq_lens, None, finished,
+                 free_blocks, free_count, block_size, 0, 0, lens.data_ptr(), count.data_ptr(), 0, 0)
+    return lens, count
 
 
 def _cache(k_cache, v_cache, k_scale, v_scale, device):
-    """Checks the cache and returns its (block, head, token) byte strides, K's then V's."""
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+    """Checks the cache; returns its shape, the four addresses, and the (block, head, token) byte
+    strides of K, then V."""
+    shape = k_cache.shape
+    if len(shape) != 4 or shape != v_cache.shape:
         raise ValueError(f"k_cache and v_cache must be [num_blocks, H_kv, block_size, D] alike, got "
                          f"{tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
-    if k_cache.dtype != _E4M3 or v_cache.dtype != _E4M3:
+    if k_cache.dtype is not _E4M3 or v_cache.dtype is not _E4M3:
         raise TypeError(f"k_cache and v_cache must be float8_e4m3fn, got {k_cache.dtype}, {v_cache.dtype}")
-    blocks, heads, block_size, headdim = k_cache.shape
+    blocks, heads, block_size, headdim = shape
     if headdim not in _HEAD_DIMS:
         raise KeyError(headdim)
     if block_size not in _BLOCK_SIZES:
         raise ValueError(f"block_size must be one of {_BLOCK_SIZES}, got {block_size}")
-    for s in (k_scale, v_scale):
-        if s.dtype != torch.float32 or s.shape != (blocks, heads) or not s.is_contiguous() or s.device != device:
-            raise ValueError(f"k_scale and v_scale must be contiguous float32 {(blocks, heads)} on {device}, got "
-                             f"{s.dtype} {tuple(s.shape)} on {s.device}")
     if blocks == 0 or heads == 0:
         raise ValueError("the cache has no blocks or no heads")
+    k_at, v_at = k_cache.data_ptr(), v_cache.data_ptr()
     strides = []
-    for c in (k_cache, v_cache):
+    for c, ptr in ((k_cache, k_at), (v_cache, v_at)):
         sb, sh, st, sd = c.stride()
-        sh = sh if heads > 1 else block_size * headdim
-        sb = sb if blocks > 1 else heads * block_size * headdim
+        if heads == 1:
+            sh = block_size * headdim
+        if blocks == 1:
+            sb = heads * block_size * headdim
         # The cache is written and kept by its owner, so a layout that the kernels cannot
         # take is refused instead of copied.
-        if sd != 1 or st < headdim or (sb | sh | st | c.data_ptr()) & 15 or c.device != device:
+        if sd != 1 or st < headdim or (sb | sh | st | ptr) & 15 or c.get_device() != device:
             raise ValueError("k_cache and v_cache need unit stride along D, other strides multiples of 16, 16-byte "
-                             f"aligned storage, and the device {device}")
+                             f"aligned storage, and the CUDA device {device}")
         strides += (sb, sh, st)
-    return strides
+    for s in (k_scale, v_scale):
+        if s.dtype is not torch.float32 or s.shape != (blocks, heads) or not s.is_contiguous() \
+                or s.get_device() != device:
+            raise ValueError(f"k_scale and v_scale must be contiguous float32 {(blocks, heads)} on the CUDA device "
+                             f"{device}, got {s.dtype} {tuple(s.shape)} on {s.device}")
+    return shape, (k_at, v_at, k_scale.data_ptr(), v_scale.data_ptr()), strides
 
 
-def _rows(t, name):
-    """[rows, H, D] as the kernels read it: unit stride along D, others multiples of 8."""
+def _rows(t):
+    """[rows, H, D] as the kernels read it (unit stride along D, others multiples of 8), copied if
+    need be, with its token and head strides."""
     st, sh, sd = t.stride()
     if sd != 1 or (st | sh) & 7 or sh < t.shape[2] or t.data_ptr() & 15:
-        return t.contiguous()
-    return t
+        t = t.contiguous()
+        st, sh, sd = t.stride()
+    return t, st, sh
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(nheads, kv_heads, max_seqlen_q, headdim):
+    return _lib.load().apex_attn_fwd_paged_workspace_bytes(nheads, kv_heads, max_seqlen_q, headdim)
 
 
 def kv_cache_append(k, v, k_cache, v_cache, k_scale, v_scale, slots) -> None:
@@ -178,30 +206,31 @@ def kv_cache_append(k, v, k_cache, v_cache, k_scale, v_scale, slots) -> None:
     not finite are stored as NaN and leave the scale alone. In one call at most one run may go
     to a block, and a block must belong to one request. ``slots`` may be longer than ``k``
     (then its first ``total`` entries count)."""
-    if k.dim() != 3 or k.shape != v.shape:
+    shape = k.shape
+    if len(shape) != 3 or shape != v.shape:
         raise ValueError(f"k and v must be [total, H_kv, D] alike, got {tuple(k.shape)}, {tuple(v.shape)}")
-    total, heads, headdim = k.shape
-    device = k.device
-    if k.dtype not in _DTYPES or v.dtype != k.dtype:
+    total, heads, headdim = shape
+    dtype = _DTYPES.get(k.dtype)
+    if dtype is None or v.dtype is not k.dtype:
         raise TypeError(f"k and v must both be float16 or bfloat16, got {k.dtype}, {v.dtype}")
-    if not k.is_cuda or v.device != device:
+    device = k.get_device()
+    if device < 0 or v.get_device() != device:
         raise ValueError("k and v must be CUDA tensors on one device")
-    cache_strides = _cache(k_cache, v_cache, k_scale, v_scale, device)
-    blocks, cache_heads, block_size, cache_dim = k_cache.shape
-    if (cache_heads, cache_dim) != (heads, headdim):
-        raise ValueError(f"k {tuple(k.shape)} does not match the cache {tuple(k_cache.shape)}")
-    if slots.dtype != torch.int64 or slots.dim() != 1 or slots.numel() < total or slots.device != device \
+    (blocks, cache_heads, block_size, cache_dim), at, cache_strides = _cache(k_cache, v_cache, k_scale, v_scale, device)
+    if cache_heads != heads or cache_dim != headdim:
+        raise ValueError(f"k {tuple(shape)} does not match the cache {tuple(k_cache.shape)}")
+    if slots.dtype is not torch.int64 or slots.dim() != 1 or slots.numel() < total or slots.get_device() != device \
             or not slots.is_contiguous():
-        raise ValueError(f"slots must be a contiguous int64 tensor of at least {total} values on {device}")
+        raise ValueError(f"slots must be a contiguous int64 tensor of at least {total} values on the CUDA device {device}")
     if total == 0:
         return
-    k, v = _rows(k, "k"), _rows(v, "v")
-    args = _lib.KVAppendArgs(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                             k_scale.data_ptr(), v_scale.data_ptr(), slots.data_ptr(), total, heads, headdim,
-                             _DTYPES[k.dtype], blocks, block_size,
-                             (k.stride(0), k.stride(1), v.stride(0), v.stride(1), *cache_strides))
-    stream = torch.cuda.current_stream(device).cuda_stream
-    _lib.check(_lib.load().apex_attn_kv_append(ctypes.byref(args), stream), "kv_cache_append")
+    k, k_st, k_sh = _rows(k)
+    v, v_st, v_sh = _rows(v)
+    args = _lib.KV_APPEND_ARGS.pack(k.data_ptr(), v.data_ptr(), *at, slots.data_ptr(), total, heads, headdim, dtype,
+                                    blocks, block_size, k_st, k_sh, v_st, v_sh, *cache_strides, device + 1)
+    rc = _lib.load().apex_attn_kv_append(args, _raw_stream(device))
+    if rc:
+        _lib.check(rc, "kv_cache_append")
 
 
 def custom_attention_paged_forward(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens,
@@ -221,59 +250,59 @@ def custom_attention_paged_forward(q, k_cache, v_cache, k_scale, v_scale, block_
     they hold.
 
     Head dims 64, 128, 256 (others: KeyError). Asynchronous on the current CUDA stream."""
-    if q.dim() != 3:
-        raise ValueError(f"q must be [total_q, H, D], got {tuple(q.shape)}")
-    total, nheads, headdim = q.shape
-    device = q.device
-    if q.dtype not in _DTYPES:
+    shape = q.shape
+    if len(shape) != 3:
+        raise ValueError(f"q must be [total_q, H, D], got {tuple(shape)}")
+    total, nheads, headdim = shape
+    dtype = _DTYPES.get(q.dtype)
+    if dtype is None:
         raise TypeError(f"q must be float16 or bfloat16, got {q.dtype}")
-    if not q.is_cuda:
+    device = q.get_device()
+    if device < 0:
         raise ValueError("q must be a CUDA tensor")
-    cache_strides = _cache(k_cache, v_cache, k_scale, v_scale, device)
-    blocks, kv_heads, block_size, cache_dim = k_cache.shape
+    (blocks, kv_heads, block_size, cache_dim), at, cache_strides = _cache(k_cache, v_cache, k_scale, v_scale, device)
     if cache_dim != headdim or nheads == 0 or nheads % kv_heads != 0:
-        raise ValueError(f"q {tuple(q.shape)} does not match the cache {tuple(k_cache.shape)}: D alike, and H_kv "
+        raise ValueError(f"q {tuple(shape)} does not match the cache {tuple(k_cache.shape)}: D alike, and H_kv "
                          "dividing q's heads")
     batch, width, table_stride = _table(block_table)
-    if block_table.device != device:
+    if block_table.get_device() != device:
         raise ValueError("all tensors must be CUDA tensors on one device")
-    _int32(seq_lens, "seq_lens", batch, device)
+    if batch == 0 or width == 0:
+        raise ValueError(f"block_table has no entries: {tuple(block_table.shape)}")
+    lens_at = _int32(seq_lens, "seq_lens", batch, device)
+    cu_at = 0
     if cu_seqlens_q is not None:
-        _int32(cu_seqlens_q, "cu_seqlens_q", batch + 1, device)
+        cu_at = _int32(cu_seqlens_q, "cu_seqlens_q", batch + 1, device)
         if max_seqlen_q is None or max_seqlen_q < 1:
             raise ValueError("cu_seqlens_q needs a positive max_seqlen_q")
-    elif batch == 0 or total % batch != 0 or (max_seqlen_q is not None and max_seqlen_q * batch != total):
+    elif total % batch != 0 or (max_seqlen_q is not None and max_seqlen_q * batch != total):
         raise ValueError(f"without cu_seqlens_q, q's {total} rows must be max_seqlen_q for each of {batch} requests")
     else:
         max_seqlen_q = total // batch
     if window_left is not None and (window_left < 0 or not causal):
         raise ValueError("window_left must be >= 0 and needs causal=True")
+    where = q.device
     if out is None:
-        o = torch.empty(q.shape, dtype=q.dtype, device=device)
+        o = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=q.dtype, device=where)
+        o_st, o_sh = nheads * headdim, headdim
     else:
-        o = out
-        if o.shape != q.shape or o.dtype != q.dtype or o.device != device or _rows(o, "out") is not o:
+        o, o_st, o_sh = _rows(out)
+        if o is not out or o.shape != shape or o.dtype is not q.dtype or o.get_device() != device:
             raise ValueError("out must be like q, with unit stride along D and other strides multiples of 8")
-    lse = torch.empty((nheads, total), dtype=torch.float32, device=device) if return_lse else None
-    if total == 0 or batch == 0 or width == 0:
-        if out is None:
-            o.zero_()
-        return (o, lse.zero_()) if return_lse else o
-    q = _rows(q, "q")
+    lse = torch.empty(nheads, total, dtype=torch.float32, device=where) if return_lse else None
+    if total == 0:
+        return (o, lse) if return_lse else o
+    q, q_st, q_sh = _rows(q)
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(headdim)
-    lib = _lib.load()
-    ws_bytes = lib.apex_attn_fwd_paged_workspace_bytes(nheads, kv_heads, max_seqlen_q, headdim)
-    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
-    args = _lib.PagedArgs(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-                          v_scale.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
-                          None if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), o.data_ptr(),
-                          None if lse is None else lse.data_ptr(), table_stride,
-                          (q.stride(0), q.stride(1), o.stride(0), o.stride(1), *cache_strides), batch, nheads,
-                          kv_heads, total, max_seqlen_q, headdim, _DTYPES[q.dtype], blocks, block_size, width,
-                          1 if causal else 0, -1 if window_left is None else window_left, 1 if out is None else 0,
-                          sm_scale)
-    stream = torch.cuda.current_stream(device).cuda_stream
-    rc = lib.apex_attn_fwd_paged(ctypes.byref(args), workspace.data_ptr(), ws_bytes, stream)
-    _lib.check(rc, "custom_attention_paged_forward")
+    ws_bytes = _workspace_bytes(nheads, kv_heads, max_seqlen_q, headdim)
+    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=where)
+    args = _lib.PAGED_ARGS.pack(
+        q.data_ptr(), *at, block_table.data_ptr(), lens_at, cu_at, o.data_ptr(), 0 if lse is None else lse.data_ptr(),
+        table_stride, q_st, q_sh, o_st, o_sh, *cache_strides, batch, nheads, kv_heads, total, max_seqlen_q, headdim,
+        dtype, blocks, block_size, width, 1 if causal else 0, -1 if window_left is None else window_left,
+        1 if out is None else 0, sm_scale, device + 1)
+    rc = _lib.load().apex_attn_fwd_paged(args, workspace.data_ptr(), ws_bytes, _raw_stream(device))
+    if rc:
+        _lib.check(rc, "custom_attention_paged_forward")
     return (o, lse) if return_lse else o

@@ -21,8 +21,8 @@
 // K/V head; as the M side they would leave most of a 128-row tile empty. Thread t owns token t of a
 // tile: its scales are per-thread scalars and its row of P is 16 contiguous bytes per 16 query
 // rows. The price is that a row's maximum runs across threads; so the running maximum is only
-// moved when some p' would pass 2^8.75 (one vote per tile, folded into a barrier that the
-// tile needs anyway), which is rare after a row's first tile.
+// moved when some p' would pass 2^8.75 (one vote per tile), which is rare after a row's
+// first tile.
 //
 // m_i tracks the maximum of x_ij + log2 b_j, kept 2^6 below p's top so that small weights stay
 // above e4m3's floor: the largest weight of a row is held at 2^6 .. 2^8.75 (e4m3's largest is 448).
@@ -34,7 +34,8 @@
 // rows and their base-2 logsumexp) and attn_paged_combine_kernel joins them in a fixed order.
 // Lengths are read on the device only.
 //
-// Warps: 4 or 8 softmax (32 token rows of TMEM each), then TMA producer, MMA issuer, scales.
+// Warps: 4 or 8 softmax (32 token rows of TMEM each), then TMA producer, MMA issuer, scales,
+// query rows.
 #pragma once
 
 #include "attn_fwd_kernel.cuh"
@@ -45,7 +46,6 @@ namespace apex {
 constexpr int kPagedTile = 128;      // cached tokens per tile
 constexpr float kPagedTop = 6.0f;    // log2 of the weight that a row's maximum maps to
 constexpr float kPagedMost = 8.75f;  // a weight above 2^this moves the maximum (448 = 2^8.807)
-constexpr float kPagedUnset = -1e30f;
 // V scales below 2^-100 (0 among them) count as 2^-100, so that 1 / b stays in range.
 constexpr float kPagedLeastScale = 7.888609052210118e-31f;
 
@@ -67,6 +67,7 @@ struct PagedParams {
   long long table_stride;
   long long q_st, q_sh, o_st, o_sh;  // token, head strides (elements)
   int batch, heads_kv, group, total_q, max_q;
+  unsigned group_magic;  // ceil(2^32 / group), for rows of a tile (0: group is 1)
   int num_blocks, block_shift, table_width;
   int causal, window, zero_rest;
   int stream_once;   // the cache is read once per call: do not keep it in L2
@@ -74,8 +75,8 @@ struct PagedParams {
 };
 
 // One entry per CTA for the item that reaches it from the CTA before (2c) and for the one
-// that it leaves to the next (2c + 1): batch, head, query tile, first and last CTA; batch -1:
-// none.
+// that it leaves to the next (2c + 1): first query row of the request (-1: no entry), K/V head,
+// first row of the tile, its rows, first and last CTA.
 constexpr int kShareInts = 8;
 
 template <typename T, int D, int NQ>
@@ -85,36 +86,40 @@ struct PagedCfg {
   static constexpr int kChunks = (D + 127) / 128;
   static constexpr uint32_t kSwizzle = kRow == 128 ? 2 : 4;
   static constexpr int kTerms = std::is_same<T, __half>::value ? 3 : 2;  // of q
-  static constexpr int kWG = NQ >= 64 ? 2 : 1;           // softmax warpgroups, NC query rows each
-  static constexpr int kNC = NQ / kWG;
+  static constexpr int kNC = NQ < 32 ? NQ : 32;          // query rows per softmax warpgroup
+  static constexpr int kWG = NQ / kNC;
   static constexpr int kSoftWarps = 4 * kWG;
-  static constexpr int kThreads = 128 * kWG + 96;
+  static constexpr int kThreads = 128 * (kWG + 1);
   // Two CTAs per SM cover each other's latencies where their shared memory fits.
   static constexpr int kCtas = (D <= 128 && NQ <= 32) ? 2 : 1;
   static constexpr int kSlotBytes = kPagedTile * D;      // one K or V tile
   static constexpr int kPBufs = 2;
-  static constexpr int kQBytes = kTerms * NQ * D;
+  static constexpr int kQBytes = kTerms * NQ * D;        // one segment's query rows
   static constexpr int kPTerm = kPagedTile * NQ;         // one term of one P buffer
   static constexpr int kBudget = kCtas == 2 ? 115712 : 232448;
-  static constexpr int kMiscBytes = 1280 + NQ * 40;      // what the plan below adds
-  static constexpr int kNSMax = (kBudget - kQBytes - kPBufs * kTerms * kPTerm - kMiscBytes) / kSlotBytes;
-  static constexpr int kNS = kNSMax > 12 ? 12 : kNSMax;  // ring slots
+  static constexpr int kMiscBytes = 1856 + NQ * 56;      // what the plan below adds
+  static constexpr int slots(int q_bufs) {
+    return (kBudget - q_bufs * kQBytes - kPBufs * kTerms * kPTerm - kMiscBytes) / kSlotBytes;
+  }
+  // The next segment's query rows are split ahead of time where that leaves four ring slots.
+  static constexpr int kQBufs = slots(2) >= 4 ? 2 : 1;
+  static constexpr int kNS = slots(kQBufs) > 12 ? 12 : slots(kQBufs);  // ring slots
   static_assert(kNS >= 3, "the ring needs K(j + 1) beside K(j) and V(j)");
-  static constexpr int kScaleRing = 4;
+  static constexpr int kScaleRing = 8;
   // TMEM: S buffers at 0 and NQ, O (one block of NQ columns per 128 of the head dim) from 2 NQ.
   static constexpr int kTmemCols = (2 + kChunks) * NQ <= 64 ? 64
                                    : ((2 + kChunks) * NQ <= 128 ? 128 : ((2 + kChunks) * NQ <= 256 ? 256 : 512));
   static_assert((2 + kChunks) * NQ <= 512 && kCtas * kTmemCols <= 512, "TMEM plan");
   // shared-memory plan
   static constexpr int kQ = kNS * kSlotBytes;
-  static constexpr int kP = kQ + kQBytes;
+  static constexpr int kP = kQ + kQBufs * kQBytes;
   static constexpr int kBars = kP + kPBufs * kTerms * kPTerm;
-  static constexpr int kKvFull = 0, kKvEmpty = kNS, kQFull = 2 * kNS, kSFull = kQFull + 1, kSFree = kSFull + 2,
-                       kPFull = kSFree + 2, kPvDone = kPFull + 2, kScFull = kPvDone + 2,
+  static constexpr int kKvFull = 0, kKvEmpty = kNS, kQFull = 2 * kNS, kQEmpty = kQFull + 2,
+                       kColEmpty = kQEmpty + 2, kSFull = kColEmpty + 2, kSFree = kSFull + 2, kPFull = kSFree + 2, kPvDone = kPFull + 2, kScFull = kPvDone + 2,
                        kScEmpty = kScFull + kScaleRing, kDrain = kScEmpty + kScaleRing, kNumBars = kDrain + 1;
   static constexpr int kScales = (kBars + kNumBars * 8 + 15) / 16 * 16;  // float4 [kScaleRing][8 pages]
-  static constexpr int kCol = kScales + kScaleRing * 8 * 16;  // per query row: m, q scale, factor, hi, lo
-  static constexpr int kRed = kCol + 5 * NQ * 4;              // [kWG][4 warps][kNC]
+  static constexpr int kCol = kScales + kScaleRing * 8 * 16;  // two of, per query row: -m, q scale, factor, hi, lo
+  static constexpr int kRed = kCol + 2 * 5 * NQ * 4;          // [kWG][4 warps][kNC]
   static constexpr int kScan = (kRed + 4 * NQ * 4 + 15) / 16 * 16;       // long long [32], start of the CTA's range
   static constexpr int kMisc = kScan + 32 * 8 + 32;
   static constexpr int kBytes = kMisc + 16;
@@ -140,6 +145,20 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedParams& p, int 
   return r;
 }
 
+// Row c (below 2^15) of a tile that begins at row `base` of its request's K/V head: its query
+// token, and its head in the group.
+struct PagedTileRows {
+  int token0, head0;
+  __device__ __forceinline__ PagedTileRows(const PagedParams& p, int base)
+      : token0(base / p.group), head0(base - base / p.group * p.group) {}
+  __device__ __forceinline__ void row(const PagedParams& p, int c, int& token, int& head) const {
+    const unsigned x = (unsigned)(head0 + c);  // x * group < 2^32: the product with the magic is exact
+    const int t = p.group_magic ? (int)__umulhi(x, p.group_magic) : (int)x;
+    token = token0 + t;
+    head = (int)x - t * p.group;
+  }
+};
+
 // Tokens [lo, hi) are what the rows of query tile qt see together; [t0, t0 + n) are their tiles.
 struct PagedSpan {
   int lo, hi, t0, n;
@@ -163,13 +182,21 @@ __device__ __forceinline__ int paged_qtiles(const PagedParams& p, const PagedReq
   return (r.nq * p.group + NQ - 1) / NQ;
 }
 
-// Units of one K/V head of a request: its items' tiles, at least one each (an item that sees
-// nothing still has rows to write).
+// A CTA that begins an item spends about as long on it as on this many tiles: units of an item
+// are these and then its tiles, at least one (an item that sees nothing still has rows to
+// write). Without them the CTAs that got short requests finished last: 48 requests of 129 to
+// 8191 tokens took 115 us instead of TODO us.
+#ifndef ITEMU
+#define ITEMU 3
+#endif
+constexpr int kPagedItemUnits = ITEMU;
+
+// Units of one K/V head of a request.
 template <int NQ>
 __device__ __forceinline__ int paged_head_units(const PagedParams& p, const PagedRequest& r) {
   const int qts = paged_qtiles<NQ>(p, r);
   int units = 0;
-  for (int qt = 0; qt < qts; ++qt) units += max(1, paged_span<NQ>(p, r, qt).n);
+  for (int qt = 0; qt < qts; ++qt) units += kPagedItemUnits + max(1, paged_span<NQ>(p, r, qt).n);
   return units;
 }
 
@@ -186,69 +213,82 @@ struct PagedSegment {
 // Where every role walks from: the CTA's range of units and the item that it begins in.
 struct PagedStart {
   long long unit, end;     // the CTA's range
-  long long total;         // units of the whole call
   long long request_unit;  // first unit of request b
-  int b, ctas;
+  long long share;         // units per CTA, one more for each of the first `more`
+  int b, more;
 };
+
+// Quotient of nonnegative numbers; the 64-bit division is several times as long.
+__device__ __forceinline__ long long paged_div(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return (long long)((unsigned)a / (unsigned)b);
+  return a / b;
+}
 
 template <int NQ>
 struct PagedWalk {
   const PagedParams& p;
-  long long unit, end, total;
-  int ctas;
+  long long unit, end, share;
+  int more;
   int b, h, qt, qts;
   long long item;  // first unit of the item (b, h, qt)
   PagedRequest r;
 
   __device__ __forceinline__ PagedWalk(const PagedParams& params, const PagedStart& s)
-      : p(params), unit(s.unit), end(s.end), total(s.total), ctas(s.ctas), b(s.b), h(0), qt(0), qts(0),
+      : p(params), unit(s.unit), end(s.end), share(s.share), more(s.more), b(s.b), h(0), qt(0), qts(0),
         item(s.request_unit) {
     if (unit >= end) return;
     r = paged_request(p, b);
     qts = paged_qtiles<NQ>(p, r);
     const int per_head = paged_head_units<NQ>(p, r);
-    h = (int)((unit - item) / per_head);
+    h = (int)paged_div(unit - item, per_head);
     item += (long long)h * per_head;
     while (true) {
-      const int n = max(1, paged_span<NQ>(p, r, qt).n);
+      const int n = kPagedItemUnits + max(1, paged_span<NQ>(p, r, qt).n);
       if (item + n > unit) break;
       item += n;
       ++qt;
     }
   }
 
+  // The CTA whose range holds a unit.
+  __device__ __forceinline__ int cta_of(long long u) const {
+    const long long large = more * (share + 1);
+    return u < large ? (int)paged_div(u, share + 1) : more + (int)paged_div(u - large, share);
+  }
+
   __device__ __forceinline__ bool next(PagedSegment& s) {
-    if (unit >= end) return false;
-    while (qt == qts) {  // on to the next head or request that has query rows
-      qt = 0;
-      if (++h == p.heads_kv || qts == 0) {
-        h = 0;
-        ++b;
-        r = paged_request(p, b);
-        qts = paged_qtiles<NQ>(p, r);
+    while (unit < end) {
+      while (qt == qts) {  // on to the next head or request that has query rows
+        qt = 0;
+        if (++h == p.heads_kv || qts == 0) {
+          h = 0;
+          ++b;
+          r = paged_request(p, b);
+          qts = paged_qtiles<NQ>(p, r);
+        }
       }
+      s.span = paged_span<NQ>(p, r, qt);
+      const int n = max(1, s.span.n);
+      const long long first = item + kPagedItemUnits, last = first + n;  // the tiles' units
+      const long long from = max(unit, first), to = min(end, last);
+      s.b = b;
+      s.h = h;
+      s.qt = qt;
+      s.r = r;
+      s.tile = s.span.t0 + (int)(from - first);
+      s.n = s.span.n == 0 ? 0 : (int)(to - from);
+      s.slot = -1;
+      if (to - from < n) {
+        s.slot = 2 * blockIdx.x + (from > first ? 0 : 1);
+        s.c0 = cta_of(first);
+        s.c1 = cta_of(last - 1);
+      }
+      unit = min(end, last);
+      item = last;
+      ++qt;
+      if (from < to) return true;  // else the range ends before the item's first tile
     }
-    s.b = b;
-    s.h = h;
-    s.qt = qt;
-    s.r = r;
-    s.span = paged_span<NQ>(p, r, qt);
-    const int n = max(1, s.span.n);
-    const int skip = (int)(unit - item);
-    const int take = (int)min((long long)(n - skip), end - unit);
-    s.tile = s.span.t0 + skip;
-    s.n = s.span.n == 0 ? 0 : take;
-    s.slot = -1;
-    if (take < n) {
-      s.slot = 2 * blockIdx.x + (skip > 0 ? 0 : 1);
-      // CTA c has the units [c * total / ctas, (c + 1) * total / ctas).
-      s.c0 = (int)(((item + 1) * ctas - 1) / total);
-      s.c1 = (int)(((item + n) * ctas - 1) / total);
-    }
-    unit += take;
-    item += n;
-    ++qt;
-    return true;
+    return false;
   }
 };
 
@@ -261,11 +301,13 @@ __device__ __forceinline__ PagedStart paged_start(const PagedParams& p, long lon
   long long mine = 0;
   for (int b = b0; b < b1; ++b) mine += (long long)paged_head_units<NQ>(p, paged_request(p, b)) * p.heads_kv;
   PagedStart s;
-  const long long upto = block_scan<long long>(mine, scan, s.total);
-  s.ctas = (int)min((long long)gridDim.x, max(s.total, 1LL));
-  const long long c = min((int)blockIdx.x, s.ctas);
-  s.unit = c * s.total / s.ctas;
-  s.end = (int)blockIdx.x < s.ctas ? (c + 1) * s.total / s.ctas : s.unit;
+  long long total;
+  const long long upto = block_scan<long long>(mine, scan, total);
+  s.share = paged_div(total, gridDim.x);
+  s.more = (int)(total - s.share * gridDim.x);
+  const int c = (int)blockIdx.x;
+  s.unit = c * s.share + min(c, s.more);
+  s.end = s.unit + s.share + (c < s.more ? 1 : 0);
   long long at = upto - mine;
   __syncthreads();  // scan is written again
   if (s.unit < s.end && at <= s.unit && s.unit < upto) {
@@ -297,8 +339,8 @@ __device__ __forceinline__ __half2 half2_of_e4m3x2(uint32_t v) {
   return *reinterpret_cast<__half2*>(&h);
 }
 
-// Sums over the warp, N values at a time, each lane ending with the sums of N / 32 (at least
-// one) of them: v[0 .. max(1, N / 32)) for the columns from `column_of_lane` on.
+// Sums N (at most 32) values per lane over the warp; each lane ends with the sum of one in
+// v[0] and gets its index (lanes that differ in the lowest bit share one if N is 16).
 template <int N>
 __device__ __forceinline__ int warp_column_sums(float (&v)[N]) {
   const int lane = threadIdx.x & 31;
@@ -324,6 +366,87 @@ __device__ __forceinline__ int warp_column_sums(float (&v)[N]) {
   return col;
 }
 
+// Splits a segment's query rows: each is scaled by a power of two to (224, 448], split into
+// e4m3 terms and stored as the B operand of S^T, [term][16-byte chunk of the head dim][row]; the
+// rows' column arrays are set up. Warp `w` of `warps` takes its share of the rows.
+template <typename T, int D, int NQ>
+__device__ __forceinline__ void split_query_rows(const PagedParams& p, const PagedSegment& seg, uint8_t* smem,
+                                                 int n, int w, int warps) {
+  using C = PagedCfg<T, D, NQ>;
+  constexpr int kPerRow = D / 16;      // lanes per query row, 16 values each
+  constexpr int kStep = 32 / kPerRow;  // rows per warp and step
+  const int lane = (int)(threadIdx.x & 31), chunk = lane % kPerRow;
+  const int rows = min(NQ, seg.r.nq * p.group - seg.qt * NQ);
+  float* const col_nm = reinterpret_cast<float*>(smem + C::kCol) + (n & 1) * 5 * NQ;
+  const uint32_t dst = ptx::smem_u32(smem) + C::kQ + (n % C::kQBufs) * C::kQBytes + chunk * (NQ * 16);
+  const PagedTileRows tile(p, seg.qt * NQ);
+  const T* const q = static_cast<const T*>(p.q) + (long long)seg.r.q0 * p.q_st +
+                     (long long)(seg.h * p.group) * p.q_sh + chunk * 16;
+  constexpr int kAhead = 4;  // steps whose loads are under way
+  uint4 na[kAhead], nb[kAhead];
+  auto load = [&](int c, uint4& a, uint4& b) {
+    a = b = make_uint4(0, 0, 0, 0);
+    if (c < rows) {
+      int token, head;
+      tile.row(p, c, token, head);
+      const uint4* src = reinterpret_cast<const uint4*>(q + (long long)token * p.q_st + (long long)head * p.q_sh);
+      a = __ldg(src);
+      b = __ldg(src + 1);
+    }
+  };
+  const int first = w * kStep + lane / kPerRow, step = warps * kStep;
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) load(first + i * step, na[i], nb[i]);
+#pragma unroll 1
+  for (int c = first; c < NQ; c += step) {
+    uint32_t x[8] = {na[0].x, na[0].y, na[0].z, na[0].w, nb[0].x, nb[0].y, nb[0].z, nb[0].w};
+#pragma unroll
+    for (int i = 0; i + 1 < kAhead; ++i) na[i] = na[i + 1], nb[i] = nb[i + 1];
+    load(c + kAhead * step, na[kAhead - 1], nb[kAhead - 1]);
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t m = x[k] & 0x7fff7fffu;
+      const uint32_t bad = __vcmpgeu2(m, Elem<T>::kInf2);
+      top = __vmaxu2(top, m & ~bad);
+      x[k] |= bad & 0x7fff7fffu;  // infinities become NaN: the row's scores have no value
+    }
+    top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+    for (int d = 1; d < kPerRow; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const float s = append_scale(Elem<T>::to_float2(top).x);
+    const float inv = 1.f / s;  // a power of two
+    uint32_t term[C::kTerms][4];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      // Scaled values fit fp16 exactly (11 bits; below 2^-13 fewer, far under e4m3's floor).
+      const float2 f = __fmul2_rn(Elem<T>::to_float2(x[k]), make_float2(inv, inv));
+      __half2 rest = __floats2half2_rn(f.x, f.y);
+#pragma unroll
+      for (int j = 0; j < C::kTerms; ++j) {
+        const uint32_t e = e4m3x2_of_half2(rest);
+        if (j + 1 < C::kTerms) rest = __hsub2(rest, half2_of_e4m3x2(e));
+        term[j][k >> 1] = (k & 1) ? term[j][k >> 1] | (e << 16) : e;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < C::kTerms; ++j)
+      ptx::st_shared_v4(dst + j * NQ * D + c * 16, term[j][0], term[j][1], term[j][2], term[j][3]);
+    if (chunk == 0) {
+      int token, head;
+      tile.row(p, c, token, head);
+      const int place = seg.r.len - seg.r.nq + min(token, seg.r.nq - 1);
+      col_nm[c] = 0.f;
+      col_nm[NQ + c] = s;
+      col_nm[2 * NQ + c] = -1.f;
+      reinterpret_cast<int*>(col_nm)[3 * NQ + c] = p.causal ? min(place + 1, seg.r.len) : seg.r.len;
+      reinterpret_cast<int*>(col_nm)[4 * NQ + c] = p.window >= 0 ? max(place - p.window, 0) : 0;
+    }
+  }
+  ptx::fence_proxy_async_smem();
+  __syncwarp();
+}
+
 template <typename T, int D, int NQ>
 __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, NQ>::kCtas)
     attn_paged_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -337,9 +460,12 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     if (threadIdx.x < 2) p.share[(2 * blockIdx.x + threadIdx.x) * kShareInts] = -1;
     return;
   }
+  // All CTAs of this launch are on the device at once, so the joining kernel's may take the
+  // places that they leave, and wait there for the last.
+  ptx::launch_dependents();
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
   const int lane = (int)(threadIdx.x & 31);
-  constexpr int kWarpProd = C::kSoftWarps, kWarpMma = kWarpProd + 1, kWarpScale = kWarpProd + 2;
+  constexpr int kWarpProd = C::kSoftWarps, kWarpMma = kWarpProd + 1, kWarpScale = kWarpProd + 2, kWarpQ = kWarpProd + 3;
   auto bar = [&](int slot) -> uint32_t { return sbase + C::kBars + slot * 8; };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kMisc + 4);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::kMisc);
@@ -349,8 +475,10 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       ptx::mbar_init(bar(C::kKvFull + s), 1);
       ptx::mbar_init(bar(C::kKvEmpty + s), 1);
     }
-    ptx::mbar_init(bar(C::kQFull), C::kSoftWarps);
     for (int b = 0; b < 2; ++b) {
+      ptx::mbar_init(bar(C::kQFull + b), 1);
+      ptx::mbar_init(bar(C::kQEmpty + b), 1);
+      ptx::mbar_init(bar(C::kColEmpty + b), C::kSoftWarps);
       ptx::mbar_init(bar(C::kSFull + b), 1);
       ptx::mbar_init(bar(C::kSFree + b), C::kSoftWarps);
       ptx::mbar_init(bar(C::kPFull + b), C::kSoftWarps);
@@ -395,85 +523,34 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     const int t = (warp & 3) * 32 + lane;  // token of the tile; column of the head dim
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     const int c_first = wg * NC;           // this warpgroup's query rows of the tile
-    float* const col_m = reinterpret_cast<float*>(smem + C::kCol) + c_first;  // max - kPagedTop
-    float* const col_q = col_m + NQ;       // q's scale
-    float* const col_f = col_m + 2 * NQ;   // factor of a moved maximum; 1 / sum at the end
-    int* const col_hi = reinterpret_cast<int*>(col_m + 3 * NQ);
-    int* const col_lo = reinterpret_cast<int*>(col_m + 4 * NQ);
     float* const red = reinterpret_cast<float*>(smem + C::kRed) + wg * 4 * NC;
     const float4* const scales = reinterpret_cast<const float4*>(smem + C::kScales);
     const int page = t >> p.block_shift;
     int g = 0;  // tiles so far
     uint32_t fills = 0;  // ring fills of the segments before
-    while (walk.next(seg)) {
+    for (int n = 0; walk.next(seg); ++n) {
       const int rows = min(NQ, seg.r.nq * p.group - seg.qt * NQ) - c_first;  // of this warpgroup; may be <= 0
-      // ---- the query rows: scale each to (224, 448], split, store as the B operand ----
-      ptx::named_bar_sync(1 + wg, 128);  // the last segment's reads of the column arrays are done
-      constexpr int kPerRow = D / 16;    // threads (and 16-byte chunks of e4m3) per query row
-      const int chunk = t % kPerRow;
-#pragma unroll 1
-      for (int c = t / kPerRow; c < NC; c += 128 / kPerRow) {
-        const int row = seg.qt * NQ + c_first + c;
-        const int i = row / p.group, hq = seg.h * p.group + row % p.group;
-        uint32_t w[8];
-        uint32_t top = 0;
-        if (c < rows) {
-          const uint4* src = reinterpret_cast<const uint4*>(
-              static_cast<const T*>(p.q) + (long long)(seg.r.q0 + i) * p.q_st + (long long)hq * p.q_sh + chunk * 16);
-          const uint4 a = __ldg(src), b = __ldg(src + 1);
-          w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) w[k] = 0;
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t m = w[k] & 0x7fff7fffu;
-          const uint32_t bad = __vcmpgeu2(m, Elem<T>::kInf2);
-          top = __vmaxu2(top, m & ~bad);
-          w[k] |= bad & 0x7fff7fffu;  // infinities become NaN: the row's scores have no value
-        }
-        top = max(top & 0xffffu, top >> 16);
-#pragma unroll
-        for (int d = 1; d < kPerRow; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-        const float s = append_scale(Elem<T>::to_float2(top).x);
-        const float inv = 1.f / s;  // a power of two
-        uint32_t term[C::kTerms][4];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          float2 f = Elem<T>::to_float2(w[k]);
-          f = make_float2(f.x * inv, f.y * inv);
-#pragma unroll
-          for (int j = 0; j < C::kTerms; ++j) {
-            const uint32_t e = e4m3x2(f.x, f.y);
-            const float2 back = e4m3x2_to_float2(e);
-            f = make_float2(f.x - back.x, f.y - back.y);
-            term[j][k >> 1] = (k & 1) ? term[j][k >> 1] | (e << 16) : e;
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < C::kTerms; ++j)
-          ptx::st_shared_v4(sbase + C::kQ + j * NQ * D + chunk * (NQ * 16) + (c_first + c) * 16, term[j][0],
-                            term[j][1], term[j][2], term[j][3]);
-        if (chunk == 0) {
-          const int place = seg.r.len - seg.r.nq + min(i, seg.r.nq - 1);
-          col_m[c] = kPagedUnset;
-          col_q[c] = s;
-          col_hi[c] = p.causal ? min(place + 1, seg.r.len) : seg.r.len;
-          col_lo[c] = p.window >= 0 ? max(place - p.window, 0) : 0;
-        }
+      float* const col_nm = reinterpret_cast<float*>(smem + C::kCol) + (n & 1) * 5 * NQ + c_first;  // kPagedTop - max
+      const float* const col_q = col_nm + NQ;  // q's scale
+      float* const col_f = col_nm + 2 * NQ;    // factor of a moved maximum, -1 before the first; 1 / sum at the end
+      const int* const col_hi = reinterpret_cast<const int*>(col_nm + 3 * NQ);  // tokens [lo, hi) are seen
+      const int* const col_lo = reinterpret_cast<const int*>(col_nm + 4 * NQ);
+      if (n == 0) {  // these warps have nothing else to do yet; later segments' rows are split ahead
+        split_query_rows<T, D, NQ>(p, seg, smem, 0, warp, C::kSoftWarps);
+        ptx::named_bar_sync(7, 32 * C::kSoftWarps);
+        if (threadIdx.x == 0) ptx::mbar_arrive(bar(C::kQFull));
       }
-      ptx::fence_proxy_async_smem();
-      ptx::named_bar_sync(1 + wg, 128);
-      if (seg.n > 0 && lane == 0) ptx::mbar_arrive(bar(C::kQFull));
+      wait(C::kQFull + (n & 1), (uint32_t)(n >> 1));
+      const PagedTileRows tile_rows(p, seg.qt * NQ);
       // Tiles within [lo_all, hi_all) are seen whole by every row of the tile.
-      const int p_first = seg.r.len - seg.r.nq + seg.qt * NQ / p.group;
+      const int p_first = seg.r.len - seg.r.nq + tile_rows.token0;
       const int p_last = seg.r.len - seg.r.nq + (min(seg.r.nq * p.group, (seg.qt + 1) * NQ) - 1) / p.group;
       const int hi_all = p.causal ? min(seg.r.len, p_first + 1) : seg.r.len;
       const int lo_all = p.window >= 0 ? max(0, p_last - p.window) : 0;
-      float l[NC];
+      float2 l[NC / 2];
 #pragma unroll
-      for (int c = 0; c < NC; ++c) l[c] = 0.f;
+      for (int c = 0; c < NC / 2; ++c) l[c] = make_float2(0.f, 0.f);
+      bool force = true;  // a row's maximum may not be set: first tile, or behind one left of a row's window
 
 #pragma unroll 1
       for (int j = 0; j < seg.n; ++j, ++g) {
@@ -483,56 +560,65 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
         const float4 sc = scales[(g % C::kScaleRing) * 8 + page];  // a * scale_log2, log2 b, 1 / b
         wait(C::kSFull + sb, (uint32_t)(g >> 1));
         ptx::tc_fence_after();
-        uint32_t s[NC];
+        float2 d[NC / 2];
 #pragma unroll
-        for (int c = 0; c < NC; c += 16) ptx::tmem_ld16(tmem + lane_off + (uint32_t)(sb * NQ + c_first + c), s + c);
+        for (int c = 0; c < NC; c += 16)
+          ptx::tmem_ld16(tmem + lane_off + (uint32_t)(sb * NQ + c_first + c), reinterpret_cast<uint32_t*>(d) + c);
         ptx::tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < NC; c += 16) ptx::reg_fence16(s + c);
+        for (int c = 0; c < NC; c += 16) ptx::reg_fence16(reinterpret_cast<uint32_t*>(d) + c);
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) {
           ptx::mbar_arrive(bar(C::kScEmpty + g % C::kScaleRing));
           ptx::mbar_arrive(bar(C::kSFree + sb));
         }
-        // y = x + log2 b, in place; -inf where the row does not see the token.
-#pragma unroll
-        for (int c = 0; c < NC; c += 4) {
-          const float4 q4 = *reinterpret_cast<const float4*>(col_q + c);
-          s[c] = __float_as_uint(fmaf(__uint_as_float(s[c]), sc.x * q4.x, sc.y));
-          s[c + 1] = __float_as_uint(fmaf(__uint_as_float(s[c + 1]), sc.x * q4.y, sc.y));
-          s[c + 2] = __float_as_uint(fmaf(__uint_as_float(s[c + 2]), sc.x * q4.z, sc.y));
-          s[c + 3] = __float_as_uint(fmaf(__uint_as_float(s[c + 3]), sc.x * q4.w, sc.y));
-        }
-        if (pos0 < lo_all || pos0 + kPagedTile > hi_all) {
-#pragma unroll
-          for (int c = 0; c < NC; ++c)
-            if (pos < col_lo[c] || pos >= col_hi[c]) s[c] = 0xff800000u;
-        }
+        // d = x + log2 b - m; -inf where the row does not see the token.
+        const float2 a2 = make_float2(sc.x, sc.x), b2 = make_float2(sc.y, sc.y), i2 = make_float2(sc.z, sc.z);
         float most = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < NC; c += 4) {
-          const float4 m4 = *reinterpret_cast<const float4*>(col_m + c);
-          most = fmaxf(fmaxf(most, __uint_as_float(s[c]) - m4.x), __uint_as_float(s[c + 1]) - m4.y);
-          most = fmaxf(fmaxf(most, __uint_as_float(s[c + 2]) - m4.z), __uint_as_float(s[c + 3]) - m4.w);
+        for (int c = 0; c < NC / 2; c += 2) {
+          const float4 q4 = *reinterpret_cast<const float4*>(col_q + 2 * c);
+          const float4 n4 = *reinterpret_cast<const float4*>(col_nm + 2 * c);
+          d[c] = __ffma2_rn(d[c], __fmul2_rn(a2, make_float2(q4.x, q4.y)), __fadd2_rn(b2, make_float2(n4.x, n4.y)));
+          d[c + 1] =
+              __ffma2_rn(d[c + 1], __fmul2_rn(a2, make_float2(q4.z, q4.w)), __fadd2_rn(b2, make_float2(n4.z, n4.w)));
+          most = ptx::fmax3(most, d[c].x, d[c].y);
+          most = ptx::fmax3(most, d[c + 1].x, d[c + 1].y);
         }
-        if (ptx::named_bar_or(1 + wg, 128, most > kPagedMost)) {
-          // Move the maxima: over the warp, over the warps, then rescale the sums and O.
+        const bool masked = pos0 < lo_all || pos0 + kPagedTile > hi_all;
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+            if (pos < col_lo[c] || pos >= col_hi[c]) (c & 1 ? d[c / 2].y : d[c / 2].x) = -INFINITY;
+        }
+        const bool left = pos0 < lo_all;
+        const bool move = force || left ? true : ptx::named_bar_or(1 + wg, 128, most > kPagedMost);
+        force = left;
+        if (move) {
+          // Move the maxima: over the warp, over the warps; then rescale the sums and O.
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
-            const float top = ptx::warp_max(__uint_as_float(s[c]));
-            if (lane == (c & 31)) red[(warp & 3) * NC + c] = top;
+            const float top = ptx::warp_max(c & 1 ? d[c / 2].y : d[c / 2].x);
+            if (lane == c) red[(warp & 3) * NC + c] = top;
           }
           ptx::named_bar_sync(1 + wg, 128);
           if (t < NC) {
-            const float top = fmaxf(fmaxf(red[t], red[NC + t]), fmaxf(red[2 * NC + t], red[3 * NC + t])) - kPagedTop;
-            const float old = col_m[t], now = fmaxf(old, top);
-            col_f[t] = ptx::ex2(old - now);
-            col_m[t] = now;
+            const float top = fmaxf(fmaxf(red[t], red[NC + t]), fmaxf(red[2 * NC + t], red[3 * NC + t]));
+            // By how much the maximum moves: up only, but freely the first time.
+            const bool set = col_f[t] >= 0.f;
+            const float by = top == -INFINITY ? 0.f : (set ? fmaxf(top - kPagedTop, 0.f) : top - kPagedTop);
+            if (set || top != -INFINITY) col_f[t] = set ? ptx::ex2(-by) : 0.f;
+            col_nm[t] -= by;
+            red[t] = by;
           }
           ptx::named_bar_sync(1 + wg, 128);
 #pragma unroll
-          for (int c = 0; c < NC; ++c) l[c] *= col_f[c];
+          for (int c = 0; c < NC / 2; ++c) {
+            const float2 by = *reinterpret_cast<const float2*>(red + 2 * c);
+            d[c] = make_float2(d[c].x - by.x, d[c].y - by.y);
+            l[c] = __fmul2_rn(l[c], *reinterpret_cast<const float2*>(col_f + 2 * c));
+          }
           if (j > 0) {
             wait(C::kPvDone + (sb ^ 1), (uint32_t)((g - 1) >> 1));
             ptx::tc_fence_after();
@@ -559,15 +645,12 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           uint32_t term[C::kTerms][4];
 #pragma unroll
           for (int k = 0; k < 16; k += 4) {
-            const float4 m4 = *reinterpret_cast<const float4*>(col_m + c + k);
-            float e[4];
-            e[0] = ptx::ex2(__uint_as_float(s[c + k]) - m4.x);
-            e[1] = ptx::ex2(__uint_as_float(s[c + k + 1]) - m4.y);
-            e[2] = ptx::ex2(__uint_as_float(s[c + k + 2]) - m4.z);
-            e[3] = ptx::ex2(__uint_as_float(s[c + k + 3]) - m4.w);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) l[c + k + x] = fmaf(e[x], sc.z, l[c + k + x]);
-            __half2 a = __floats2half2_rn(e[0], e[1]), b = __floats2half2_rn(e[2], e[3]);
+            const int x = (c + k) / 2;
+            const float2 e0 = make_float2(ptx::ex2(d[x].x), ptx::ex2(d[x].y));
+            const float2 e1 = make_float2(ptx::ex2(d[x + 1].x), ptx::ex2(d[x + 1].y));
+            l[x] = __ffma2_rn(e0, i2, l[x]);
+            l[x + 1] = __ffma2_rn(e1, i2, l[x + 1]);
+            __half2 a = __floats2half2_rn(e0.x, e0.y), b = __floats2half2_rn(e1.x, e1.y);
 #pragma unroll
             for (int j2 = 0; j2 < C::kTerms; ++j2) {
               const uint32_t ea = e4m3x2_of_half2(a), eb = e4m3x2_of_half2(b);
@@ -604,31 +687,29 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
 
       // ---- the segment's result ----
       {
-        const int c = warp_column_sums<NC>(l);
-        constexpr int kMine = NC / 32 > 1 ? NC / 32 : 1;
-        if (NC >= 32 || (lane & (32 / NC - 1)) == 0)
+        float sums[NC];
 #pragma unroll
-          for (int k = 0; k < kMine; ++k) red[(warp & 3) * NC + c + k] = l[k];
+        for (int c = 0; c < NC / 2; ++c) sums[2 * c] = l[c].x, sums[2 * c + 1] = l[c].y;
+        const int c = warp_column_sums<NC>(sums);
+        if (NC == 32 || (lane & 1) == 0) red[(warp & 3) * NC + c] = sums[0];
       }
       ptx::named_bar_sync(1 + wg, 128);
       if (t < NC && t < rows) {
         const float sum = red[t] + red[NC + t] + red[2 * NC + t] + red[3 * NC + t];
-        const float lse2 = sum == 0.f ? -INFINITY : col_m[t] + __log2f(sum);
+        const float lse2 = sum == 0.f ? -INFINITY : __log2f(sum) - col_nm[t];
         col_f[t] = sum == 0.f ? 0.f : 1.f / sum;
-        const int row = seg.qt * NQ + c_first + t;
-        if (seg.slot >= 0)
+        if (seg.slot >= 0) {
           p.part_lse[(long long)seg.slot * NQ + c_first + t] = lse2;
-        else if (p.lse != nullptr)
-          p.lse[(long long)(seg.h * p.group + row % p.group) * p.total_q + seg.r.q0 + row / p.group] =
-              lse2 * 0.69314718055994531f;
+        } else if (p.lse != nullptr) {
+          int token, head;
+          tile_rows.row(p, c_first + t, token, head);
+          p.lse[(long long)(seg.h * p.group + head) * p.total_q + seg.r.q0 + token] = lse2 * 0.69314718055994531f;
+        }
       }
       if (seg.slot >= 0 && threadIdx.x == 0) {
-        int* at = p.share + seg.slot * kShareInts;
-        at[0] = seg.b;
-        at[1] = seg.h;
-        at[2] = seg.qt;
-        at[3] = seg.c0;
-        at[4] = seg.c1;
+        int4* at = reinterpret_cast<int4*>(p.share + seg.slot * kShareInts);
+        at[0] = make_int4(seg.r.q0, seg.h, seg.qt * NQ, min(NQ, seg.r.nq * p.group - seg.qt * NQ));
+        at[1] = make_int4(seg.c0, seg.c1, 0, 0);
       }
       if (seg.n > 0) wait(C::kPvDone + ((g - 1) & 1), (uint32_t)((g - 1) >> 1));
       ptx::tc_fence_after();
@@ -643,8 +724,8 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           ptx::tmem_ld16(tmem + lane_off + (uint32_t)(2 * NQ + ch * NQ + c_first + c), v);
           ptx::tmem_wait_ld();
           ptx::reg_fence16(v);
-          const int row = seg.qt * NQ + c_first + c;
-          int i = row / p.group, hq = row % p.group;
+          int i, hq;
+          tile_rows.row(p, c_first + c, i, hq);
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
             const float inv = col_f[c + k];
@@ -665,6 +746,8 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
         }
       }
       ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar(C::kColEmpty + (n & 1)));
     }
   } else if (warp == kWarpProd) {
     // ========================================================== producer ===
@@ -673,13 +756,15 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     const uint64_t policy = p.stream_once ? ptx::policy_evict_first() : ptx::policy_evict_last();
     const int pages = kPagedTile >> p.block_shift;
     uint32_t fills = 0;
-    auto page_id = [&](int tile) -> int {  // -2: not loaded
-      const int at = tile * kPagedTile + (lane << p.block_shift);
-      if (lane >= pages || at >= seg.span.hi || at + (1 << p.block_shift) <= seg.span.lo) return -2;
-      const int id = __ldg(p.block_table + (long long)seg.b * p.table_stride + (at >> p.block_shift));
-      return id >= 0 && id < p.num_blocks ? id : -1;  // -1: outside the cache, reads as zeros
+    // Block ids of four tiles at a time, one batch ahead: lane 8 i + k holds page k of the i-th.
+    // -2: not loaded; -1: outside the cache, reads as zeros.
+    auto page_ids = [&](const PagedSegment& s, int tile) -> int {
+      const int at = (tile + (lane >> 3)) * kPagedTile + ((lane & 7) << p.block_shift);
+      if ((lane & 7) >= pages || at >= s.span.hi || at + (1 << p.block_shift) <= s.span.lo) return -2;
+      const int id = __ldg(p.block_table + (long long)s.b * p.table_stride + (at >> p.block_shift));
+      return id >= 0 && id < p.num_blocks ? id : -1;
     };
-    auto fill = [&](const CUtensorMap* map, int id) {
+    auto fill = [&](const CUtensorMap* map, int id) {  // `seg`'s head
       const int slot = (int)(fills % NS);
       wait(C::kKvEmpty + slot, (fills / NS) ^ 1u);
       const uint32_t full = bar(C::kKvFull + slot);
@@ -698,20 +783,48 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       }
       __syncwarp();
     };
-    while (walk.next(seg)) {
-      if (seg.n == 0) continue;
-      int id = page_id(seg.tile);
-      fill(&tmK, id);
+    // The next segment and its first block ids are looked up while the ring is full of this one.
+    bool more = walk.next(seg);
+    int ids = -2, ahead = -2;
+    if (more) {
+      ids = page_ids(seg, seg.tile);
+      ahead = page_ids(seg, seg.tile + 4);
+    }
+    while (more) {
+      PagedSegment then;
+      int then_ids = -2, then_ahead = -2;
+      auto look = [&]() {
+        more = walk.next(then);
+        if (more) {
+          then_ids = page_ids(then, then.tile);
+          then_ahead = page_ids(then, then.tile + 4);
+        }
+      };
+      auto pick = [&](int j) {  // tile j's ids, page k in lane k
+        const int id = __shfl_sync(0xffffffffu, ids, ((j & 3) << 3) + (lane & 7));
+        return lane < 8 ? id : -2;
+      };
+      if (seg.n == 0) look();
+      int id = seg.n > 0 ? pick(0) : -2;
+      if (seg.n > 0) fill(&tmK, id);
 #pragma unroll 1
       for (int j = 0; j < seg.n; ++j) {
         int next = -2;
         if (j + 1 < seg.n) {
-          next = page_id(seg.tile + j + 1);
+          if (((j + 1) & 3) == 0) {
+            ids = ahead;
+            ahead = page_ids(seg, seg.tile + j + 5);
+          }
+          next = pick(j + 1);
           fill(&tmK, next);
         }
         fill(&tmV, id);
         id = next;
+        if (j == 0) look();
       }
+      seg = then;
+      ids = then_ids;
+      ahead = then_ahead;
     }
     // Let every load land before the CTA exits.
     if (lane == 0) {
@@ -735,7 +848,8 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       ++reads;
       return slot;
     };
-    auto issue_S = [&]() {
+    int n = 0;  // segments so far
+    auto issue_S = [&](bool last) {
       const int sb = gs & 1;
       if (gs >= 2) wait(C::kSFree + sb, (uint32_t)((gs >> 1) - 1));
       const int slot = acquire();
@@ -751,13 +865,14 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
 #pragma unroll
             for (int j = 0; j < C::kTerms; ++j) {
               const uint64_t b = ptx::smem_desc(
-                  sbase + C::kQ + j * NQ * D + (ch * (C::kRow / 16) + 2 * ks) * (NQ * 16), NQ * 16, 128, 0);
+                  sbase + C::kQ + (n % C::kQBufs) * C::kQBytes + j * NQ * D + (ch * (C::kRow / 16) + 2 * ks) * (NQ * 16), NQ * 16, 128, 0);
               ptx::umma_ss_f8_warp(tmem + (uint32_t)(sb * NQ), a, b, idS, acc);
               acc = 1;
             }
           }
         ptx::tc_commit_warp(bar(C::kKvEmpty + slot));
         ptx::tc_commit_warp(bar(C::kSFull + sb));
+        if (last) ptx::tc_commit_warp(bar(C::kQEmpty + n % C::kQBufs));
       }
       ++gs;
     };
@@ -786,33 +901,37 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       }
       ++gp;
     };
-    int n = 0;  // segments with tiles so far
-    while (walk.next(seg)) {
-      if (seg.n == 0) continue;
-      wait(C::kQFull, (uint32_t)n++);
-      issue_S();
+    for (; walk.next(seg); ++n) {
+      wait(C::kQFull + (n & 1), (uint32_t)(n >> 1));
+      if (seg.n == 0) {
+        if (lane == 0) ptx::mbar_arrive(bar(C::kQEmpty + n % C::kQBufs));
+        continue;
+      }
+      issue_S(seg.n == 1);
 #pragma unroll 1
       for (int j = 0; j < seg.n; ++j) {
-        if (j + 1 < seg.n) issue_S();
+        if (j + 1 < seg.n) issue_S(j + 2 == seg.n);
         issue_PV(j == 0);
       }
     }
     ptx::tc_commit_warp(bar(C::kDrain));
     if (lane == 0) drain_wait(bar(C::kDrain), 0, p.timeout_ns, p.status, p.host_flag);
     __syncwarp();
-  } else {
+  } else if (warp == kWarpScale) {
     // ============================================================ scales ===
     // Ahead of the softmax: per tile and page, a * sm_scale * log2 e, log2 b and 1 / b.
+    // Four tiles' loads at a time: lane 8 i + k looks after page k of the i-th.
     const int pages = kPagedTile >> p.block_shift;
     float4* const scales = reinterpret_cast<float4*>(smem + C::kScales);
     int g = 0;
     while (walk.next(seg)) {
 #pragma unroll 1
-      for (int j = 0; j < seg.n; ++j, ++g) {
-        const int at = (seg.tile + j) * kPagedTile + (lane << p.block_shift);
+      for (int j0 = 0; j0 < seg.n; j0 += 4) {
+        const int j = j0 + (lane >> 3), page = lane & 7;
+        const int at = (seg.tile + j) * kPagedTile + (page << p.block_shift);
         // Pages that are not there: zero scores and values, and a V scale too small to move a maximum.
         float4 sc = make_float4(0.f, -100.f, 1.f / kPagedLeastScale, 0.f);
-        if (lane < pages && at < seg.span.hi && at + (1 << p.block_shift) > seg.span.lo) {
+        if (j < seg.n && page < pages && at < seg.span.hi && at + (1 << p.block_shift) > seg.span.lo) {
           const int id = __ldg(p.block_table + (long long)seg.b * p.table_stride + (at >> p.block_shift));
           if (id >= 0 && id < p.num_blocks) {
             const float a = __ldg(p.k_scale + (long long)id * p.heads_kv + seg.h);
@@ -820,10 +939,14 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
             sc = make_float4(a * p.scale_log2, __log2f(b), 1.f / b, 0.f);
           }
         }
-        wait(C::kScEmpty + g % C::kScaleRing, (uint32_t)(g / C::kScaleRing) ^ 1u);
-        if (lane < pages) scales[(g % C::kScaleRing) * 8 + lane] = sc;
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(bar(C::kScFull + g % C::kScaleRing));
+        const int take = min(4, seg.n - j0);
+#pragma unroll 1
+        for (int i = 0; i < take; ++i, ++g) {
+          wait(C::kScEmpty + g % C::kScaleRing, (uint32_t)(g / C::kScaleRing) ^ 1u);
+          if ((lane >> 3) == i) scales[(g % C::kScaleRing) * 8 + page] = sc;
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(bar(C::kScFull + g % C::kScaleRing));
+        }
       }
     }
     if (p.zero_rest) {  // rows behind a request and before the next (or the first)
@@ -844,15 +967,23 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
         if (b == 0) clear(0, r.q0);
       }
     }
+  } else if (warp == kWarpQ) {
+    // ======================================================== query rows ===
+    // Ahead of the softmax, from the second segment on.
+    for (int n = 0; walk.next(seg); ++n) {
+      if (n == 0) continue;
+      if (n >= C::kQBufs) wait(C::kQEmpty + n % C::kQBufs, (uint32_t)(n / C::kQBufs - 1));
+      if (n >= 2) wait(C::kColEmpty + (n & 1), (uint32_t)((n >> 1) - 1));
+      split_query_rows<T, D, NQ>(p, seg, smem, n, 0, 1);
+      if (lane == 0) ptx::mbar_arrive(bar(C::kQFull + (n & 1)));
+    }
   }
-
   ptx::tc_fence_before();
   __syncthreads();
   if (warp == kWarpMma) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem, C::kTmemCols);
   }
-  ptx::launch_dependents();
 }
 
 // Joins the parts of the items that several CTAs shared: o = sum_k w_k o_k / sum_k w_k with
@@ -869,13 +1000,11 @@ __global__ void __launch_bounds__(kCombineThreads) attn_paged_combine_kernel(con
   ptx::wait_for_previous_grid();
 #pragma unroll 1
   for (int side = 0; side < 2; ++side) {
-    const int* at = p.share + (2 * blockIdx.x + side) * kShareInts;
-    const int b = at[0];
-    if (b < 0) continue;
-    const int h = at[1], qt = at[2], c0 = at[3], c1 = at[4];
-    const int k_parts = c1 - c0 + 1;
-    const PagedRequest r = paged_request(p, b);
-    const int rows = min(NQ, r.nq * p.group - qt * NQ);
+    const int4* at = reinterpret_cast<const int4*>(p.share + (2 * blockIdx.x + side) * kShareInts);
+    const int4 item = at[0], ctas = at[1];
+    if (item.x < 0) continue;
+    const int h = item.y, rows = item.w, c0 = ctas.x, k_parts = ctas.y - ctas.x + 1;
+    const PagedTileRows tile_rows(p, item.z);
     const bool alone = k_parts <= 4;  // a warp joins a row by itself
     const int lanes = alone ? kWarps : 1;
     for (int c = ((int)blockIdx.x - c0) * lanes + (alone ? warp : 0); c < rows; c += k_parts * lanes) {
@@ -930,15 +1059,17 @@ __global__ void __launch_bounds__(kCombineThreads) attn_paged_combine_kernel(con
         __syncthreads();
         if (warp != 0) continue;
       }
-      const int row = qt * NQ + c;
-      const int i = row / p.group, hq = h * p.group + row % p.group;
+      int i, hq;
+      tile_rows.row(p, c, i, hq);
+      i += item.x;
+      hq += h * p.group;
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      T* o = static_cast<T*>(p.o) + (long long)(r.q0 + i) * p.o_st + (long long)hq * p.o_sh + lane * E;
+      T* o = static_cast<T*>(p.o) + (long long)i * p.o_st + (long long)hq * p.o_sh + lane * E;
 #pragma unroll
       for (int e = 0; e < E; e += 2)
         *reinterpret_cast<uint32_t*>(o + e) = DType<T>::pack(acc[e] * inv, acc[e + 1] * inv);
       if (p.lse != nullptr && lane == 0)
-        p.lse[(long long)hq * p.total_q + r.q0 + i] = sum == 0.f ? -INFINITY : (m + __log2f(sum)) * 0.69314718055994531f;
+        p.lse[(long long)hq * p.total_q + i] = sum == 0.f ? -INFINITY : (m + __log2f(sum)) * 0.69314718055994531f;
     }
   }
 }

@@ -43,6 +43,12 @@ int common_device(const void* const* ptrs, int n) {
   return dev;
 }
 
+// The device of a call: the one that the caller knows to own every pointer, else looked up.
+int device_of_call(int known, const void* const* ptrs, int n) {
+  if (known != 0) return known > 0 && known <= apex::host::kMaxDevices ? known - 1 : -1;
+  return common_device(ptrs, n);
+}
+
 // Raises a kernel's dynamic shared-memory limit once per device.
 template <typename K>
 int allow_smem(K kern, int bytes, std::atomic<unsigned long long>& done, int dev) {
@@ -85,7 +91,7 @@ int plan(const apex_attn_kv_plan_args* a, bool release, void* stream) {
   // The CTAs read all inputs independently of one another's writes.
   if (a->seq_lens_out == a->seq_lens || a->free_count_out == a->free_count) return APEX_ATTN_ERR_INVALID_ARGUMENT;
 
-  const int dev = common_device(ptrs, 10);
+  const int dev = device_of_call(a->known_device, ptrs, 10);
   if (dev < 0) return APEX_ATTN_ERR_NO_DEVICE;
   DeviceGuard guard(dev);
   apex::host::Device d;
@@ -143,7 +149,7 @@ int append(const apex_attn_kv_append_args* a, void* stream) {
     return APEX_ATTN_ERR_BAD_LAYOUT;
 
   const void* ptrs[] = {a->k, a->v, a->k_cache, a->v_cache, a->k_scale, a->v_scale, a->slots};
-  const int dev = common_device(ptrs, 7);
+  const int dev = device_of_call(a->known_device, ptrs, 7);
   if (dev < 0) return APEX_ATTN_ERR_NO_DEVICE;
   DeviceGuard guard(dev);
   apex::host::Device d;
@@ -227,7 +233,9 @@ int encode_cache(CUtensorMap* m, const void* ptr, const apex_attn_paged_args& a,
   const CUresult r = apex::host::tensor_map_encoder()(
       m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(ptr), dims, strides, box, estr,
       CU_TENSOR_MAP_INTERLEAVE_NONE, a.head_dim >= 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+      // Rows that do not follow one another: fetching 256 bytes for one would read a neighbour's.
+      st[2] >= 256 && st[2] > a.head_dim ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? APEX_ATTN_OK : APEX_ATTN_ERR_TENSOR_MAP;
 }
 
@@ -297,7 +305,7 @@ int forward_paged(const apex_attn_paged_args* a, void* workspace, size_t bytes, 
   if (!apex_attn_supports_head_dim(a->head_dim)) return APEX_ATTN_ERR_UNSUPPORTED_HEAD_DIM;
   if (a->dtype != APEX_ATTN_BF16 && a->dtype != APEX_ATTN_FP16) return APEX_ATTN_ERR_UNSUPPORTED_DTYPE;
   if (!std::isfinite(a->sm_scale) || !(a->sm_scale > 0.f)) return APEX_ATTN_ERR_BAD_SCALE;
-  if (a->total_q > (1 << 30) || a->batch > 65535 || a->heads_q > 65535 ||
+  if (a->total_q > (1 << 30) || a->batch > 65535 || a->heads_q > 32767 ||
       (long long)a->max_seqlen_q * a->heads_q > (1 << 30) || (long long)a->table_width * a->block_size > (1 << 30))
     return APEX_ATTN_ERR_TOO_LARGE;
   for (int i = 0; i < 4; ++i)
@@ -318,7 +326,7 @@ int forward_paged(const apex_attn_paged_args* a, void* workspace, size_t bytes, 
   // ---- device ----
   const void* ptrs[] = {a->q,           a->k_cache,  a->v_cache,      a->k_scale, a->v_scale,
                         a->block_table, a->seq_lens, a->cu_seqlens_q, a->o,       a->lse, workspace};
-  const int dev = common_device(ptrs, 11);
+  const int dev = device_of_call(a->known_device, ptrs, 11);
   if (dev < 0) return APEX_ATTN_ERR_NO_DEVICE;
   DeviceGuard guard(dev);
   apex::host::Device d;
@@ -356,6 +364,7 @@ int forward_paged(const apex_attn_paged_args* a, void* workspace, size_t bytes, 
   p.batch = a->batch;
   p.heads_kv = a->heads_kv;
   p.group = group;
+  p.group_magic = group > 1 ? (unsigned)(((1ull << 32) + group - 1) / group) : 0;
   p.total_q = a->total_q;
   p.max_q = a->max_seqlen_q;
   p.num_blocks = a->num_blocks;

@@ -393,6 +393,7 @@ typedef struct apex_attn_kv_plan_args {
   int free_capacity;
   int block_size;
   int max_new_tokens;
+  int known_device; /* see apex_attn_paged_args */
 } apex_attn_kv_plan_args;
 
 int apex_attn_kv_plan(const apex_attn_kv_plan_args* args, void* stream);
@@ -427,6 +428,7 @@ typedef struct apex_attn_kv_append_args {
   int num_blocks;
   int block_size;
   long long strides[10];
+  int known_device; /* see apex_attn_paged_args */
 } apex_attn_kv_append_args;
 
 int apex_attn_kv_append(const apex_attn_kv_append_args* args, void* stream);
@@ -481,6 +483,9 @@ typedef struct apex_attn_paged_args {
   int window_left;
   int zero_rest;
   float sm_scale;
+  int known_device; /* 0: the pointers are looked up, and refused unless all are memory of one device.
+                       Otherwise 1 + the ordinal of the device that the caller knows to own them
+                       all (saves the host about a third of a microsecond per pointer). */
 } apex_attn_paged_args;
 
 size_t apex_attn_fwd_paged_workspace_bytes(int heads_q, int heads_kv, int max_seqlen_q, int head_dim);

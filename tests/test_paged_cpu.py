@@ -107,6 +107,24 @@ def test_attention_refuses(lib, kw, code):
     assert paged(lib, **kw) == code
 
 
+def test_packed_layouts_are_the_structs():
+    for packed, mirror in ((_lib.KV_PLAN_ARGS, _lib.KVPlanArgs), (_lib.KV_APPEND_ARGS, _lib.KVAppendArgs),
+                           (_lib.PAGED_ARGS, _lib.PagedArgs)):
+        assert -(-packed.size // 8) * 8 == ctypes.sizeof(mirror)
+        values = list(range(1, len(packed.unpack(bytes(packed.size))) + 1))
+        got = mirror.from_buffer_copy(packed.pack(*values).ljust(ctypes.sizeof(mirror), b"\0"))
+        flat = []
+        for name, _ in mirror._fields_:
+            x = getattr(got, name)
+            flat += list(x) if hasattr(x, "__len__") else [x]
+        assert flat == values
+
+
+def test_known_device_out_of_range(lib):
+    assert paged(lib, known_device=65) == NODEV
+    assert paged(lib, known_device=-1) == NODEV
+
+
 def test_null_argument_structs(lib):
     for fn in (lib.apex_attn_kv_plan, lib.apex_attn_kv_release, lib.apex_attn_kv_append):
         assert fn(None, None) == BAD
