@@ -34,8 +34,10 @@
 // rows and their base-2 logsumexp) and attn_paged_combine_kernel joins them in a fixed order.
 // Lengths are read on the device only.
 //
-// Warps: 4 or 8 softmax (32 token rows of TMEM each), then TMA producer, MMA issuer, scales,
-// query rows.
+// Warps: 4 to 16 softmax (32 token rows of TMEM each), then TMA producer, MMA issuer, scales and
+// work list, query rows. The scales' warp alone walks the work list and publishes the segments
+// in shared memory: a warp on its own takes some 4 cycles per dependent instruction, and all
+// warps walking cost each of them about 2 us at the start and 1 us per segment.
 #pragma once
 
 #include "attn_fwd_kernel.cuh"
@@ -70,13 +72,13 @@ struct PagedParams {
   unsigned group_magic;  // ceil(2^32 / group), for rows of a tile (0: group is 1)
   int num_blocks, block_shift, table_width;
   int causal, window, zero_rest;
-  int stream_once;   // the cache is read once per call: do not keep it in L2
+  int one_tile;      // every request's rows of a K/V head fit one query tile; the cache is read once
   float scale_log2;  // sm_scale * log2(e)
 };
 
 // One entry per CTA for the item that reaches it from the CTA before (2c) and for the one
 // that it leaves to the next (2c + 1): first query row of the request (-1: no entry), K/V head,
-// first row of the tile, its rows, first and last CTA.
+// rows of the tile, first token; first and last CTA, first head.
 constexpr int kShareInts = 8;
 
 template <typename T, int D, int NQ>
@@ -97,15 +99,18 @@ struct PagedCfg {
   static constexpr int kQBytes = kTerms * NQ * D;        // one segment's query rows
   static constexpr int kPTerm = kPagedTile * NQ;         // one term of one P buffer
   static constexpr int kBudget = kCtas == 2 ? 115712 : 232448;
-  static constexpr int kMiscBytes = 1856 + NQ * 56;      // what the plan below adds
+  static constexpr int kMiscBytes = 2240 + NQ * 56;      // what the plan below adds
   static constexpr int slots(int q_bufs) {
     return (kBudget - q_bufs * kQBytes - kPBufs * kTerms * kPTerm - kMiscBytes) / kSlotBytes;
   }
   // The next segment's query rows are split ahead of time where that leaves four ring slots.
-  static constexpr int kQBufs = slots(2) >= 4 ? 2 : 1;
+  // Larger tiles' rows are too many for one warp: the softmax warps split them between segments.
+  static constexpr bool kSelfSplit = NQ > 32;
+  static constexpr int kQBufs = !kSelfSplit && slots(2) >= 4 ? 2 : 1;
   static constexpr int kNS = slots(kQBufs) > 12 ? 12 : slots(kQBufs);  // ring slots
   static_assert(kNS >= 3, "the ring needs K(j + 1) beside K(j) and V(j)");
   static constexpr int kScaleRing = 8;
+  static constexpr int kSegRing = 4;
   // TMEM: S buffers at 0 and NQ, O (one block of NQ columns per 128 of the head dim) from 2 NQ.
   static constexpr int kTmemCols = (2 + kChunks) * NQ <= 64 ? 64
                                    : ((2 + kChunks) * NQ <= 128 ? 128 : ((2 + kChunks) * NQ <= 256 ? 256 : 512));
@@ -116,12 +121,14 @@ struct PagedCfg {
   static constexpr int kBars = kP + kPBufs * kTerms * kPTerm;
   static constexpr int kKvFull = 0, kKvEmpty = kNS, kQFull = 2 * kNS, kQEmpty = kQFull + 2,
                        kColEmpty = kQEmpty + 2, kSFull = kColEmpty + 2, kSFree = kSFull + 2, kPFull = kSFree + 2, kPvDone = kPFull + 2, kScFull = kPvDone + 2,
-                       kScEmpty = kScFull + kScaleRing, kDrain = kScEmpty + kScaleRing, kNumBars = kDrain + 1;
+                       kScEmpty = kScFull + kScaleRing, kSegFull = kScEmpty + kScaleRing,
+                       kSegEmpty = kSegFull + kSegRing, kDrain = kSegEmpty + kSegRing, kNumBars = kDrain + 1;
   static constexpr int kScales = (kBars + kNumBars * 8 + 15) / 16 * 16;  // float4 [kScaleRing][8 pages]
   static constexpr int kCol = kScales + kScaleRing * 8 * 16;  // two of, per query row: -m, q scale, factor, hi, lo
   static constexpr int kRed = kCol + 2 * 5 * NQ * 4;          // [kWG][4 warps][kNC]
-  static constexpr int kScan = (kRed + 4 * NQ * 4 + 15) / 16 * 16;       // long long [32], start of the CTA's range
-  static constexpr int kMisc = kScan + 32 * 8 + 32;
+  static constexpr int kSegs = (kRed + 4 * NQ * 4 + 15) / 16 * 16;       // int4 [kSegRing][kSegVecs]
+  static constexpr int kScan = kSegs + kSegRing * 5 * 16;                // long long [32], found request
+  static constexpr int kMisc = kScan + 32 * 8 + 16;
   static constexpr int kBytes = kMisc + 16;
   static_assert(kBytes <= kBudget, "shared-memory plan");
 };
@@ -145,31 +152,32 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedParams& p, int 
   return r;
 }
 
-// Row c (below 2^15) of a tile that begins at row `base` of its request's K/V head: its query
-// token, and its head in the group.
-struct PagedTileRows {
-  int token0, head0;
-  __device__ __forceinline__ PagedTileRows(const PagedParams& p, int base)
-      : token0(base / p.group), head0(base - base / p.group * p.group) {}
-  __device__ __forceinline__ void row(const PagedParams& p, int c, int& token, int& head) const {
-    const unsigned x = (unsigned)(head0 + c);  // x * group < 2^32: the product with the magic is exact
-    const int t = p.group_magic ? (int)__umulhi(x, p.group_magic) : (int)x;
-    token = token0 + t;
-    head = (int)x - t * p.group;
-  }
-};
+// Row c (below 2^15) of a tile that begins at head `head0` of the group for query token `token0`:
+// its query token, and its head in the group.
+__device__ __forceinline__ void paged_row(const PagedParams& p, int token0, int head0, int c, int& token, int& head) {
+  const unsigned x = (unsigned)(head0 + c);  // x * group < 2^32: the product with the magic is exact
+  const int t = p.group_magic ? (int)__umulhi(x, p.group_magic) : (int)x;
+  token = token0 + t;
+  head = (int)x - t * p.group;
+}
 
 // Tokens [lo, hi) are what the rows of query tile qt see together; [t0, t0 + n) are their tiles.
 struct PagedSpan {
   int lo, hi, t0, n;
+  int i0, i1;  // first and last query token of the tile
 };
 
 template <int NQ>
 __device__ __forceinline__ PagedSpan paged_span(const PagedParams& p, const PagedRequest& r, int qt) {
-  const int i0 = qt * NQ / p.group;
-  const int i1 = (min(r.nq * p.group, (qt + 1) * NQ) - 1) / p.group;
+  int i0 = 0, i1 = r.nq - 1;
+  if (!p.one_tile) {
+    i0 = qt * NQ / p.group;
+    i1 = (min(r.nq * p.group, (qt + 1) * NQ) - 1) / p.group;
+  }
   const int first = r.len - r.nq + i0, last = r.len - r.nq + i1;  // positions
   PagedSpan s;
+  s.i0 = i0;
+  s.i1 = i1;
   s.hi = p.causal ? min(r.len, last + 1) : r.len;
   s.lo = p.window >= 0 ? max(0, first - p.window) : 0;
   s.t0 = s.lo / kPagedTile;
@@ -179,49 +187,56 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedParams& p, const Page
 
 template <int NQ>
 __device__ __forceinline__ int paged_qtiles(const PagedParams& p, const PagedRequest& r) {
-  return (r.nq * p.group + NQ - 1) / NQ;
+  return p.one_tile ? min(r.nq, 1) : (r.nq * p.group + NQ - 1) / NQ;
 }
 
 // A CTA that begins an item spends about as long on it as on this many tiles: units of an item
 // are these and then its tiles, at least one (an item that sees nothing still has rows to
 // write). Without them the CTAs that got short requests finished last: 48 requests of 129 to
 // 8191 tokens took 115 us instead of TODO us.
-#ifndef ITEMU
-#define ITEMU 3
-#endif
-constexpr int kPagedItemUnits = ITEMU;
+template <int NQ>
+constexpr int kPagedItemUnits = NQ <= 32 ? 4 : 8;
 
 // Units of one K/V head of a request.
 template <int NQ>
 __device__ __forceinline__ int paged_head_units(const PagedParams& p, const PagedRequest& r) {
   const int qts = paged_qtiles<NQ>(p, r);
   int units = 0;
-  for (int qt = 0; qt < qts; ++qt) units += kPagedItemUnits + max(1, paged_span<NQ>(p, r, qt).n);
+  for (int qt = 0; qt < qts; ++qt) units += kPagedItemUnits<NQ> + max(1, paged_span<NQ>(p, r, qt).n);
   return units;
 }
 
-// A CTA's part of an item.
+// A CTA's part of an item, as the walking warp publishes it.
 struct PagedSegment {
-  int b, h, qt;
-  PagedRequest r;
-  PagedSpan span;
-  int tile, n;        // tiles [tile, tile + n) of the cache
-  int slot;           // -1: the whole item; else its entry of the workspace
-  int c0, c1;         // CTAs that share the item
+  int b, h, q0, nq;              // request, K/V head, the request's first query row and rows
+  int len, lo, hi, tile;         // cached tokens; tokens [lo, hi) are seen; first tile
+  int n, slot, rows, token0;     // tiles (-1: no more segments); workspace entry, -1 if the item is whole
+  int head0, lo_all, hi_all, pad;  // rows' first head; tokens [lo_all, hi_all) are seen by every row
 };
+constexpr int kSegVecs = sizeof(PagedSegment) / 16;
+static_assert(sizeof(PagedSegment) == 64, "published as four 16-byte words");
 
-// Where every role walks from: the CTA's range of units and the item that it begins in.
+// Where every role walks from: the CTA's range of units and the request that it begins in.
 struct PagedStart {
   long long unit, end;     // the CTA's range
   long long request_unit;  // first unit of request b
   long long share;         // units per CTA, one more for each of the first `more`
   int b, more;
+  __device__ __forceinline__ void cut(long long total);
 };
 
 // Quotient of nonnegative numbers; the 64-bit division is several times as long.
 __device__ __forceinline__ long long paged_div(long long a, long long b) {
   if (((a | b) >> 32) == 0) return (long long)((unsigned)a / (unsigned)b);
   return a / b;
+}
+
+__device__ __forceinline__ void PagedStart::cut(long long total) {
+  share = paged_div(total, gridDim.x);
+  more = (int)(total - share * gridDim.x);
+  const int c = (int)blockIdx.x;
+  unit = c * share + min(c, more);
+  end = unit + share + (c < more ? 1 : 0);
 }
 
 template <int NQ>
@@ -240,10 +255,12 @@ struct PagedWalk {
     r = paged_request(p, b);
     qts = paged_qtiles<NQ>(p, r);
     const int per_head = paged_head_units<NQ>(p, r);
-    h = (int)paged_div(unit - item, per_head);
-    item += (long long)h * per_head;
+    if (p.heads_kv > 1) {
+      h = (int)paged_div(unit - item, per_head);
+      item += (long long)h * per_head;
+    }
     while (true) {
-      const int n = kPagedItemUnits + max(1, paged_span<NQ>(p, r, qt).n);
+      const int n = kPagedItemUnits<NQ> + max(1, paged_span<NQ>(p, r, qt).n);
       if (item + n > unit) break;
       item += n;
       ++qt;
@@ -256,7 +273,10 @@ struct PagedWalk {
     return u < large ? (int)paged_div(u, share + 1) : more + (int)paged_div(u - large, share);
   }
 
-  __device__ __forceinline__ bool next(PagedSegment& s) {
+  // The next segment, or one of -1 tiles behind the last.
+  __device__ __forceinline__ PagedSegment next() {
+    PagedSegment s;
+    s.n = -1;
     while (unit < end) {
       while (qt == qts) {  // on to the next head or request that has query rows
         qt = 0;
@@ -267,47 +287,101 @@ struct PagedWalk {
           qts = paged_qtiles<NQ>(p, r);
         }
       }
-      s.span = paged_span<NQ>(p, r, qt);
-      const int n = max(1, s.span.n);
-      const long long first = item + kPagedItemUnits, last = first + n;  // the tiles' units
+      const PagedSpan span = paged_span<NQ>(p, r, qt);
+      const int n = max(1, span.n);
+      const long long first = item + kPagedItemUnits<NQ>, last = first + n;  // the tiles' units
       const long long from = max(unit, first), to = min(end, last);
-      s.b = b;
-      s.h = h;
-      s.qt = qt;
-      s.r = r;
-      s.tile = s.span.t0 + (int)(from - first);
-      s.n = s.span.n == 0 ? 0 : (int)(to - from);
-      s.slot = -1;
-      if (to - from < n) {
-        s.slot = 2 * blockIdx.x + (from > first ? 0 : 1);
-        s.c0 = cta_of(first);
-        s.c1 = cta_of(last - 1);
-      }
+      const int row0 = qt * NQ;
       unit = min(end, last);
       item = last;
       ++qt;
-      if (from < to) return true;  // else the range ends before the item's first tile
+      if (from >= to) continue;  // the range ends before the item's first tile
+      s.b = b;
+      s.h = h;
+      s.q0 = r.q0;
+      s.nq = r.nq;
+      s.len = r.len;
+      s.lo = span.lo;
+      s.hi = span.hi;
+      s.tile = span.t0 + (int)(from - first);
+      s.n = span.n == 0 ? 0 : (int)(to - from);
+      s.rows = min(NQ, r.nq * p.group - row0);
+      s.token0 = span.i0;
+      s.head0 = row0 - span.i0 * p.group;
+      const int place = r.len - r.nq;
+      s.hi_all = p.causal ? min(r.len, place + span.i0 + 1) : r.len;
+      s.lo_all = p.window >= 0 ? max(0, place + span.i1 - p.window) : 0;
+      s.slot = -1;
+      if (to - from < n) {
+        s.slot = 2 * (int)blockIdx.x + (from > first ? 0 : 1);
+        if ((threadIdx.x & 31) == 0) {
+          int4* at = reinterpret_cast<int4*>(p.share + s.slot * kShareInts);
+          at[0] = make_int4(r.q0, h, s.rows, s.token0);
+          at[1] = make_int4(cta_of(first), cta_of(last - 1), s.head0, 0);
+        }
+      }
+      return s;
     }
-    return false;
+    return s;
   }
 };
 
-// The CTA's range, and the request that it begins in. All threads call it.
+constexpr int kPagedWarpBatch = 128;  // requests that one warp looks over by itself
+
+// The CTA's range, and the request that it begins in: by one warp, for batches up to
+// kPagedWarpBatch.
 template <int NQ>
-__device__ __forceinline__ PagedStart paged_start(const PagedParams& p, long long* scan, int* found) {
-  // Each thread sums a run of requests; the one whose run holds the first unit looks closer.
+__device__ __forceinline__ PagedStart paged_start_warp(const PagedParams& p) {
+  constexpr int kRounds = kPagedWarpBatch / 32;
+  const int lane = (int)(threadIdx.x & 31);
+  PagedStart s;
+  long long upto[kRounds], mine[kRounds], total = 0;
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    const int b = 32 * i + lane;
+    mine[i] = b < p.batch ? (long long)paged_head_units<NQ>(p, paged_request(p, b)) * p.heads_kv : 0;
+  }
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    upto[i] = mine[i];
+    if (32 * i < p.batch) {
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, upto[i], d);
+        if (lane >= d) upto[i] += up;
+      }
+      upto[i] += total;
+      total = __shfl_sync(0xffffffffu, upto[i], 31);
+    }
+  }
+  s.cut(total);
+  s.b = 0;
+  s.request_unit = 0;
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    if (32 * i < p.batch) {
+      const unsigned has = __ballot_sync(0xffffffffu, upto[i] - mine[i] <= s.unit && s.unit < upto[i]);
+      if (has != 0) {
+        s.b = 32 * i + __ffs(has) - 1;
+        s.request_unit = __shfl_sync(0xffffffffu, upto[i] - mine[i], __ffs(has) - 1);
+      }
+    }
+  }
+  return s;
+}
+
+// The same by the whole CTA: each thread sums a run of requests, and the one whose run holds
+// the first unit looks closer.
+template <int NQ>
+__device__ __forceinline__ PagedStart paged_start_cta(const PagedParams& p, long long* scan, int* found) {
+  PagedStart s;
   const int per = (p.batch + blockDim.x - 1) / blockDim.x;
   const int b0 = min(p.batch, (int)threadIdx.x * per), b1 = min(p.batch, b0 + per);
   long long mine = 0;
   for (int b = b0; b < b1; ++b) mine += (long long)paged_head_units<NQ>(p, paged_request(p, b)) * p.heads_kv;
-  PagedStart s;
   long long total;
   const long long upto = block_scan<long long>(mine, scan, total);
-  s.share = paged_div(total, gridDim.x);
-  s.more = (int)(total - s.share * gridDim.x);
-  const int c = (int)blockIdx.x;
-  s.unit = c * s.share + min(c, s.more);
-  s.end = s.unit + s.share + (c < s.more ? 1 : 0);
+  s.cut(total);
   long long at = upto - mine;
   __syncthreads();  // scan is written again
   if (s.unit < s.end && at <= s.unit && s.unit < upto) {
@@ -327,16 +401,29 @@ __device__ __forceinline__ PagedStart paged_start(const PagedParams& p, long lon
   return s;
 }
 
-__device__ __forceinline__ uint32_t e4m3x2_of_half2(__half2 v) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<uint32_t*>(&v)));
+// Four fp16 values to e4m3 (a.x in the lowest byte) and back. One asm block each, so that the
+// halves are converted in place instead of being moved and merged.
+__device__ __forceinline__ uint32_t e4m3x4_of_half2(__half2 a, __half2 b) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 lo, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 hi, %2;\n\t"
+      "mov.b32 %0, {lo, hi};\n\t}"
+      : "=r"(r)
+      : "r"(*reinterpret_cast<uint32_t*>(&a)), "r"(*reinterpret_cast<uint32_t*>(&b)));
   return r;
 }
 
-__device__ __forceinline__ __half2 half2_of_e4m3x2(uint32_t v) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)v));
-  return *reinterpret_cast<__half2*>(&h);
+__device__ __forceinline__ void half2_of_e4m3x4(uint32_t v, __half2& a, __half2& b) {
+  uint32_t x, y;
+  asm("{\n\t.reg .b16 lo, hi;\n\t"
+      "mov.b32 {lo, hi}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, lo;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+      : "=r"(x), "=r"(y)
+      : "r"(v));
+  a = *reinterpret_cast<__half2*>(&x);
+  b = *reinterpret_cast<__half2*>(&y);
 }
 
 // Sums N (at most 32) values per lane over the warp; each lane ends with the sum of one in
@@ -369,27 +456,24 @@ __device__ __forceinline__ int warp_column_sums(float (&v)[N]) {
 // Splits a segment's query rows: each is scaled by a power of two to (224, 448], split into
 // e4m3 terms and stored as the B operand of S^T, [term][16-byte chunk of the head dim][row]; the
 // rows' column arrays are set up. Warp `w` of `warps` takes its share of the rows.
-template <typename T, int D, int NQ>
+template <typename T, int D, int NQ, int kAhead>
 __device__ __forceinline__ void split_query_rows(const PagedParams& p, const PagedSegment& seg, uint8_t* smem,
                                                  int n, int w, int warps) {
   using C = PagedCfg<T, D, NQ>;
   constexpr int kPerRow = D / 16;      // lanes per query row, 16 values each
-  constexpr int kStep = 32 / kPerRow;  // rows per warp and step
+  constexpr int kStep = 32 / kPerRow;  // rows per warp and step; kAhead steps' loads are under way
   const int lane = (int)(threadIdx.x & 31), chunk = lane % kPerRow;
-  const int rows = min(NQ, seg.r.nq * p.group - seg.qt * NQ);
   float* const col_nm = reinterpret_cast<float*>(smem + C::kCol) + (n & 1) * 5 * NQ;
   const uint32_t dst = ptx::smem_u32(smem) + C::kQ + (n % C::kQBufs) * C::kQBytes + chunk * (NQ * 16);
-  const PagedTileRows tile(p, seg.qt * NQ);
-  const T* const q = static_cast<const T*>(p.q) + (long long)seg.r.q0 * p.q_st +
+  const T* const q = static_cast<const T*>(p.q) + (long long)seg.q0 * p.q_st +
                      (long long)(seg.h * p.group) * p.q_sh + chunk * 16;
-  constexpr int kAhead = 4;  // steps whose loads are under way
   uint4 na[kAhead], nb[kAhead];
   auto load = [&](int c, uint4& a, uint4& b) {
     a = b = make_uint4(0, 0, 0, 0);
-    if (c < rows) {
+    if (c < seg.rows) {
       int token, head;
-      tile.row(p, c, token, head);
-      const uint4* src = reinterpret_cast<const uint4*>(q + (long long)token * p.q_st + (long long)head * p.q_sh);
+      paged_row(p, seg.token0, seg.head0, c, token, head);
+      const uint4* src = reinterpret_cast<const uint4*>(q + token * p.q_st + head * p.q_sh);
       a = __ldg(src);
       b = __ldg(src + 1);
     }
@@ -418,15 +502,20 @@ __device__ __forceinline__ void split_query_rows(const PagedParams& p, const Pag
     const float inv = 1.f / s;  // a power of two
     uint32_t term[C::kTerms][4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < 4; ++k) {
       // Scaled values fit fp16 exactly (11 bits; below 2^-13 fewer, far under e4m3's floor).
-      const float2 f = __fmul2_rn(Elem<T>::to_float2(x[k]), make_float2(inv, inv));
-      __half2 rest = __floats2half2_rn(f.x, f.y);
+      const float2 f = __fmul2_rn(Elem<T>::to_float2(x[2 * k]), make_float2(inv, inv));
+      const float2 g = __fmul2_rn(Elem<T>::to_float2(x[2 * k + 1]), make_float2(inv, inv));
+      __half2 a = __floats2half2_rn(f.x, f.y), b = __floats2half2_rn(g.x, g.y);
 #pragma unroll
       for (int j = 0; j < C::kTerms; ++j) {
-        const uint32_t e = e4m3x2_of_half2(rest);
-        if (j + 1 < C::kTerms) rest = __hsub2(rest, half2_of_e4m3x2(e));
-        term[j][k >> 1] = (k & 1) ? term[j][k >> 1] | (e << 16) : e;
+        term[j][k] = e4m3x4_of_half2(a, b);
+        if (j + 1 < C::kTerms) {
+          __half2 ra, rb;
+          half2_of_e4m3x4(term[j][k], ra, rb);
+          a = __hsub2(a, ra);
+          b = __hsub2(b, rb);
+        }
       }
     }
 #pragma unroll
@@ -434,12 +523,12 @@ __device__ __forceinline__ void split_query_rows(const PagedParams& p, const Pag
       ptx::st_shared_v4(dst + j * NQ * D + c * 16, term[j][0], term[j][1], term[j][2], term[j][3]);
     if (chunk == 0) {
       int token, head;
-      tile.row(p, c, token, head);
-      const int place = seg.r.len - seg.r.nq + min(token, seg.r.nq - 1);
+      paged_row(p, seg.token0, seg.head0, c, token, head);
+      const int place = seg.len - seg.nq + min(token, seg.nq - 1);
       col_nm[c] = 0.f;
       col_nm[NQ + c] = s;
       col_nm[2 * NQ + c] = -1.f;
-      reinterpret_cast<int*>(col_nm)[3 * NQ + c] = p.causal ? min(place + 1, seg.r.len) : seg.r.len;
+      reinterpret_cast<int*>(col_nm)[3 * NQ + c] = p.causal ? min(place + 1, seg.len) : seg.len;
       reinterpret_cast<int*>(col_nm)[4 * NQ + c] = p.window >= 0 ? max(place - p.window, 0) : 0;
     }
   }
@@ -488,6 +577,10 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       ptx::mbar_init(bar(C::kScFull + s), 1);
       ptx::mbar_init(bar(C::kScEmpty + s), C::kSoftWarps);
     }
+    for (int s = 0; s < C::kSegRing; ++s) {
+      ptx::mbar_init(bar(C::kSegFull + s), 1);
+      ptx::mbar_init(bar(C::kSegEmpty + s), C::kSoftWarps + 3);  // softmax, producer, MMA, query rows
+    }
     ptx::mbar_init(bar(C::kDrain), 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
@@ -500,8 +593,10 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     ptx::prefetch_tmap(&tmK);
     ptx::prefetch_tmap(&tmV);
   }
-  const PagedStart start = paged_start<NQ>(p, reinterpret_cast<long long*>(smem + C::kScan),
-                                           reinterpret_cast<int*>(smem + C::kScan + 256));
+  PagedStart start{};
+  if (p.batch > kPagedWarpBatch)
+    start = paged_start_cta<NQ>(p, reinterpret_cast<long long*>(smem + C::kScan),
+                                reinterpret_cast<int*>(smem + C::kScan + 256));
   if (threadIdx.x < 2) p.share[(2 * blockIdx.x + threadIdx.x) * kShareInts] = -1;
   ptx::tc_fence_before();
   __syncthreads();
@@ -514,7 +609,22 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
   auto wait = [&](int slot, uint32_t parity) {
     if (ok) ok = W.wait_warp(bar(slot), parity & 1u);
   };
-  PagedWalk<NQ> walk(p, start);
+  // Readers of the segment ring: every warp but the walking one (the scales').
+  int seg_reads = 0;
+  auto next_segment = [&](PagedSegment& seg) -> bool {
+    const int at = seg_reads % C::kSegRing;
+    wait(C::kSegFull + at, (uint32_t)(seg_reads / C::kSegRing));
+    ++seg_reads;
+    const int4* src = reinterpret_cast<const int4*>(smem + C::kSegs) + at * kSegVecs;
+    int4 v[kSegVecs];
+#pragma unroll
+    for (int k = 0; k < kSegVecs; ++k) v[k] = src[k];
+    seg = PagedSegment{v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w,
+                       v[2].x, v[2].y, v[2].z, v[2].w, v[3].x, v[3].y, v[3].z, v[3].w};
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(bar(C::kSegEmpty + at));
+    return ok && seg.n >= 0;  // after a failed wait the ring may hold anything
+  };
   PagedSegment seg;
 
   if (warp < C::kSoftWarps) {
@@ -528,25 +638,29 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     const int page = t >> p.block_shift;
     int g = 0;  // tiles so far
     uint32_t fills = 0;  // ring fills of the segments before
-    for (int n = 0; walk.next(seg); ++n) {
-      const int rows = min(NQ, seg.r.nq * p.group - seg.qt * NQ) - c_first;  // of this warpgroup; may be <= 0
+    auto split = [&](const PagedSegment& s, int n) {
+      if (n >= 2) wait(C::kColEmpty + (n & 1), (uint32_t)((n >> 1) - 1));
+      split_query_rows<T, D, NQ, 1>(p, s, smem, n, warp, C::kSoftWarps);
+      ptx::named_bar_sync(7, 32 * C::kSoftWarps);
+      if (threadIdx.x == 0) ptx::mbar_arrive(bar(C::kQFull + (n & 1)));
+    };
+    // One answer for all softmax warps, or those that go on would miss the others at a barrier.
+    auto next_for_all = [&](PagedSegment& s) {
+      const bool more = next_segment(s);
+      return !ptx::named_bar_or(7, 32 * C::kSoftWarps, !more);
+    };
+    bool more = next_for_all(seg);
+    // The first rows are split here in any case: these warps have nothing else to do yet.
+#pragma unroll 1
+    for (int n = 0; more; ++n) {
+      const int rows = seg.rows - c_first;  // of this warpgroup; may be <= 0
       float* const col_nm = reinterpret_cast<float*>(smem + C::kCol) + (n & 1) * 5 * NQ + c_first;  // kPagedTop - max
       const float* const col_q = col_nm + NQ;  // q's scale
       float* const col_f = col_nm + 2 * NQ;    // factor of a moved maximum, -1 before the first; 1 / sum at the end
       const int* const col_hi = reinterpret_cast<const int*>(col_nm + 3 * NQ);  // tokens [lo, hi) are seen
       const int* const col_lo = reinterpret_cast<const int*>(col_nm + 4 * NQ);
-      if (n == 0) {  // these warps have nothing else to do yet; later segments' rows are split ahead
-        split_query_rows<T, D, NQ>(p, seg, smem, 0, warp, C::kSoftWarps);
-        ptx::named_bar_sync(7, 32 * C::kSoftWarps);
-        if (threadIdx.x == 0) ptx::mbar_arrive(bar(C::kQFull));
-      }
+      if (n == 0) split(seg, 0);
       wait(C::kQFull + (n & 1), (uint32_t)(n >> 1));
-      const PagedTileRows tile_rows(p, seg.qt * NQ);
-      // Tiles within [lo_all, hi_all) are seen whole by every row of the tile.
-      const int p_first = seg.r.len - seg.r.nq + tile_rows.token0;
-      const int p_last = seg.r.len - seg.r.nq + (min(seg.r.nq * p.group, (seg.qt + 1) * NQ) - 1) / p.group;
-      const int hi_all = p.causal ? min(seg.r.len, p_first + 1) : seg.r.len;
-      const int lo_all = p.window >= 0 ? max(0, p_last - p.window) : 0;
       float2 l[NC / 2];
 #pragma unroll
       for (int c = 0; c < NC / 2; ++c) l[c] = make_float2(0.f, 0.f);
@@ -586,13 +700,13 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           most = ptx::fmax3(most, d[c].x, d[c].y);
           most = ptx::fmax3(most, d[c + 1].x, d[c + 1].y);
         }
-        const bool masked = pos0 < lo_all || pos0 + kPagedTile > hi_all;
+        const bool masked = pos0 < seg.lo_all || pos0 + kPagedTile > seg.hi_all;
         if (masked) {
 #pragma unroll
           for (int c = 0; c < NC; ++c)
             if (pos < col_lo[c] || pos >= col_hi[c]) (c & 1 ? d[c / 2].y : d[c / 2].x) = -INFINITY;
         }
-        const bool left = pos0 < lo_all;
+        const bool left = pos0 < seg.lo_all;
         const bool move = force || left ? true : ptx::named_bar_or(1 + wg, 128, most > kPagedMost);
         force = left;
         if (move) {
@@ -653,11 +767,12 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
             __half2 a = __floats2half2_rn(e0.x, e0.y), b = __floats2half2_rn(e1.x, e1.y);
 #pragma unroll
             for (int j2 = 0; j2 < C::kTerms; ++j2) {
-              const uint32_t ea = e4m3x2_of_half2(a), eb = e4m3x2_of_half2(b);
-              term[j2][k >> 2] = ea | (eb << 16);
+              term[j2][k >> 2] = e4m3x4_of_half2(a, b);
               if (j2 + 1 < C::kTerms) {
-                a = __hsub2(a, half2_of_e4m3x2(ea));
-                b = __hsub2(b, half2_of_e4m3x2(eb));
+                __half2 ra, rb;
+                half2_of_e4m3x4(term[j2][k >> 2], ra, rb);
+                a = __hsub2(a, ra);
+                b = __hsub2(b, rb);
               }
             }
           }
@@ -667,11 +782,11 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
         }
         // Tokens that no row sees: their V rows hold anything (NaN, an older tile), and 0 * NaN
         // would reach O. Clear them.
-        if (pos0 < seg.span.lo || pos0 + kPagedTile > seg.span.hi) {
+        if (pos0 < seg.lo || pos0 + kPagedTile > seg.hi) {
           const uint32_t fill = fills + (j + 1 < seg.n ? 2 * j + 2 : 2 * j + 1);  // V(j)'s place in the ring
           const int slot = (int)(fill % NS);
           wait(C::kKvFull + slot, fill / NS);
-          if (wg == 0 && (pos < seg.span.lo || pos >= seg.span.hi)) {
+          if (wg == 0 && (pos < seg.lo || pos >= seg.hi)) {
 #pragma unroll 1
             for (int k = 0; k < C::kChunks * C::kRow; k += 16)
               ptx::st_shared_v4(sbase + slot * C::kSlotBytes + (k / C::kRow) * (kPagedTile * C::kRow) + t * C::kRow +
@@ -684,6 +799,13 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
         if (lane == 0) ptx::mbar_arrive(bar(C::kPFull + sb));
       }
       fills += 2 * seg.n;
+      // The next segment's scores are under way while this one's result is written. (Q's buffer is
+      // free: the last S of this segment is here.)
+      PagedSegment then;
+      if (C::kSelfSplit) {
+        more = next_for_all(then);
+        if (more) split(then, n + 1);
+      }
 
       // ---- the segment's result ----
       {
@@ -702,14 +824,9 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           p.part_lse[(long long)seg.slot * NQ + c_first + t] = lse2;
         } else if (p.lse != nullptr) {
           int token, head;
-          tile_rows.row(p, c_first + t, token, head);
-          p.lse[(long long)(seg.h * p.group + head) * p.total_q + seg.r.q0 + token] = lse2 * 0.69314718055994531f;
+          paged_row(p, seg.token0, seg.head0, c_first + t, token, head);
+          p.lse[(long long)(seg.h * p.group + head) * p.total_q + seg.q0 + token] = lse2 * 0.69314718055994531f;
         }
-      }
-      if (seg.slot >= 0 && threadIdx.x == 0) {
-        int4* at = reinterpret_cast<int4*>(p.share + seg.slot * kShareInts);
-        at[0] = make_int4(seg.r.q0, seg.h, seg.qt * NQ, min(NQ, seg.r.nq * p.group - seg.qt * NQ));
-        at[1] = make_int4(seg.c0, seg.c1, 0, 0);
       }
       if (seg.n > 0) wait(C::kPvDone + ((g - 1) & 1), (uint32_t)((g - 1) >> 1));
       ptx::tc_fence_after();
@@ -724,43 +841,45 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           ptx::tmem_ld16(tmem + lane_off + (uint32_t)(2 * NQ + ch * NQ + c_first + c), v);
           ptx::tmem_wait_ld();
           ptx::reg_fence16(v);
-          int i, hq;
-          tile_rows.row(p, c_first + c, i, hq);
+          int token, head;
+          paged_row(p, seg.token0, seg.head0, c_first + c, token, head);
+          T* o = static_cast<T*>(p.o) + (seg.q0 + token) * p.o_st + (seg.h * p.group + head) * p.o_sh + d;
+          float* part = p.part_o + ((long long)seg.slot * NQ + c_first + c) * D + d;
+          const long long wrap = p.o_st - (p.group - 1) * p.o_sh;  // from a token's last head to the next's first
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
+            if (c + k >= rows) break;
             const float inv = col_f[c + k];
             // A row that saw nothing has no O (its tiles may not have run): 0, whatever TMEM holds.
             const float val = inv == 0.f ? 0.f : __uint_as_float(v[k]) * inv;
-            if (c + k < rows && d < D) {
-              if (seg.slot >= 0)
-                p.part_o[((long long)seg.slot * NQ + c_first + c + k) * D + d] = val;
-              else
-                static_cast<T*>(p.o)[(long long)(seg.r.q0 + i) * p.o_st + (long long)(seg.h * p.group + hq) * p.o_sh +
-                                     d] = (T)val;
+            if (d < D) {
+              if (seg.slot >= 0) part[k * D] = val;
+              else *o = (T)val;
             }
-            if (++hq == p.group) {
-              hq = 0;
-              ++i;
-            }
+            const bool last = ++head == p.group;
+            o += last ? wrap : p.o_sh;
+            head = last ? 0 : head;
           }
         }
       }
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar(C::kColEmpty + (n & 1)));
+      if (!C::kSelfSplit) more = next_for_all(then);
+      seg = then;
     }
   } else if (warp == kWarpProd) {
     // ========================================================== producer ===
     // Ring order per segment: K(0); then K(j + 1), V(j) for each j: the MMA warp's order.
     // Lane i loads page i of the tile; pages that no row sees are left out.
-    const uint64_t policy = p.stream_once ? ptx::policy_evict_first() : ptx::policy_evict_last();
+    const uint64_t policy = p.one_tile ? ptx::policy_evict_first() : ptx::policy_evict_last();
     const int pages = kPagedTile >> p.block_shift;
     uint32_t fills = 0;
     // Block ids of four tiles at a time, one batch ahead: lane 8 i + k holds page k of the i-th.
     // -2: not loaded; -1: outside the cache, reads as zeros.
     auto page_ids = [&](const PagedSegment& s, int tile) -> int {
       const int at = (tile + (lane >> 3)) * kPagedTile + ((lane & 7) << p.block_shift);
-      if ((lane & 7) >= pages || at >= s.span.hi || at + (1 << p.block_shift) <= s.span.lo) return -2;
+      if ((lane & 7) >= pages || at >= s.hi || at + (1 << p.block_shift) <= s.lo) return -2;
       const int id = __ldg(p.block_table + (long long)s.b * p.table_stride + (at >> p.block_shift));
       return id >= 0 && id < p.num_blocks ? id : -1;
     };
@@ -784,7 +903,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       __syncwarp();
     };
     // The next segment and its first block ids are looked up while the ring is full of this one.
-    bool more = walk.next(seg);
+    bool more = next_segment(seg);
     int ids = -2, ahead = -2;
     if (more) {
       ids = page_ids(seg, seg.tile);
@@ -794,7 +913,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       PagedSegment then;
       int then_ids = -2, then_ahead = -2;
       auto look = [&]() {
-        more = walk.next(then);
+        more = next_segment(then);
         if (more) {
           then_ids = page_ids(then, then.tile);
           then_ahead = page_ids(then, then.tile + 4);
@@ -901,7 +1020,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       }
       ++gp;
     };
-    for (; walk.next(seg); ++n) {
+    for (; next_segment(seg); ++n) {
       wait(C::kQFull + (n & 1), (uint32_t)(n >> 1));
       if (seg.n == 0) {
         if (lane == 0) ptx::mbar_arrive(bar(C::kQEmpty + n % C::kQBufs));
@@ -923,15 +1042,37 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     // Four tiles' loads at a time: lane 8 i + k looks after page k of the i-th.
     const int pages = kPagedTile >> p.block_shift;
     float4* const scales = reinterpret_cast<float4*>(smem + C::kScales);
+    if (p.batch <= kPagedWarpBatch) start = paged_start_warp<NQ>(p);
+    PagedWalk<NQ> walk(p, start);
+    int published = 0;
+    auto publish = [&](const PagedSegment& x) {
+      const int at = published % C::kSegRing;
+      wait(C::kSegEmpty + at, (uint32_t)(published / C::kSegRing) ^ 1u);
+      ++published;
+      int4* dst = reinterpret_cast<int4*>(smem + C::kSegs) + at * kSegVecs;
+      if (lane == 0) {
+        dst[0] = make_int4(x.b, x.h, x.q0, x.nq);
+        dst[1] = make_int4(x.len, x.lo, x.hi, x.tile);
+        dst[2] = make_int4(x.n, x.slot, x.rows, x.token0);
+        dst[3] = make_int4(x.head0, x.lo_all, x.hi_all, 0);
+        ptx::mbar_arrive(bar(C::kSegFull + at));
+      }
+      __syncwarp();
+    };
     int g = 0;
-    while (walk.next(seg)) {
+    seg = walk.next();
+    publish(seg);
+    while (seg.n >= 0) {
+      // One segment ahead of its scales, so that the other roles can look ahead too.
+      const PagedSegment then = walk.next();
+      publish(then);
 #pragma unroll 1
       for (int j0 = 0; j0 < seg.n; j0 += 4) {
         const int j = j0 + (lane >> 3), page = lane & 7;
         const int at = (seg.tile + j) * kPagedTile + (page << p.block_shift);
         // Pages that are not there: zero scores and values, and a V scale too small to move a maximum.
         float4 sc = make_float4(0.f, -100.f, 1.f / kPagedLeastScale, 0.f);
-        if (j < seg.n && page < pages && at < seg.span.hi && at + (1 << p.block_shift) > seg.span.lo) {
+        if (j < seg.n && page < pages && at < seg.hi && at + (1 << p.block_shift) > seg.lo) {
           const int id = __ldg(p.block_table + (long long)seg.b * p.table_stride + (at >> p.block_shift));
           if (id >= 0 && id < p.num_blocks) {
             const float a = __ldg(p.k_scale + (long long)id * p.heads_kv + seg.h);
@@ -948,6 +1089,8 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           if (lane == 0) ptx::mbar_arrive(bar(C::kScFull + g % C::kScaleRing));
         }
       }
+      seg = then;
+      if (!ok) break;
     }
     if (p.zero_rest) {  // rows behind a request and before the next (or the first)
       for (int b = (int)blockIdx.x; b < p.batch; b += gridDim.x) {
@@ -970,11 +1113,11 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
   } else if (warp == kWarpQ) {
     // ======================================================== query rows ===
     // Ahead of the softmax, from the second segment on.
-    for (int n = 0; walk.next(seg); ++n) {
-      if (n == 0) continue;
+    for (int n = 0; next_segment(seg); ++n) {
+      if (n == 0 || C::kSelfSplit) continue;
       if (n >= C::kQBufs) wait(C::kQEmpty + n % C::kQBufs, (uint32_t)(n / C::kQBufs - 1));
       if (n >= 2) wait(C::kColEmpty + (n & 1), (uint32_t)((n >> 1) - 1));
-      split_query_rows<T, D, NQ>(p, seg, smem, n, 0, 1);
+      split_query_rows<T, D, NQ, 4>(p, seg, smem, n, 0, 1);
       if (lane == 0) ptx::mbar_arrive(bar(C::kQFull + (n & 1)));
     }
   }
@@ -1003,8 +1146,7 @@ __global__ void __launch_bounds__(kCombineThreads) attn_paged_combine_kernel(con
     const int4* at = reinterpret_cast<const int4*>(p.share + (2 * blockIdx.x + side) * kShareInts);
     const int4 item = at[0], ctas = at[1];
     if (item.x < 0) continue;
-    const int h = item.y, rows = item.w, c0 = ctas.x, k_parts = ctas.y - ctas.x + 1;
-    const PagedTileRows tile_rows(p, item.z);
+    const int h = item.y, rows = item.z, c0 = ctas.x, k_parts = ctas.y - ctas.x + 1;
     const bool alone = k_parts <= 4;  // a warp joins a row by itself
     const int lanes = alone ? kWarps : 1;
     for (int c = ((int)blockIdx.x - c0) * lanes + (alone ? warp : 0); c < rows; c += k_parts * lanes) {
@@ -1060,7 +1202,7 @@ __global__ void __launch_bounds__(kCombineThreads) attn_paged_combine_kernel(con
         if (warp != 0) continue;
       }
       int i, hq;
-      tile_rows.row(p, c, i, hq);
+      paged_row(p, item.w, ctas.z, c, i, hq);
       i += item.x;
       hq += h * p.group;
       const float inv = sum == 0.f ? 0.f : 1.f / sum;

@@ -374,7 +374,7 @@ int forward_paged(const apex_attn_paged_args* a, void* workspace, size_t bytes, 
   // A window that reaches past every table hides nothing.
   p.window = a->window_left < a->table_width * a->block_size ? a->window_left : -1;
   p.zero_rest = a->zero_rest && a->cu_seqlens_q ? 1 : 0;
-  p.stream_once = group * a->max_seqlen_q <= tile ? 1 : 0;
+  p.one_tile = group * a->max_seqlen_q <= tile ? 1 : 0;
   p.scale_log2 = a->sm_scale * 1.4426950408889634f;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return a->dtype == APEX_ATTN_BF16 ? launch_dim<__nv_bfloat16>(a->head_dim, tile, p, mk, mv, dev, d.num_sms, s)
