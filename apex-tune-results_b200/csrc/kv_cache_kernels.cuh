@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(1024) kv_release_kernel(const PlanParams p) {
 }
 
 // ----------------------------------------------------------------------- append --
-constexpr int kAppendThreads = 128;
+constexpr int kAppendWarps = 8;
 constexpr int kMinScaleExponent = -100;
 
 struct AppendParams {
@@ -207,7 +207,7 @@ struct AppendParams {
   long long x_st[2], x_sh[2];  // token and head strides (elements)
   long long c_sb[2], c_sh[2], c_st[2];  // block, head and token strides of the cache (bytes)
   long long num_slots;         // num_blocks * block
-  int total, heads, head_dim, block_shift, window;
+  int total, heads, block_shift, window;  // window: at most 32 tokens
 };
 
 // The smallest power of two, at least 2^-100, whose 448-fold is at least `amax` (>= 0,
@@ -219,9 +219,15 @@ __device__ __forceinline__ float append_scale(float amax) {
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-__device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));  // a: low byte
+// Four fp32 values to e4m3, a.x in the lowest byte; nearest even, at most 448, NaN stays.
+__device__ __forceinline__ uint32_t e4m3x4(float2 a, float2 b) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+      "mov.b32 %0, {lo, hi};\n\t}"
+      : "=r"(r)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
 
@@ -259,89 +265,137 @@ struct Elem<__half> {
 // floating format it would not make the others more exact. Values that are not finite leave
 // the scale alone and are stored as NaN.
 //
-// One CTA takes the runs that start in its window of `window` tokens, for one head of K or V.
+// A warp takes the runs that start in its CTA's window of tokens, for one head of K or V: a lane
+// looks at one token of the window each, so that finding the runs is one load. A run of up to
+// 2048 values (16 tokens of 128) stays in registers between the pass for the maximum and the
+// one for the codes; a longer one is read again, from the L2.
 // Bound: DRAM for prompts (2 bytes read, 1 written per value), latency for a decode step.
-template <typename T>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendParams p) {
-  __shared__ uint32_t warp_max[kAppendThreads / 32];
-  __shared__ int run_s;
-  const int kv = blockIdx.z, h = blockIdx.y;
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * kAppendWarps, 3) kv_append_kernel(const AppendParams p) {
+  constexpr int kPerRow = D / 8;   // 8 values (16 bytes of input) per lane and step
+  constexpr int kAhead = 8;        // steps in registers at once
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int unit = blockIdx.y * kAppendWarps + warp;
+  if (unit >= 2 * p.heads) return;
+  const int kv = unit >= p.heads, h = unit - kv * p.heads;
   const int block = 1 << p.block_shift;
-  const int chunks = p.head_dim >> 4;  // 16 values per thread and step
-  const int t_end = min(p.total, (int)(blockIdx.x + 1) * p.window);
-  for (int t = blockIdx.x * p.window; t < t_end; ++t) {
-    const long long slot = __ldg(p.slots + t);
-    if (slot < 0 || slot >= p.num_slots) continue;
+  const int t0 = blockIdx.x * p.window;
+  // Lane i looks at token t0 + i, beyond the window too. It follows the token before it if its
+  // slot does and no block begins there; a run begins where one in the window does not follow.
+  const bool real = t0 + lane < p.total;
+  const long long mine = real ? __ldg(p.slots + t0 + lane) : -1;
+  long long prev = __shfl_up_sync(0xffffffffu, mine, 1);
+  if (lane == 0) prev = t0 > 0 ? __ldg(p.slots + t0 - 1) : -2;
+  const unsigned follows =
+      __ballot_sync(0xffffffffu, real && mine == prev + 1 && (mine & (block - 1)) != 0 && prev >= 0);
+  const unsigned in_cache = __ballot_sync(0xffffffffu, lane < p.window && mine >= 0 && mine < p.num_slots);
+  for (unsigned runs = in_cache & ~follows; runs != 0; runs &= runs - 1) {
+    const int first = __ffs(runs) - 1;
+    const int t = t0 + first;
+    const long long slot = __shfl_sync(0xffffffffu, mine, first);
     const int o = (int)(slot & (block - 1));
-    if (o != 0 && t > 0 && __ldg(p.slots + t - 1) == slot - 1) continue;  // inside an earlier run
-    if (threadIdx.x == 0) run_s = min(block - o, p.total - t);
-    __syncthreads();
-    for (int i = threadIdx.x; i < min(block - o, p.total - t); i += kAppendThreads)
-      if (__ldg(p.slots + t + i) != slot + i) atomicMin(&run_s, i);
-    __syncthreads();
-    const int n = run_s;
-    const T* x = static_cast<const T*>(p.x[kv]) + (long long)t * p.x_st[kv] + (long long)h * p.x_sh[kv];
-    uint32_t top = 0;
-    for (int i = threadIdx.x; i < n * chunks; i += kAppendThreads) {
-      const int r = i / chunks, c = i - r * chunks;
-      const uint4* src = reinterpret_cast<const uint4*>(x + (long long)r * p.x_st[kv] + c * 16);
-      const uint4 a = __ldg(src), b = __ldg(src + 1);
-      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t m = w[k] & 0x7fff7fffu;
-        top = __vmaxu2(top, m & ~__vcmpgeu2(m, Elem<T>::kInf2));
+    // Its length, at most to the block's end: the bits of `follows` behind it, and if they reach
+    // the last lane, the tokens behind.
+    const unsigned after = first < 31 ? ~(follows >> (first + 1)) : 1u;  // 0 bits: tokens that follow
+    int n = after != 0 ? __ffs(after) : 32;
+    n = min(n, 32 - first);
+    if (first + n == 32) {
+      const int most = min(block - o, p.total - t);
+      for (int i = n; i < most; i += 32) {
+        const unsigned ends =
+            __ballot_sync(0xffffffffu, i + lane >= most || __ldg(p.slots + t + i + lane) != slot + i + lane);
+        n = i + (ends != 0 ? __ffs(ends) - 1 : 32);
+        if (ends != 0) break;
       }
     }
-    top = max(top & 0xffffu, top >> 16);
-    top = __reduce_max_sync(0xffffffffu, top);
-    if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = top;
+    // This lane's chunks: i = 32 k + lane, 8 values each; 32 chunks are kRows rows.
+    constexpr int kRows = 32 / kPerRow;
+    const int chunks = n * kPerRow;
+    const int row = lane / kPerRow, col = lane % kPerRow * 8;
+    const T* x = static_cast<const T*>(p.x[kv]) + (t + row) * p.x_st[kv] + h * p.x_sh[kv] + col;
+    const long long x_step = kRows * p.x_st[kv];
+    uint4 v[kAhead];
+    auto load = [&](int base) {
+      const T* at = x + base / 32 * x_step;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        v[k] = make_uint4(0, 0, 0, 0);
+        if (base + 32 * k + lane < chunks) v[k] = __ldg(reinterpret_cast<const uint4*>(at + k * x_step));
+      }
+    };
+    // Largest magnitude, compared as bits; what is not finite has the largest bits, and then
+    // (never in a sound model) a second look leaves it out.
+    uint32_t top = 0;
+    for (int base = 0; base < chunks; base += 32 * kAhead) {
+      load(base);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        top = __vmaxu2(top, __vmaxu2(v[k].x & 0x7fff7fffu, v[k].y & 0x7fff7fffu));
+        top = __vmaxu2(top, __vmaxu2(v[k].z & 0x7fff7fffu, v[k].w & 0x7fff7fffu));
+      }
+    }
+    top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+    const bool all_finite = top < (Elem<T>::kInf2 & 0xffffu);
+    if (!all_finite) {
+      top = 0;
+#pragma unroll 1
+      for (int i = lane; i < chunks; i += 32) {
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(x + i / 32 * x_step));
+        const uint32_t u[4] = {w.x & 0x7fff7fffu, w.y & 0x7fff7fffu, w.z & 0x7fff7fffu, w.w & 0x7fff7fffu};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = __vmaxu2(top, u[e] & ~__vcmpgeu2(u[e], Elem<T>::kInf2));
+      }
+      top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+    }
+    const float wanted = append_scale(Elem<T>::to_float2(top).x);
     float* scale = p.scale[kv] + (slot >> p.block_shift) * p.heads + h;
     const float before = o > 0 ? *scale : 0.f;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kAppendThreads / 32; ++k) top = max(top, warp_max[k]);
-    const float wanted = append_scale(Elem<T>::to_float2(top).x);
     const float s = o > 0 ? fmaxf(before, wanted) : wanted;
-    if (threadIdx.x == 0) *scale = s;  // every thread has read it
+    __syncwarp();
+    if (lane == 0) *scale = s;  // every lane has read it
     unsigned char* dst = p.codes[kv] + (slot >> p.block_shift) * p.c_sb[kv] + (long long)h * p.c_sh[kv];
     if (o > 0 && s != before) {
       const float shrink = before / s;
-      for (int i = threadIdx.x; i < o * chunks; i += kAppendThreads) {
-        const int r = i / chunks, c = i - r * chunks;
-        uint4* at = reinterpret_cast<uint4*>(dst + (long long)r * p.c_st[kv] + c * 16);
-        uint4 v = *at;
-        uint32_t* w = &v.x;
+#pragma unroll 4
+      for (int i = lane; i < o * (D / 16); i += 32) {
+        uint4* at = reinterpret_cast<uint4*>(dst + (i / (D / 16)) * p.c_st[kv] + (i % (D / 16)) * 16);
+        uint4 c = *at;
+        uint32_t* w = &c.x;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float2 lo = e4m3x2_to_float2(w[k] & 0xffffu), hi = e4m3x2_to_float2(w[k] >> 16);
-          w[k] = e4m3x2(lo.x * shrink, lo.y * shrink) | (e4m3x2(hi.x * shrink, hi.y * shrink) << 16);
+          w[k] = e4m3x4(make_float2(lo.x * shrink, lo.y * shrink), make_float2(hi.x * shrink, hi.y * shrink));
         }
-        *at = v;
+        *at = c;
       }
     }
     // x / s: by the exact reciprocal when s is a power of two (always, unless the old scale
     // came from elsewhere).
-    const bool power = (__float_as_uint(s) & 0x7fffffu) == 0;
+    const bool plain = all_finite && (__float_as_uint(s) & 0x7fffffu) == 0;
     const float inv = 1.f / s;
-    for (int i = threadIdx.x; i < n * chunks; i += kAppendThreads) {
-      const int r = i / chunks, c = i - r * chunks;
-      const uint4* src = reinterpret_cast<const uint4*>(x + (long long)r * p.x_st[kv] + c * 16);
-      const uint4 a = __ldg(src), b = __ldg(src + 1);
-      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-      uint32_t out[4];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t bad = __vcmpgeu2(w[k] & 0x7fff7fffu, Elem<T>::kInf2);
-        float2 f = Elem<T>::to_float2(w[k] | (bad & 0x7fff7fffu));
-        f = power ? make_float2(f.x * inv, f.y * inv) : make_float2(f.x / s, f.y / s);
-        const uint32_t c2 = e4m3x2(f.x, f.y);
-        out[k >> 1] = (k & 1) ? out[k >> 1] | (c2 << 16) : c2;
+    unsigned char* to = dst + (o + row) * p.c_st[kv] + col;
+    const long long to_step = kRows * p.c_st[kv];
+    auto codes_of = [&](uint32_t a, uint32_t b) -> uint32_t {
+      float2 f = Elem<T>::to_float2(a), g = Elem<T>::to_float2(b);
+      if (plain) {
+        f = __fmul2_rn(f, make_float2(inv, inv));
+        g = __fmul2_rn(g, make_float2(inv, inv));
+      } else {
+        auto quotient = [&](float q) { return isfinite(q) ? q / s : __int_as_float(0x7fffffff); };
+        f = make_float2(quotient(f.x), quotient(f.y));
+        g = make_float2(quotient(g.x), quotient(g.y));
       }
-      *reinterpret_cast<uint4*>(dst + (long long)(o + r) * p.c_st[kv] + c * 16) =
-          make_uint4(out[0], out[1], out[2], out[3]);
+      return e4m3x4(f, g);
+    };
+    for (int base = 0; base < chunks; base += 32 * kAhead) {
+      if (chunks > 32 * kAhead) load(base);
+      unsigned char* at = to + base / 32 * to_step;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (base + 32 * k + lane < chunks)
+          *reinterpret_cast<uint2*>(at + k * to_step) =
+              make_uint2(codes_of(v[k].x, v[k].y), codes_of(v[k].z, v[k].w));
     }
-    __syncthreads();  // run_s and warp_max are written again
   }
 }
 

@@ -130,6 +130,16 @@ int plan(const apex_attn_kv_plan_args* a, bool release, void* stream) {
 }
 
 // ----------------------------------------------------------------------- append --
+template <typename T>
+void launch_append(const apex::AppendParams& p, int head_dim, dim3 grid, cudaStream_t s) {
+  constexpr int kThreads = 32 * apex::kAppendWarps;
+  switch (head_dim) {
+    case 64: apex::kv_append_kernel<T, 64><<<grid, kThreads, 0, s>>>(p); break;
+    case 128: apex::kv_append_kernel<T, 128><<<grid, kThreads, 0, s>>>(p); break;
+    default: apex::kv_append_kernel<T, 256><<<grid, kThreads, 0, s>>>(p);
+  }
+}
+
 int append(const apex_attn_kv_append_args* a, void* stream) {
   if (!a || !a->k || !a->v || !a->k_cache || !a->v_cache || !a->k_scale || !a->v_scale || !a->slots)
     return APEX_ATTN_ERR_INVALID_ARGUMENT;
@@ -174,18 +184,16 @@ int append(const apex_attn_kv_append_args* a, void* stream) {
   p.num_slots = (long long)a->num_blocks * a->block_size;
   p.total = a->total;
   p.heads = a->heads_kv;
-  p.head_dim = a->head_dim;
   p.block_shift = shift;
-  // One token per CTA while all CTAs fit the device at once (decode: every token is a run of
-  // its own); longer windows, up to the smallest block, once there are more.
-  const long long ctas = 2LL * a->heads_kv * a->total;
-  p.window = (int)std::max(1LL, std::min(16LL, ctas / (16LL * d.num_sms)));
-  const dim3 grid((unsigned)((a->total + p.window - 1) / p.window), (unsigned)a->heads_kv, 2);
+  // A window of one token while that leaves at most four CTAs for each of the device's places
+  // (decode: every token is a run of its own); else windows that a run mostly fills.
+  const int groups = (2 * a->heads_kv + apex::kAppendWarps - 1) / apex::kAppendWarps;
+  const bool few = (long long)a->total * groups <= 4LL * 8 * d.num_sms;
+  p.window = few ? 1 : std::min(a->block_size, 32);
+  const dim3 grid((unsigned)((a->total + p.window - 1) / p.window), (unsigned)groups);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (a->dtype == APEX_ATTN_BF16)
-    apex::kv_append_kernel<__nv_bfloat16><<<grid, apex::kAppendThreads, 0, s>>>(p);
-  else
-    apex::kv_append_kernel<__half><<<grid, apex::kAppendThreads, 0, s>>>(p);
+  if (a->dtype == APEX_ATTN_BF16) launch_append<__nv_bfloat16>(p, a->head_dim, grid, s);
+  else launch_append<__half>(p, a->head_dim, grid, s);
   return launched();
 }
 
