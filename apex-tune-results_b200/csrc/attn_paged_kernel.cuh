@@ -88,33 +88,36 @@ struct PagedCfg {
   static constexpr int kChunks = (D + 127) / 128;
   static constexpr uint32_t kSwizzle = kRow == 128 ? 2 : 4;
   static constexpr int kTerms = std::is_same<T, __half>::value ? 3 : 2;  // of q
-  static constexpr int kNC = NQ < 32 ? NQ : 32;          // query rows per softmax warpgroup
-  static constexpr int kWG = NQ / kNC;
+  static constexpr bool kQueryMajor = NQ == 128;
+  static constexpr int kWG = kQueryMajor ? 4 : 1;        // softmax warpgroups
+  static constexpr int kNC = 32 < NQ ? 32 : NQ;          // S values per thread: query rows, or tokens
   static constexpr int kSoftWarps = 4 * kWG;
   static constexpr int kThreads = 128 * (kWG + 1);
   // Two CTAs per SM cover each other's latencies where their shared memory fits.
   static constexpr int kCtas = (D <= 128 && NQ <= 32) ? 2 : 1;
   static constexpr int kSlotBytes = kPagedTile * D;      // one K or V tile
-  static constexpr int kPBufs = 2;
   static constexpr int kQBytes = kTerms * NQ * D;        // one segment's query rows
   static constexpr int kPTerm = kPagedTile * NQ;         // one term of one P buffer
   static constexpr int kBudget = kCtas == 2 ? 115712 : 232448;
-  static constexpr int kMiscBytes = 2240 + NQ * 56;      // what the plan below adds
-  static constexpr int slots(int q_bufs) {
-    return (kBudget - q_bufs * kQBytes - kPBufs * kTerms * kPTerm - kMiscBytes) / kSlotBytes;
+  static constexpr int kMiscBytes = 2240 + NQ * 88;      // what the plan below adds
+  static constexpr int slots(int q_bufs, int p_bufs) {
+    return (kBudget - q_bufs * kQBytes - p_bufs * kTerms * kPTerm - kMiscBytes) / kSlotBytes;
   }
-  // The next segment's query rows are split ahead of time where that leaves four ring slots.
-  // Larger tiles' rows are too many for one warp: the softmax warps split them between segments.
-  static constexpr bool kSelfSplit = NQ > 32;
-  static constexpr int kQBufs = !kSelfSplit && slots(2) >= 4 ? 2 : 1;
-  static constexpr int kNS = slots(kQBufs) > 12 ? 12 : slots(kQBufs);  // ring slots
-  static_assert(kNS >= 3, "the ring needs K(j + 1) beside K(j) and V(j)");
+  static constexpr int kPBufs = slots(1, 2) >= 3 ? 2 : 1;
+  // The next segment's query rows are split ahead of time, by a warp of their own, where that
+  // leaves four ring slots; a query-major tile's are too many for one warp, and the softmax
+  // warps split them between segments.
+  static constexpr bool kSelfSplit = kQueryMajor;
+  static constexpr int kQBufs = !kSelfSplit && slots(2, kPBufs) >= 4 ? 2 : 1;
+  static constexpr int kNS = slots(kQBufs, kPBufs) > 12 ? 12 : slots(kQBufs, kPBufs);  // ring slots
+  static_assert(kNS >= 2, "the ring needs K(j + 1) beside V(j)");
   static constexpr int kScaleRing = 8;
   static constexpr int kSegRing = 4;
-  // TMEM: S buffers at 0 and NQ, O (one block of NQ columns per 128 of the head dim) from 2 NQ.
-  static constexpr int kTmemCols = (2 + kChunks) * NQ <= 64 ? 64
-                                   : ((2 + kChunks) * NQ <= 128 ? 128 : ((2 + kChunks) * NQ <= 256 ? 256 : 512));
-  static_assert((2 + kChunks) * NQ <= 512 && kCtas * kTmemCols <= 512, "TMEM plan");
+  // TMEM: S buffers at 0 and NQ, O from 2 NQ on (token-major: a block of NQ columns per 128 of
+  // the head dim; query-major: the head dim).
+  static constexpr int kTmemUsed = kQueryMajor ? 2 * NQ + D : (2 + kChunks) * NQ;
+  static constexpr int kTmemCols = kTmemUsed <= 64 ? 64 : (kTmemUsed <= 128 ? 128 : (kTmemUsed <= 256 ? 256 : 512));
+  static_assert(kTmemUsed <= 512 && kCtas * kTmemCols <= 512, "TMEM plan");
   // shared-memory plan
   static constexpr int kQ = kNS * kSlotBytes;
   static constexpr int kP = kQ + kQBufs * kQBytes;
@@ -125,8 +128,8 @@ struct PagedCfg {
                        kSegEmpty = kSegFull + kSegRing, kDrain = kSegEmpty + kSegRing, kNumBars = kDrain + 1;
   static constexpr int kScales = (kBars + kNumBars * 8 + 15) / 16 * 16;  // float4 [kScaleRing][8 pages]
   static constexpr int kCol = kScales + kScaleRing * 8 * 16;  // two of, per query row: -m, q scale, factor, hi, lo
-  static constexpr int kRed = kCol + 2 * 5 * NQ * 4;          // [kWG][4 warps][kNC]
-  static constexpr int kSegs = (kRed + 4 * NQ * 4 + 15) / 16 * 16;       // int4 [kSegRing][kSegVecs]
+  static constexpr int kRed = kCol + 2 * 5 * NQ * 4;          // token-major [4 warps][NQ], query-major [3][4 warpgroups][128]
+  static constexpr int kSegs = (kRed + (kQueryMajor ? 12 : 4) * NQ * 4 + 15) / 16 * 16;       // int4 [kSegRing][kSegVecs]
   static constexpr int kScan = kSegs + kSegRing * 5 * 16;                // long long [32], found request
   static constexpr int kMisc = kScan + 32 * 8 + 16;
   static constexpr int kBytes = kMisc + 16;
@@ -464,7 +467,15 @@ __device__ __forceinline__ void split_query_rows(const PagedParams& p, const Pag
   constexpr int kStep = 32 / kPerRow;  // rows per warp and step; kAhead steps' loads are under way
   const int lane = (int)(threadIdx.x & 31), chunk = lane % kPerRow;
   float* const col_nm = reinterpret_cast<float*>(smem + C::kCol) + (n & 1) * 5 * NQ;
-  const uint32_t dst = ptx::smem_u32(smem) + C::kQ + (n % C::kQBufs) * C::kQBytes + chunk * (NQ * 16);
+  const uint32_t dst = ptx::smem_u32(smem) + C::kQ + (n % C::kQBufs) * C::kQBytes;
+  // Row c's place: token-major [16-byte chunk of the head dim][row], query-major rows of up to 128
+  // bytes, swizzled as the TMA writes K.
+  auto place_of = [&](int c) -> uint32_t {
+    if constexpr (!C::kQueryMajor) return dst + chunk * (NQ * 16) + c * 16;
+    constexpr int kUnits = C::kRow / 16;
+    const uint32_t off = (uint32_t)(c * C::kRow + chunk % kUnits * 16);
+    return dst + chunk / kUnits * (NQ * C::kRow) + (off ^ (((off >> 7) & (kUnits - 1)) << 4));
+  };
   const T* const q = static_cast<const T*>(p.q) + (long long)seg.q0 * p.q_st +
                      (long long)(seg.h * p.group) * p.q_sh + chunk * 16;
   uint4 na[kAhead], nb[kAhead];
@@ -520,8 +531,10 @@ __device__ __forceinline__ void split_query_rows(const PagedParams& p, const Pag
     }
 #pragma unroll
     for (int j = 0; j < C::kTerms; ++j)
-      ptx::st_shared_v4(dst + j * NQ * D + c * 16, term[j][0], term[j][1], term[j][2], term[j][3]);
-    if (chunk == 0) {
+      ptx::st_shared_v4(place_of(c) + j * NQ * D, term[j][0], term[j][1], term[j][2], term[j][3]);
+    if (C::kQueryMajor) {
+      if (chunk == 0) col_nm[NQ + c] = s;
+    } else if (chunk == 0) {
       int token, head;
       paged_row(p, seg.token0, seg.head0, c, token, head);
       const int place = seg.len - seg.nq + min(token, seg.nq - 1);
@@ -639,7 +652,6 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     int g = 0;  // tiles so far
     uint32_t fills = 0;  // ring fills of the segments before
     auto split = [&](const PagedSegment& s, int n) {
-      if (n >= 2) wait(C::kColEmpty + (n & 1), (uint32_t)((n >> 1) - 1));
       split_query_rows<T, D, NQ, 1>(p, s, smem, n, warp, C::kSoftWarps);
       ptx::named_bar_sync(7, 32 * C::kSoftWarps);
       if (threadIdx.x == 0) ptx::mbar_arrive(bar(C::kQFull + (n & 1)));
@@ -649,7 +661,206 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       const bool more = next_segment(s);
       return !ptx::named_bar_or(7, 32 * C::kSoftWarps, !more);
     };
+    // Tokens of tile j that no row sees: their V rows hold anything (NaN, an older tile), and
+    // 0 * NaN would reach O. Clear them. Thread t of the first warpgroup takes token t.
+    auto clear_unseen = [&](int j) {
+      const int pos0 = (seg.tile + j) * kPagedTile, pos = pos0 + t;
+      if (pos0 >= seg.lo && pos0 + kPagedTile <= seg.hi) return;
+      const uint32_t fill = fills + (j + 1 < seg.n ? 2 * j + 2 : 2 * j + 1);  // V(j)'s place in the ring
+      const int slot = (int)(fill % NS);
+      wait(C::kKvFull + slot, fill / NS);
+      if (wg == 0 && (pos < seg.lo || pos >= seg.hi)) {
+#pragma unroll 1
+        for (int k = 0; k < D; k += 16)
+          ptx::st_shared_v4(sbase + slot * C::kSlotBytes + (k / C::kRow) * (kPagedTile * C::kRow) + t * C::kRow +
+                                k % C::kRow, 0, 0, 0, 0);
+      }
+    };
     bool more = next_for_all(seg);
+    if constexpr (C::kQueryMajor) {
+      // Thread: row `t` of the tile, tokens c_first .. c_first + 31; the four warps of a TMEM quarter
+      // share their rows and agree on the maxima.
+      const int quarter = warp & 3;
+      const int tok0 = wg * NC;
+      float* const exchange = reinterpret_cast<float*>(smem + C::kRed);  // [3][4][128]
+#pragma unroll 1
+      for (int n = 0; more; ++n) {
+        if (n == 0) split(seg, 0);
+        const float qs = reinterpret_cast<const float*>(smem + C::kCol)[(n & 1) * 5 * NQ + NQ + t];
+        int token, head;
+        paged_row(p, seg.token0, seg.head0, t, token, head);
+        const int place = seg.len - seg.nq + min(token, seg.nq - 1);
+        const int hi = p.causal ? min(place + 1, seg.len) : seg.len;
+        const int lo = p.window >= 0 ? max(place - p.window, 0) : 0;
+        float nm = 0.f, l = 0.f;  // kPagedTop - max; the row's sum over this thread's tokens
+        bool set = false, force = true;
+#pragma unroll 1
+        for (int j = 0; j < seg.n; ++j, ++g) {
+          const int sb = g & 1;
+          const int pos0 = (seg.tile + j) * kPagedTile;
+          wait(C::kScFull + g % C::kScaleRing, (uint32_t)(g / C::kScaleRing));
+          const float4* const sc = scales + (g % C::kScaleRing) * 8;
+          const float4 sc0 = sc[tok0 >> p.block_shift], sc1 = sc[(tok0 + 16) >> p.block_shift];
+          wait(C::kSFull + sb, (uint32_t)(g >> 1));
+          ptx::tc_fence_after();
+          float2 d[NC / 2];
+          ptx::tmem_ld16(tmem + lane_off + (uint32_t)(sb * NQ + tok0), reinterpret_cast<uint32_t*>(d));
+          ptx::tmem_ld16(tmem + lane_off + (uint32_t)(sb * NQ + tok0 + 16), reinterpret_cast<uint32_t*>(d) + 16);
+          ptx::tmem_wait_ld();
+          ptx::reg_fence16(reinterpret_cast<uint32_t*>(d));
+          ptx::reg_fence16(reinterpret_cast<uint32_t*>(d) + 16);
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            ptx::mbar_arrive(bar(C::kScEmpty + g % C::kScaleRing));
+            ptx::mbar_arrive(bar(C::kSFree + sb));
+          }
+          // d = x + log2 b - m; -inf where the row does not see the token.
+          float most = -INFINITY;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const float a = (half ? sc1.x : sc0.x) * qs, b = (half ? sc1.y : sc0.y) + nm;
+            const float2 a2 = make_float2(a, a), b2 = make_float2(b, b);
+#pragma unroll
+            for (int c = 8 * half; c < 8 * half + 8; ++c) {
+              d[c] = __ffma2_rn(d[c], a2, b2);
+              most = ptx::fmax3(most, d[c].x, d[c].y);
+            }
+          }
+          if (pos0 < seg.lo_all || pos0 + kPagedTile > seg.hi_all) {
+            most = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+              const int pos = pos0 + tok0 + c;
+              float& x = c & 1 ? d[c / 2].y : d[c / 2].x;
+              if (pos < lo || pos >= hi) x = -INFINITY;
+              most = fmaxf(most, x);
+            }
+          }
+          const bool left = pos0 < seg.lo_all;
+          const bool move = force || left ? true : ptx::named_bar_or(1 + quarter, 128, most > kPagedMost);
+          force = left;
+          if (move) {
+            float* const tops = exchange + sb * 4 * NQ;
+            tops[wg * NQ + t] = most;
+            ptx::named_bar_sync(1 + quarter, 128);
+            const float top = fmaxf(fmaxf(tops[t], tops[NQ + t]), fmaxf(tops[2 * NQ + t], tops[3 * NQ + t]));
+            // By how much the maximum moves: up only, but freely the first time.
+            const bool some = top != -INFINITY;
+            const float by = some ? (set ? fmaxf(top - kPagedTop, 0.f) : top - kPagedTop) : 0.f;
+            const float f = set ? ptx::ex2(-by) : 0.f;
+            set = set || some;
+            nm -= by;
+            l *= f;
+            const float2 by2 = make_float2(-by, -by);
+#pragma unroll
+            for (int c = 0; c < NC / 2; ++c) d[c] = __fadd2_rn(d[c], by2);
+            if (j > 0) {
+              wait(C::kPvDone + (sb ^ 1), (uint32_t)((g - 1) >> 1));
+              ptx::tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < D / 4; c += 16) {
+                const uint32_t at = tmem + lane_off + (uint32_t)(2 * NQ + wg * (D / 4) + c);
+                uint32_t v[16];
+                ptx::tmem_ld16(at, v);
+                ptx::tmem_wait_ld();
+                ptx::reg_fence16(v);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
+                ptx::tmem_st16(at, v);
+              }
+              ptx::tmem_wait_st();
+            }
+          }
+          // The P buffer was read by an earlier tile's P V.
+          if (g >= C::kPBufs) wait(C::kPvDone + ((g - C::kPBufs) & 1), (uint32_t)((g - C::kPBufs) >> 1));
+          const uint32_t dst = sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kTerms * C::kPTerm + t * 128;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t term[C::kTerms][4];
+            float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int x = 8 * half + 2 * k;
+              const float2 e0 = make_float2(ptx::ex2(d[x].x), ptx::ex2(d[x].y));
+              const float2 e1 = make_float2(ptx::ex2(d[x + 1].x), ptx::ex2(d[x + 1].y));
+              sum = __fadd2_rn(sum, __fadd2_rn(e0, e1));
+              __half2 a = __floats2half2_rn(e0.x, e0.y), b = __floats2half2_rn(e1.x, e1.y);
+#pragma unroll
+              for (int i = 0; i < C::kTerms; ++i) {
+                term[i][k] = e4m3x4_of_half2(a, b);
+                if (i + 1 < C::kTerms) {
+                  __half2 ra, rb;
+                  half2_of_e4m3x4(term[i][k], ra, rb);
+                  a = __hsub2(a, ra);
+                  b = __hsub2(b, rb);
+                }
+              }
+            }
+            l = fmaf(sum.x + sum.y, half ? sc1.z : sc0.z, l);
+            const uint32_t unit = (uint32_t)(((tok0 >> 4) + half) ^ (t & 7)) << 4;
+#pragma unroll
+            for (int i = 0; i < C::kTerms; ++i)
+              ptx::st_shared_v4(dst + unit + i * C::kPTerm, term[i][0], term[i][1], term[i][2], term[i][3]);
+          }
+          clear_unseen(j);
+          ptx::fence_proxy_async_smem();
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(bar(C::kPFull + sb));
+        }
+        fills += 2 * seg.n;
+        // The next segment's scores are under way while this one's result is written. (Q's buffer is
+        // free: the last S of this segment is here.)
+        PagedSegment then;
+        more = next_for_all(then);
+        if (more) split(then, n + 1);
+
+        // ---- the segment's result: this thread's row, a quarter of its columns ----
+        float* const sums = exchange + 2 * 4 * NQ;
+        sums[wg * NQ + t] = l;
+        ptx::named_bar_sync(1 + quarter, 128);
+        const float sum = sums[t] + sums[NQ + t] + sums[2 * NQ + t] + sums[3 * NQ + t];
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const bool real = t < seg.rows;
+        if (wg == 0 && real) {
+          const float lse2 = sum == 0.f ? -INFINITY : __log2f(sum) - nm;
+          if (seg.slot >= 0)
+            p.part_lse[(long long)seg.slot * NQ + t] = lse2;
+          else if (p.lse != nullptr)
+            p.lse[(long long)(seg.h * p.group + head) * p.total_q + seg.q0 + token] = lse2 * 0.69314718055994531f;
+        }
+        if (seg.n > 0) wait(C::kPvDone + ((g - 1) & 1), (uint32_t)((g - 1) >> 1));
+        ptx::tc_fence_after();
+        T* const o = static_cast<T*>(p.o) + (seg.q0 + token) * p.o_st + (seg.h * p.group + head) * p.o_sh;
+        float* const part = p.part_o + ((long long)seg.slot * NQ + t) * D;
+#pragma unroll 1
+        for (int c = wg * (D / 4); c < (wg + 1) * (D / 4); c += 16) {
+          uint32_t v[16];
+          ptx::tmem_ld16(tmem + lane_off + (uint32_t)(2 * NQ + c), v);
+          ptx::tmem_wait_ld();
+          ptx::reg_fence16(v);
+          if (!real) continue;
+          // A row that saw nothing has no O (its tiles may not have run): 0, whatever TMEM holds.
+#pragma unroll
+          for (int k = 0; k < 16; ++k) v[k] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(v[k]) * inv);
+          if (seg.slot >= 0) {
+#pragma unroll
+            for (int k = 0; k < 16; k += 4)
+              *reinterpret_cast<uint4*>(part + c + k) = make_uint4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+          } else {
+            uint32_t pk[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              pk[k] = DType<T>::pack(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1]));
+            *reinterpret_cast<uint4*>(o + c) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            *reinterpret_cast<uint4*>(o + c + 8) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
+          }
+        }
+        ptx::tc_fence_before();
+        seg = then;
+      }
+    } else {
     // The first rows are split here in any case: these warps have nothing else to do yet.
 #pragma unroll 1
     for (int n = 0; more; ++n) {
@@ -780,32 +991,13 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           for (int j2 = 0; j2 < C::kTerms; ++j2)
             ptx::st_shared_v4(dst + c * 128 + j2 * C::kPTerm, term[j2][0], term[j2][1], term[j2][2], term[j2][3]);
         }
-        // Tokens that no row sees: their V rows hold anything (NaN, an older tile), and 0 * NaN
-        // would reach O. Clear them.
-        if (pos0 < seg.lo || pos0 + kPagedTile > seg.hi) {
-          const uint32_t fill = fills + (j + 1 < seg.n ? 2 * j + 2 : 2 * j + 1);  // V(j)'s place in the ring
-          const int slot = (int)(fill % NS);
-          wait(C::kKvFull + slot, fill / NS);
-          if (wg == 0 && (pos < seg.lo || pos >= seg.hi)) {
-#pragma unroll 1
-            for (int k = 0; k < C::kChunks * C::kRow; k += 16)
-              ptx::st_shared_v4(sbase + slot * C::kSlotBytes + (k / C::kRow) * (kPagedTile * C::kRow) + t * C::kRow +
-                                    k % C::kRow, 0, 0, 0, 0);
-          }
-        }
+        clear_unseen(j);
         ptx::fence_proxy_async_smem();
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(bar(C::kPFull + sb));
       }
       fills += 2 * seg.n;
-      // The next segment's scores are under way while this one's result is written. (Q's buffer is
-      // free: the last S of this segment is here.)
-      PagedSegment then;
-      if (C::kSelfSplit) {
-        more = next_for_all(then);
-        if (more) split(then, n + 1);
-      }
 
       // ---- the segment's result ----
       {
@@ -865,8 +1057,8 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar(C::kColEmpty + (n & 1)));
-      if (!C::kSelfSplit) more = next_for_all(then);
-      seg = then;
+      more = next_for_all(seg);
+    }
     }
   } else if (warp == kWarpProd) {
     // ========================================================== producer ===
@@ -956,9 +1148,12 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     __syncwarp();
   } else if (warp == kWarpMma) {
     // =============================================================== MMA ===
-    constexpr uint32_t kDesc = (1u << 4) | ((uint32_t)(NQ >> 3) << 17) | ((uint32_t)(kPagedTile >> 4) << 24);
-    constexpr uint32_t idS = kDesc;                              // e4m3, fp32 sums, both K-major
-    constexpr uint32_t idPV = kDesc | (1u << 15) | (1u << 16);   // both MN-major
+    // e4m3, fp32 sums, M = 128. S: both operands K-major. P V: V is always MN-major; the weights
+    // are MN-major as the B operand (token-major), K-major as the A operand (query-major).
+    constexpr uint32_t kDesc = (1u << 4) | ((uint32_t)(128 >> 4) << 24);
+    constexpr uint32_t idS = kDesc | ((uint32_t)(NQ >> 3) << 17);
+    constexpr uint32_t idPV = C::kQueryMajor ? kDesc | (1u << 16) | ((uint32_t)(D >> 3) << 17)
+                                             : kDesc | (1u << 15) | (1u << 16) | ((uint32_t)(NQ >> 3) << 17);
     uint32_t reads = 0;  // ring slots consumed
     int gs = 0, gp = 0;  // S and P V tiles issued
     auto acquire = [&]() -> int {
@@ -979,13 +1174,19 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
         for (int ch = 0; ch < C::kChunks; ++ch)
 #pragma unroll
           for (int ks = 0; ks < C::kRow / 32; ++ks) {
-            const uint64_t a = ptx::smem_desc(sbase + slot * C::kSlotBytes + ch * (kPagedTile * C::kRow) + ks * 32, 16,
+            const uint64_t k = ptx::smem_desc(sbase + slot * C::kSlotBytes + ch * (kPagedTile * C::kRow) + ks * 32, 16,
                                               8 * C::kRow, C::kSwizzle);
 #pragma unroll
             for (int j = 0; j < C::kTerms; ++j) {
-              const uint64_t b = ptx::smem_desc(
-                  sbase + C::kQ + (n % C::kQBufs) * C::kQBytes + j * NQ * D + (ch * (C::kRow / 16) + 2 * ks) * (NQ * 16), NQ * 16, 128, 0);
-              ptx::umma_ss_f8_warp(tmem + (uint32_t)(sb * NQ), a, b, idS, acc);
+              const uint32_t rows = sbase + C::kQ + (n % C::kQBufs) * C::kQBytes + j * NQ * D;
+              const uint32_t dS = tmem + (uint32_t)(sb * NQ);
+              if constexpr (C::kQueryMajor) {
+                const uint64_t q = ptx::smem_desc(rows + ch * (NQ * C::kRow) + ks * 32, 16, 8 * C::kRow, C::kSwizzle);
+                ptx::umma_ss_f8_warp(dS, q, k, idS, acc);
+              } else {
+                const uint64_t q = ptx::smem_desc(rows + (ch * (C::kRow / 16) + 2 * ks) * (NQ * 16), NQ * 16, 128, 0);
+                ptx::umma_ss_f8_warp(dS, k, q, idS, acc);
+              }
               acc = 1;
             }
           }
@@ -1001,20 +1202,35 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       const int slot = acquire();
       ptx::tc_fence_after();
       if (ok) {
-#pragma unroll
-        for (int ch = 0; ch < C::kChunks; ++ch)
+        const uint32_t weights = sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kTerms * C::kPTerm;
+        const uint32_t dO = tmem + (uint32_t)(2 * NQ);
+        if constexpr (C::kQueryMajor) {
 #pragma unroll
           for (int ks = 0; ks < kPagedTile / 32; ++ks) {
-            // d = 64: the second 64 rows of M repeat the first (zero stride); nobody reads them.
-            const uint64_t a = ptx::smem_desc(
-                sbase + slot * C::kSlotBytes + ch * (kPagedTile * C::kRow) + ks * 32 * C::kRow, 0, 8 * C::kRow,
-                C::kSwizzle);
+            const uint64_t v = ptx::smem_desc(sbase + slot * C::kSlotBytes + ks * 32 * C::kRow, kPagedTile * C::kRow,
+                                              8 * C::kRow, C::kSwizzle);
 #pragma unroll
             for (int j = 0; j < C::kTerms; ++j) {
-              const uint64_t b = ptx::smem_desc(sbase + C::kP + (sb * C::kTerms + j) * C::kPTerm + ks * 32 * 16, 128, 2048, 0);
-              ptx::umma_ss_f8_warp(tmem + (uint32_t)(2 * NQ + ch * NQ), a, b, idPV, first && ks == 0 && j == 0 ? 0u : 1u);
+              const uint64_t w = ptx::smem_desc(weights + j * C::kPTerm + ks * 32, 16, 1024, 2);
+              ptx::umma_ss_f8_warp(dO, w, v, idPV, first && ks == 0 && j == 0 ? 0u : 1u);
             }
           }
+        } else {
+#pragma unroll
+          for (int ch = 0; ch < C::kChunks; ++ch)
+#pragma unroll
+            for (int ks = 0; ks < kPagedTile / 32; ++ks) {
+              // d = 64: the second 64 rows of M repeat the first (zero stride); nobody reads them.
+              const uint64_t v = ptx::smem_desc(
+                  sbase + slot * C::kSlotBytes + ch * (kPagedTile * C::kRow) + ks * 32 * C::kRow, 0, 8 * C::kRow,
+                  C::kSwizzle);
+#pragma unroll
+              for (int j = 0; j < C::kTerms; ++j) {
+                const uint64_t w = ptx::smem_desc(weights + j * C::kPTerm + ks * 32 * 16, 128, 2048, 0);
+                ptx::umma_ss_f8_warp(dO + (uint32_t)(ch * NQ), v, w, idPV, first && ks == 0 && j == 0 ? 0u : 1u);
+              }
+            }
+        }
         ptx::tc_commit_warp(bar(C::kKvEmpty + slot));
         ptx::tc_commit_warp(bar(C::kPvDone + sb));
       }

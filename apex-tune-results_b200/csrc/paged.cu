@@ -200,13 +200,9 @@ int append(const apex_attn_kv_append_args* a, void* stream) {
 // -------------------------------------------------------------------- attention --
 constexpr int kMaxSms = 160;  // the workspace holds what this many SMs' CTAs may write
 
-// Query rows per tile: the smallest tile that holds all rows of a request's K/V head, else the
-// largest. d = 256 stops at 64 rows (shared memory).
-int query_tile(int rows, int head_dim) {
-  if (rows <= 16) return 16;
-  if (rows <= 32) return 32;
-  return rows <= 64 || head_dim == 256 ? 64 : 128;
-}
+// Query rows per tile: 16 or 32 (tokens as the M side of the products) where they hold all rows of
+// a request's K/V head, else 128 (query rows as the M side).
+int query_tile(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 128; }
 
 struct Workspace {
   size_t share, lse, o, bytes;  // offsets and size
@@ -225,7 +221,7 @@ Workspace workspace_plan(int query_rows, int head_dim) {
 size_t workspace_bytes(int heads_q, int heads_kv, int max_seqlen_q, int head_dim) {
   if (heads_q <= 0 || heads_kv <= 0 || max_seqlen_q <= 0 || head_dim <= 0) return 0;
   const long long rows = (long long)((heads_q + heads_kv - 1) / heads_kv) * max_seqlen_q;
-  return workspace_plan(query_tile((int)std::min(rows, 1LL << 30), head_dim), head_dim).bytes;
+  return workspace_plan(query_tile((int)std::min(rows, 1LL << 30)), head_dim).bytes;
 }
 
 // 4-D map over the cache [num_blocks, H_kv, block, D], dims ordered (D, block, H_kv, blocks); a
@@ -280,10 +276,7 @@ int launch_tile(int tile, const apex::PagedParams& p, const CUtensorMap& mk, con
   switch (tile) {
     case 16: return launch_paged<T, D, 16>(p, mk, mv, dev, num_sms, s);
     case 32: return launch_paged<T, D, 32>(p, mk, mv, dev, num_sms, s);
-    case 64: return launch_paged<T, D, 64>(p, mk, mv, dev, num_sms, s);
-    default:
-      if constexpr (D <= 128) return launch_paged<T, D, 128>(p, mk, mv, dev, num_sms, s);
-      return APEX_ATTN_ERR_INVALID_ARGUMENT;
+    default: return launch_paged<T, D, 128>(p, mk, mv, dev, num_sms, s);
   }
 }
 
@@ -346,7 +339,7 @@ int forward_paged(const apex_attn_paged_args* a, void* workspace, size_t bytes, 
   if ((rc = encode_cache(&mk, a->k_cache, *a, st + 4)) || (rc = encode_cache(&mv, a->v_cache, *a, st + 7))) return rc;
 
   const int group = a->heads_q / a->heads_kv;
-  const int tile = query_tile(group * a->max_seqlen_q, a->head_dim);
+  const int tile = query_tile(group * a->max_seqlen_q);
   const Workspace w = workspace_plan(tile, a->head_dim);
   char* ws = static_cast<char*>(workspace);
   apex::PagedParams p{};
