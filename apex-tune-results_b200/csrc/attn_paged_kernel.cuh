@@ -90,8 +90,13 @@ struct PagedCfg {
   static constexpr int kTerms = std::is_same<T, __half>::value ? 3 : 2;  // of q
   static constexpr bool kQueryMajor = NQ == 128;
   static constexpr int kWG = kQueryMajor ? 4 : 1;        // softmax warpgroups
-  static constexpr int kNC = 32 < NQ ? 32 : NQ;          // S values per thread: query rows, or tokens
+  // Query-major, d <= 128: two pairs of warpgroups take the tiles in turn, each pair with its own
+  // maxima, sums and O, so that one's exponentials run while the other loads and converts.
+  static constexpr int kPairs = kQueryMajor && D <= 128 ? 2 : 1;
+  static constexpr int kLead = kPairs;                   // S runs this many tiles ahead of P V
+  static constexpr int kNC = 32 < NQ ? 32 : NQ;          // S values per thread at once: query rows, or tokens
   static constexpr int kSoftWarps = 4 * kWG;
+  static constexpr int kTileWarps = kSoftWarps / kPairs; // softmax warps per tile
   static constexpr int kThreads = 128 * (kWG + 1);
   // Two CTAs per SM cover each other's latencies where their shared memory fits.
   static constexpr int kCtas = (D <= 128 && NQ <= 32) ? 2 : 1;
@@ -99,7 +104,7 @@ struct PagedCfg {
   static constexpr int kQBytes = kTerms * NQ * D;        // one segment's query rows
   static constexpr int kPTerm = kPagedTile * NQ;         // one term of one P buffer
   static constexpr int kBudget = kCtas == 2 ? 115712 : 232448;
-  static constexpr int kMiscBytes = 2240 + NQ * 88;      // what the plan below adds
+  static constexpr int kMiscBytes = 2240 + NQ * (NQ == 128 ? 96 : 56);      // what the plan below adds
   static constexpr int slots(int q_bufs, int p_bufs) {
     return (kBudget - q_bufs * kQBytes - p_bufs * kTerms * kPTerm - kMiscBytes) / kSlotBytes;
   }
@@ -110,12 +115,12 @@ struct PagedCfg {
   static constexpr bool kSelfSplit = kQueryMajor;
   static constexpr int kQBufs = !kSelfSplit && slots(2, kPBufs) >= 4 ? 2 : 1;
   static constexpr int kNS = slots(kQBufs, kPBufs) > 12 ? 12 : slots(kQBufs, kPBufs);  // ring slots
-  static_assert(kNS >= 2, "the ring needs K(j + 1) beside V(j)");
+  static_assert(kNS > kLead, "the ring needs K(j + kLead) beside V(j)");
   static constexpr int kScaleRing = 8;
   static constexpr int kSegRing = 4;
   // TMEM: S buffers at 0 and NQ, O from 2 NQ on (token-major: a block of NQ columns per 128 of
-  // the head dim; query-major: the head dim).
-  static constexpr int kTmemUsed = kQueryMajor ? 2 * NQ + D : (2 + kChunks) * NQ;
+  // the head dim; query-major: the head dim, for each pair).
+  static constexpr int kTmemUsed = kQueryMajor ? 2 * NQ + kPairs * D : (2 + kChunks) * NQ;
   static constexpr int kTmemCols = kTmemUsed <= 64 ? 64 : (kTmemUsed <= 128 ? 128 : (kTmemUsed <= 256 ? 256 : 512));
   static_assert(kTmemUsed <= 512 && kCtas * kTmemCols <= 512, "TMEM plan");
   // shared-memory plan
@@ -128,8 +133,8 @@ struct PagedCfg {
                        kSegEmpty = kSegFull + kSegRing, kDrain = kSegEmpty + kSegRing, kNumBars = kDrain + 1;
   static constexpr int kScales = (kBars + kNumBars * 8 + 15) / 16 * 16;  // float4 [kScaleRing][8 pages]
   static constexpr int kCol = kScales + kScaleRing * 8 * 16;  // two of, per query row: -m, q scale, factor, hi, lo
-  static constexpr int kRed = kCol + 2 * 5 * NQ * 4;          // token-major [4 warps][NQ], query-major [3][4 warpgroups][128]
-  static constexpr int kSegs = (kRed + (kQueryMajor ? 12 : 4) * NQ * 4 + 15) / 16 * 16;       // int4 [kSegRing][kSegVecs]
+  static constexpr int kRed = kCol + 2 * 5 * NQ * 4;          // token-major [4 warps][NQ], query-major [14][128]
+  static constexpr int kSegs = (kRed + (kQueryMajor ? 14 : 4) * NQ * 4 + 15) / 16 * 16;       // int4 [kSegRing][kSegVecs]
   static constexpr int kScan = kSegs + kSegRing * 5 * 16;                // long long [32], found request
   static constexpr int kMisc = kScan + 32 * 8 + 16;
   static constexpr int kBytes = kMisc + 16;
@@ -582,13 +587,13 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       ptx::mbar_init(bar(C::kQEmpty + b), 1);
       ptx::mbar_init(bar(C::kColEmpty + b), C::kSoftWarps);
       ptx::mbar_init(bar(C::kSFull + b), 1);
-      ptx::mbar_init(bar(C::kSFree + b), C::kSoftWarps);
-      ptx::mbar_init(bar(C::kPFull + b), C::kSoftWarps);
+      ptx::mbar_init(bar(C::kSFree + b), C::kTileWarps);
+      ptx::mbar_init(bar(C::kPFull + b), C::kTileWarps);
       ptx::mbar_init(bar(C::kPvDone + b), 1);
     }
     for (int s = 0; s < C::kScaleRing; ++s) {
       ptx::mbar_init(bar(C::kScFull + s), 1);
-      ptx::mbar_init(bar(C::kScEmpty + s), C::kSoftWarps);
+      ptx::mbar_init(bar(C::kScEmpty + s), C::kTileWarps);
     }
     for (int s = 0; s < C::kSegRing; ++s) {
       ptx::mbar_init(bar(C::kSegFull + s), 1);
@@ -653,23 +658,23 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     uint32_t fills = 0;  // ring fills of the segments before
     auto split = [&](const PagedSegment& s, int n) {
       split_query_rows<T, D, NQ, 1>(p, s, smem, n, warp, C::kSoftWarps);
-      ptx::named_bar_sync(7, 32 * C::kSoftWarps);
+      ptx::named_bar_sync(15, 32 * C::kSoftWarps);
       if (threadIdx.x == 0) ptx::mbar_arrive(bar(C::kQFull + (n & 1)));
     };
     // One answer for all softmax warps, or those that go on would miss the others at a barrier.
     auto next_for_all = [&](PagedSegment& s) {
       const bool more = next_segment(s);
-      return !ptx::named_bar_or(7, 32 * C::kSoftWarps, !more);
+      return !ptx::named_bar_or(15, 32 * C::kSoftWarps, !more);
     };
     // Tokens of tile j that no row sees: their V rows hold anything (NaN, an older tile), and
-    // 0 * NaN would reach O. Clear them. Thread t of the first warpgroup takes token t.
+    // 0 * NaN would reach O. Clear them. Thread t of a tile's first warpgroup takes token t.
     auto clear_unseen = [&](int j) {
       const int pos0 = (seg.tile + j) * kPagedTile, pos = pos0 + t;
       if (pos0 >= seg.lo && pos0 + kPagedTile <= seg.hi) return;
-      const uint32_t fill = fills + (j + 1 < seg.n ? 2 * j + 2 : 2 * j + 1);  // V(j)'s place in the ring
+      const uint32_t fill = fills + min(seg.n, j + 1 + C::kLead) + j;  // V(j)'s place in the ring
       const int slot = (int)(fill % NS);
       wait(C::kKvFull + slot, fill / NS);
-      if (wg == 0 && (pos < seg.lo || pos >= seg.hi)) {
+      if ((wg & 1) == 0 && (pos < seg.lo || pos >= seg.hi)) {
 #pragma unroll 1
         for (int k = 0; k < D; k += 16)
           ptx::st_shared_v4(sbase + slot * C::kSlotBytes + (k / C::kRow) * (kPagedTile * C::kRow) + t * C::kRow +
@@ -678,11 +683,14 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     };
     bool more = next_for_all(seg);
     if constexpr (C::kQueryMajor) {
-      // Thread: row `t` of the tile, tokens c_first .. c_first + 31; the four warps of a TMEM quarter
-      // share their rows and agree on the maxima.
-      const int quarter = warp & 3;
-      const int tok0 = wg * NC;
-      float* const exchange = reinterpret_cast<float*>(smem + C::kRed);  // [3][4][128]
+      // Thread: row `t` of the tile, tokens tok0 .. tok0 + kTok - 1 of the tiles of its pair; the warps
+      // of a pair that share a TMEM quarter share its rows and agree on their maxima.
+      constexpr int kWGs = C::kWG / C::kPairs;     // warpgroups per pair
+      constexpr int kTok = kPagedTile / kWGs;      // tokens per thread, 32 at a time
+      const int quarter = warp & 3, pair = wg / kWGs, tok0 = wg % kWGs * kTok;
+      const int vote = 1 + pair * 4 + quarter;     // barrier of the quarter's warps in the pair
+      // Exchange: maxima [2 tiles][kWG][128], sums [kWG][128], references [pairs][128].
+      float* const exchange = reinterpret_cast<float*>(smem + C::kRed);
 #pragma unroll 1
       for (int n = 0; more; ++n) {
         if (n == 0) split(seg, 0);
@@ -697,54 +705,58 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
 #pragma unroll 1
         for (int j = 0; j < seg.n; ++j, ++g) {
           const int sb = g & 1;
+          if (C::kPairs == 2 && sb != pair) continue;
           const int pos0 = (seg.tile + j) * kPagedTile;
+          const bool masked = pos0 < seg.lo_all || pos0 + kPagedTile > seg.hi_all;
           wait(C::kScFull + g % C::kScaleRing, (uint32_t)(g / C::kScaleRing));
           const float4* const sc = scales + (g % C::kScaleRing) * 8;
-          const float4 sc0 = sc[tok0 >> p.block_shift], sc1 = sc[(tok0 + 16) >> p.block_shift];
           wait(C::kSFull + sb, (uint32_t)(g >> 1));
           ptx::tc_fence_after();
           float2 d[NC / 2];
-          ptx::tmem_ld16(tmem + lane_off + (uint32_t)(sb * NQ + tok0), reinterpret_cast<uint32_t*>(d));
-          ptx::tmem_ld16(tmem + lane_off + (uint32_t)(sb * NQ + tok0 + 16), reinterpret_cast<uint32_t*>(d) + 16);
-          ptx::tmem_wait_ld();
-          ptx::reg_fence16(reinterpret_cast<uint32_t*>(d));
-          ptx::reg_fence16(reinterpret_cast<uint32_t*>(d) + 16);
-          ptx::tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            ptx::mbar_arrive(bar(C::kScEmpty + g % C::kScaleRing));
-            ptx::mbar_arrive(bar(C::kSFree + sb));
-          }
+          auto load = [&](int c0) {  // 32 tokens' scores
+            const uint32_t at = tmem + lane_off + (uint32_t)(sb * NQ + c0);
+            ptx::tmem_ld16(at, reinterpret_cast<uint32_t*>(d));
+            ptx::tmem_ld16(at + 16, reinterpret_cast<uint32_t*>(d) + 16);
+            ptx::tmem_wait_ld();
+            ptx::reg_fence16(reinterpret_cast<uint32_t*>(d));
+            ptx::reg_fence16(reinterpret_cast<uint32_t*>(d) + 16);
+          };
           // d = x + log2 b - m; -inf where the row does not see the token.
+          auto scaled = [&](int c0) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const float4 s = sc[(c0 + 16 * half) >> p.block_shift];
+              const float a = s.x * qs, b = s.y + nm;
+              const float2 a2 = make_float2(a, a), b2 = make_float2(b, b);
+#pragma unroll
+              for (int c = 8 * half; c < 8 * half + 8; ++c) d[c] = __ffma2_rn(d[c], a2, b2);
+            }
+            if (masked) {
+#pragma unroll
+              for (int c = 0; c < NC; ++c) {
+                const int pos = pos0 + c0 + c;
+                if (pos < lo || pos >= hi) (c & 1 ? d[c / 2].y : d[c / 2].x) = -INFINITY;
+              }
+            }
+          };
           float most = -INFINITY;
+#pragma unroll 1
+          for (int c0 = 0; c0 < kTok; c0 += NC) {
+            load(tok0 + c0);
+            scaled(tok0 + c0);
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const float a = (half ? sc1.x : sc0.x) * qs, b = (half ? sc1.y : sc0.y) + nm;
-            const float2 a2 = make_float2(a, a), b2 = make_float2(b, b);
-#pragma unroll
-            for (int c = 8 * half; c < 8 * half + 8; ++c) {
-              d[c] = __ffma2_rn(d[c], a2, b2);
-              most = ptx::fmax3(most, d[c].x, d[c].y);
-            }
-          }
-          if (pos0 < seg.lo_all || pos0 + kPagedTile > seg.hi_all) {
-            most = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-              const int pos = pos0 + tok0 + c;
-              float& x = c & 1 ? d[c / 2].y : d[c / 2].x;
-              if (pos < lo || pos >= hi) x = -INFINITY;
-              most = fmaxf(most, x);
-            }
+            for (int c = 0; c < NC / 2; ++c) most = ptx::fmax3(most, d[c].x, d[c].y);
           }
           const bool left = pos0 < seg.lo_all;
-          const bool move = force || left ? true : ptx::named_bar_or(1 + quarter, 128, most > kPagedMost);
+          const bool move = force || left ? true : ptx::named_bar_or(vote, 32 * kWGs, most > kPagedMost);
           force = left;
           if (move) {
-            float* const tops = exchange + sb * 4 * NQ;
+            float* const tops = exchange + ((g / C::kPairs) & 1) * C::kWG * NQ;
             tops[wg * NQ + t] = most;
-            ptx::named_bar_sync(1 + quarter, 128);
-            const float top = fmaxf(fmaxf(tops[t], tops[NQ + t]), fmaxf(tops[2 * NQ + t], tops[3 * NQ + t]));
+            ptx::named_bar_sync(vote, 32 * kWGs);
+            float top = most;
+#pragma unroll
+            for (int k = 0; k < kWGs; ++k) top = fmaxf(top, tops[(pair * kWGs + k) * NQ + t]);
             // By how much the maximum moves: up only, but freely the first time.
             const bool some = top != -INFINITY;
             const float by = some ? (set ? fmaxf(top - kPagedTop, 0.f) : top - kPagedTop) : 0.f;
@@ -752,15 +764,17 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
             set = set || some;
             nm -= by;
             l *= f;
-            const float2 by2 = make_float2(-by, -by);
+            if (C::kPairs == 1) {  // d is still here; else it is loaded again below
+              const float2 by2 = make_float2(-by, -by);
 #pragma unroll
-            for (int c = 0; c < NC / 2; ++c) d[c] = __fadd2_rn(d[c], by2);
-            if (j > 0) {
-              wait(C::kPvDone + (sb ^ 1), (uint32_t)((g - 1) >> 1));
+              for (int c = 0; c < NC / 2; ++c) d[c] = __fadd2_rn(d[c], by2);
+            }
+            if (j >= C::kPairs) {
+              wait(C::kPvDone + ((g - C::kPairs) & 1), (uint32_t)((g - C::kPairs) >> 1));
               ptx::tc_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < D / 4; c += 16) {
-                const uint32_t at = tmem + lane_off + (uint32_t)(2 * NQ + wg * (D / 4) + c);
+              for (int c = 0; c < D / kWGs; c += 16) {
+                const uint32_t at = tmem + lane_off + (uint32_t)(2 * NQ + pair * D + wg % kWGs * (D / kWGs) + c);
                 uint32_t v[16];
                 ptx::tmem_ld16(at, v);
                 ptx::tmem_wait_ld();
@@ -775,84 +789,125 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           // The P buffer was read by an earlier tile's P V.
           if (g >= C::kPBufs) wait(C::kPvDone + ((g - C::kPBufs) & 1), (uint32_t)((g - C::kPBufs) >> 1));
           const uint32_t dst = sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kTerms * C::kPTerm + t * 128;
+#pragma unroll 1
+          for (int c0 = 0; c0 < kTok; c0 += NC) {
+            if (C::kPairs == 2) {
+              load(tok0 + c0);
+              scaled(tok0 + c0);
+            }
+            if (c0 + NC == kTok) {  // S is in registers: the MMA warp may write the buffer again
+              ptx::tc_fence_before();
+              __syncwarp();
+              if (lane == 0) ptx::mbar_arrive(bar(C::kSFree + sb));
+            }
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t term[C::kTerms][4];
-            float2 sum = make_float2(0.f, 0.f);
+            for (int half = 0; half < 2; ++half) {
+              const int c16 = tok0 + c0 + 16 * half;
+              uint32_t term[C::kTerms][4];
+              float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int x = 8 * half + 2 * k;
-              const float2 e0 = make_float2(ptx::ex2(d[x].x), ptx::ex2(d[x].y));
-              const float2 e1 = make_float2(ptx::ex2(d[x + 1].x), ptx::ex2(d[x + 1].y));
-              sum = __fadd2_rn(sum, __fadd2_rn(e0, e1));
-              __half2 a = __floats2half2_rn(e0.x, e0.y), b = __floats2half2_rn(e1.x, e1.y);
+              for (int k = 0; k < 4; ++k) {
+                const int x = 8 * half + 2 * k;
+                const float2 e0 = make_float2(ptx::ex2(d[x].x), ptx::ex2(d[x].y));
+                const float2 e1 = make_float2(ptx::ex2(d[x + 1].x), ptx::ex2(d[x + 1].y));
+                sum = __fadd2_rn(sum, __fadd2_rn(e0, e1));
+                __half2 a = __floats2half2_rn(e0.x, e0.y), b = __floats2half2_rn(e1.x, e1.y);
 #pragma unroll
-              for (int i = 0; i < C::kTerms; ++i) {
-                term[i][k] = e4m3x4_of_half2(a, b);
-                if (i + 1 < C::kTerms) {
-                  __half2 ra, rb;
-                  half2_of_e4m3x4(term[i][k], ra, rb);
-                  a = __hsub2(a, ra);
-                  b = __hsub2(b, rb);
+                for (int i = 0; i < C::kTerms; ++i) {
+                  term[i][k] = e4m3x4_of_half2(a, b);
+                  if (i + 1 < C::kTerms) {
+                    __half2 ra, rb;
+                    half2_of_e4m3x4(term[i][k], ra, rb);
+                    a = __hsub2(a, ra);
+                    b = __hsub2(b, rb);
+                  }
                 }
               }
-            }
-            l = fmaf(sum.x + sum.y, half ? sc1.z : sc0.z, l);
-            const uint32_t unit = (uint32_t)(((tok0 >> 4) + half) ^ (t & 7)) << 4;
+              l = fmaf(sum.x + sum.y, sc[c16 >> p.block_shift].z, l);
+              const uint32_t unit = (uint32_t)((c16 >> 4) ^ (t & 7)) << 4;
 #pragma unroll
-            for (int i = 0; i < C::kTerms; ++i)
-              ptx::st_shared_v4(dst + unit + i * C::kPTerm, term[i][0], term[i][1], term[i][2], term[i][3]);
+              for (int i = 0; i < C::kTerms; ++i)
+                ptx::st_shared_v4(dst + unit + i * C::kPTerm, term[i][0], term[i][1], term[i][2], term[i][3]);
+            }
           }
           clear_unseen(j);
           ptx::fence_proxy_async_smem();
           ptx::tc_fence_before();
           __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(bar(C::kPFull + sb));
+          if (lane == 0) {
+            ptx::mbar_arrive(bar(C::kScEmpty + g % C::kScaleRing));
+            ptx::mbar_arrive(bar(C::kPFull + sb));
+          }
         }
         fills += 2 * seg.n;
         // The next segment's scores are under way while this one's result is written. (Q's buffer is
-        // free: the last S of this segment is here.)
+        // free: every S of this segment is here once all warps meet.)
         PagedSegment then;
         more = next_for_all(then);
         if (more) split(then, n + 1);
 
         // ---- the segment's result: this thread's row, a quarter of its columns ----
-        float* const sums = exchange + 2 * 4 * NQ;
+        float* const sums = exchange + 2 * C::kWG * NQ;
+        float* const refs = sums + C::kWG * NQ;
         sums[wg * NQ + t] = l;
-        ptx::named_bar_sync(1 + quarter, 128);
-        const float sum = sums[t] + sums[NQ + t] + sums[2 * NQ + t] + sums[3 * NQ + t];
+        if (wg % kWGs == 0) refs[pair * NQ + t] = set ? nm : INFINITY;
+        ptx::named_bar_sync(9 + quarter, 32 * C::kWG);
+        float ref = refs[t];
+#pragma unroll
+        for (int k = 1; k < C::kPairs; ++k) ref = fminf(ref, refs[k * NQ + t]);
+        // o = (sum_k f_k O_k) / (sum_k f_k l_k) over the pairs, f_k = 2^(m_k - max m).
+        float f[C::kPairs], sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < C::kPairs; ++k) {
+          const float mine = refs[k * NQ + t];
+          f[k] = mine == INFINITY ? 0.f : ptx::ex2(ref - mine);
+          float s = 0.f;
+#pragma unroll
+          for (int x = 0; x < kWGs; ++x) s += sums[(k * kWGs + x) * NQ + t];
+          sum = fmaf(f[k], s, sum);
+        }
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int k = 0; k < C::kPairs; ++k) f[k] *= inv;
         const bool real = t < seg.rows;
         if (wg == 0 && real) {
-          const float lse2 = sum == 0.f ? -INFINITY : __log2f(sum) - nm;
+          const float lse2 = sum == 0.f ? -INFINITY : __log2f(sum) - ref;
           if (seg.slot >= 0)
             p.part_lse[(long long)seg.slot * NQ + t] = lse2;
           else if (p.lse != nullptr)
             p.lse[(long long)(seg.h * p.group + head) * p.total_q + seg.q0 + token] = lse2 * 0.69314718055994531f;
         }
-        if (seg.n > 0) wait(C::kPvDone + ((g - 1) & 1), (uint32_t)((g - 1) >> 1));
+#pragma unroll
+        for (int k = 1; k <= C::kPairs; ++k)
+          if (seg.n >= k) wait(C::kPvDone + ((g - k) & 1), (uint32_t)((g - k) >> 1));
         ptx::tc_fence_after();
         T* const o = static_cast<T*>(p.o) + (seg.q0 + token) * p.o_st + (seg.h * p.group + head) * p.o_sh;
         float* const part = p.part_o + ((long long)seg.slot * NQ + t) * D;
 #pragma unroll 1
-        for (int c = wg * (D / 4); c < (wg + 1) * (D / 4); c += 16) {
-          uint32_t v[16];
-          ptx::tmem_ld16(tmem + lane_off + (uint32_t)(2 * NQ + c), v);
-          ptx::tmem_wait_ld();
-          ptx::reg_fence16(v);
-          if (!real) continue;
-          // A row that saw nothing has no O (its tiles may not have run): 0, whatever TMEM holds.
+        for (int c = wg * (D / C::kWG); c < (wg + 1) * (D / C::kWG); c += 16) {
+          float out[16];
 #pragma unroll
-          for (int k = 0; k < 16; ++k) v[k] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(v[k]) * inv);
+          for (int k = 0; k < C::kPairs; ++k) {
+            uint32_t v[16];
+            ptx::tmem_ld16(tmem + lane_off + (uint32_t)(2 * NQ + k * D + c), v);
+            ptx::tmem_wait_ld();
+            ptx::reg_fence16(v);
+            // f = 0: the pair has nothing of this row, and TMEM may hold anything.
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              const float y = f[k] == 0.f ? 0.f : __uint_as_float(v[x]) * f[k];
+              out[x] = k == 0 ? y : out[x] + y;
+            }
+          }
+          if (!real) continue;
           if (seg.slot >= 0) {
 #pragma unroll
             for (int k = 0; k < 16; k += 4)
-              *reinterpret_cast<uint4*>(part + c + k) = make_uint4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+              *reinterpret_cast<float4*>(part + c + k) = make_float4(out[k], out[k + 1], out[k + 2], out[k + 3]);
           } else {
             uint32_t pk[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              pk[k] = DType<T>::pack(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1]));
+            for (int k = 0; k < 8; ++k) pk[k] = DType<T>::pack(out[2 * k], out[2 * k + 1]);
             *reinterpret_cast<uint4*>(o + c) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
             *reinterpret_cast<uint4*>(o + c + 8) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
           }
@@ -1062,7 +1117,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     }
   } else if (warp == kWarpProd) {
     // ========================================================== producer ===
-    // Ring order per segment: K(0); then K(j + 1), V(j) for each j: the MMA warp's order.
+    // Ring order per segment: K(0 .. kLead - 1); then K(j + kLead), V(j) for each j: the MMA warp's.
     // Lane i loads page i of the tile; pages that no row sees are left out.
     const uint64_t policy = p.one_tile ? ptx::policy_evict_first() : ptx::policy_evict_last();
     const int pages = kPagedTile >> p.block_shift;
@@ -1115,22 +1170,30 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
         const int id = __shfl_sync(0xffffffffu, ids, ((j & 3) << 3) + (lane & 7));
         return lane < 8 ? id : -2;
       };
+      // Tiles' ids in fill order: K runs kLead tiles ahead of V.
       if (seg.n == 0) look();
-      int id = seg.n > 0 ? pick(0) : -2;
-      if (seg.n > 0) fill(&tmK, id);
+      int behind[C::kLead];
+#pragma unroll
+      for (int k = 0; k < C::kLead; ++k) {
+        behind[k] = k < seg.n ? pick(k) : -2;
+        if (k < seg.n) fill(&tmK, behind[k]);
+      }
 #pragma unroll 1
       for (int j = 0; j < seg.n; ++j) {
+        const int ahead_tile = j + C::kLead;
         int next = -2;
-        if (j + 1 < seg.n) {
-          if (((j + 1) & 3) == 0) {
+        if (ahead_tile < seg.n) {
+          if ((ahead_tile & 3) == 0) {
             ids = ahead;
-            ahead = page_ids(seg, seg.tile + j + 5);
+            ahead = page_ids(seg, seg.tile + ahead_tile + 4);
           }
-          next = pick(j + 1);
+          next = pick(ahead_tile);
           fill(&tmK, next);
         }
-        fill(&tmV, id);
-        id = next;
+        fill(&tmV, behind[0]);
+#pragma unroll
+        for (int k = 0; k + 1 < C::kLead; ++k) behind[k] = behind[k + 1];
+        behind[C::kLead - 1] = next;
         if (j == 0) look();
       }
       seg = then;
@@ -1203,7 +1266,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       ptx::tc_fence_after();
       if (ok) {
         const uint32_t weights = sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kTerms * C::kPTerm;
-        const uint32_t dO = tmem + (uint32_t)(2 * NQ);
+        const uint32_t dO = tmem + (uint32_t)(2 * NQ + (C::kPairs == 2 ? sb * D : 0));
         if constexpr (C::kQueryMajor) {
 #pragma unroll
           for (int ks = 0; ks < kPagedTile / 32; ++ks) {
@@ -1242,11 +1305,12 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
         if (lane == 0) ptx::mbar_arrive(bar(C::kQEmpty + n % C::kQBufs));
         continue;
       }
-      issue_S(seg.n == 1);
+#pragma unroll 1
+      for (int j = 0; j < min(seg.n, C::kLead); ++j) issue_S(j + 1 == seg.n);
 #pragma unroll 1
       for (int j = 0; j < seg.n; ++j) {
-        if (j + 1 < seg.n) issue_S(j + 2 == seg.n);
-        issue_PV(j == 0);
+        if (j + C::kLead < seg.n) issue_S(j + C::kLead + 1 == seg.n);
+        issue_PV(j < C::kPairs);
       }
     }
     ptx::tc_commit_warp(bar(C::kDrain));
