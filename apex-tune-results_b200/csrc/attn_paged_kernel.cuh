@@ -224,36 +224,31 @@ struct PagedSegment {
 constexpr int kSegVecs = sizeof(PagedSegment) / 16;
 static_assert(sizeof(PagedSegment) == 64, "published as four 16-byte words");
 
-// Where every role walks from: the CTA's range of units and the request that it begins in.
+// Where the walk begins: the CTA's range of units and the request that it begins in. The host
+// refuses calls whose units might not fit 31 bits; offsets that overlap could name more, and then
+// nothing is done.
 struct PagedStart {
-  long long unit, end;     // the CTA's range
-  long long request_unit;  // first unit of request b
-  long long share;         // units per CTA, one more for each of the first `more`
+  int unit, end;     // the CTA's range
+  int request_unit;  // first unit of request b
+  int share;         // units per CTA, one more for each of the first `more`
   int b, more;
-  __device__ __forceinline__ void cut(long long total);
+
+  __device__ __forceinline__ void cut(long long units) {
+    const int total = units > 0x7fffffff ? 0 : (int)units;
+    share = (int)((unsigned)total / gridDim.x);
+    more = total - share * (int)gridDim.x;
+    const int c = (int)blockIdx.x;
+    unit = c * share + min(c, more);
+    end = unit + share + (c < more ? 1 : 0);
+  }
 };
-
-// Quotient of nonnegative numbers; the 64-bit division is several times as long.
-__device__ __forceinline__ long long paged_div(long long a, long long b) {
-  if (((a | b) >> 32) == 0) return (long long)((unsigned)a / (unsigned)b);
-  return a / b;
-}
-
-__device__ __forceinline__ void PagedStart::cut(long long total) {
-  share = paged_div(total, gridDim.x);
-  more = (int)(total - share * gridDim.x);
-  const int c = (int)blockIdx.x;
-  unit = c * share + min(c, more);
-  end = unit + share + (c < more ? 1 : 0);
-}
 
 template <int NQ>
 struct PagedWalk {
   const PagedParams& p;
-  long long unit, end, share;
-  int more;
+  int unit, end, share, more;
   int b, h, qt, qts;
-  long long item;  // first unit of the item (b, h, qt)
+  int item;  // first unit of the item (b, h, qt)
   PagedRequest r;
 
   __device__ __forceinline__ PagedWalk(const PagedParams& params, const PagedStart& s)
@@ -264,10 +259,10 @@ struct PagedWalk {
     qts = paged_qtiles<NQ>(p, r);
     const int per_head = paged_head_units<NQ>(p, r);
     if (p.heads_kv > 1) {
-      h = (int)paged_div(unit - item, per_head);
-      item += (long long)h * per_head;
+      h = (int)((unsigned)(unit - item) / (unsigned)per_head);
+      item += h * per_head;
     }
-    while (true) {
+    while (qt + 1 < qts) {
       const int n = kPagedItemUnits<NQ> + max(1, paged_span<NQ>(p, r, qt).n);
       if (item + n > unit) break;
       item += n;
@@ -276,9 +271,9 @@ struct PagedWalk {
   }
 
   // The CTA whose range holds a unit.
-  __device__ __forceinline__ int cta_of(long long u) const {
-    const long long large = more * (share + 1);
-    return u < large ? (int)paged_div(u, share + 1) : more + (int)paged_div(u - large, share);
+  __device__ __forceinline__ int cta_of(int u) const {
+    const int large = more * (share + 1);
+    return u < large ? (int)((unsigned)u / (unsigned)(share + 1)) : more + (int)((unsigned)(u - large) / (unsigned)share);
   }
 
   // The next segment, or one of -1 tiles behind the last.
@@ -290,15 +285,15 @@ struct PagedWalk {
         qt = 0;
         if (++h == p.heads_kv || qts == 0) {
           h = 0;
-          ++b;
+          if (++b >= p.batch) return s;  // (units and requests always end together)
           r = paged_request(p, b);
           qts = paged_qtiles<NQ>(p, r);
         }
       }
       const PagedSpan span = paged_span<NQ>(p, r, qt);
       const int n = max(1, span.n);
-      const long long first = item + kPagedItemUnits<NQ>, last = first + n;  // the tiles' units
-      const long long from = max(unit, first), to = min(end, last);
+      const int first = item + kPagedItemUnits<NQ>, last = first + n;  // the tiles' units
+      const int from = max(unit, first), to = min(end, last);
       const int row0 = qt * NQ;
       unit = min(end, last);
       item = last;
@@ -311,8 +306,8 @@ struct PagedWalk {
       s.len = r.len;
       s.lo = span.lo;
       s.hi = span.hi;
-      s.tile = span.t0 + (int)(from - first);
-      s.n = span.n == 0 ? 0 : (int)(to - from);
+      s.tile = span.t0 + (from - first);
+      s.n = span.n == 0 ? 0 : to - from;
       s.rows = min(NQ, r.nq * p.group - row0);
       s.token0 = span.i0;
       s.head0 = row0 - span.i0 * p.group;
@@ -343,11 +338,15 @@ __device__ __forceinline__ PagedStart paged_start_warp(const PagedParams& p) {
   constexpr int kRounds = kPagedWarpBatch / 32;
   const int lane = (int)(threadIdx.x & 31);
   PagedStart s;
-  long long upto[kRounds], mine[kRounds], total = 0;
+  int upto[kRounds], mine[kRounds], total = 0;
+  long long whole = 0;  // the total, which `total` may not hold
 #pragma unroll
   for (int i = 0; i < kRounds; ++i) {
-    const int b = 32 * i + lane;
-    mine[i] = b < p.batch ? (long long)paged_head_units<NQ>(p, paged_request(p, b)) * p.heads_kv : 0;
+    mine[i] = 0;
+    if (32 * i < p.batch) {
+      const int b = 32 * i + lane;
+      if (b < p.batch) mine[i] = paged_head_units<NQ>(p, paged_request(p, b)) * p.heads_kv;
+    }
   }
 #pragma unroll
   for (int i = 0; i < kRounds; ++i) {
@@ -355,14 +354,16 @@ __device__ __forceinline__ PagedStart paged_start_warp(const PagedParams& p) {
     if (32 * i < p.batch) {
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, upto[i], d);
+        const int up = __shfl_up_sync(0xffffffffu, upto[i], d);
         if (lane >= d) upto[i] += up;
       }
       upto[i] += total;
       total = __shfl_sync(0xffffffffu, upto[i], 31);
+      whole += __reduce_add_sync(0xffffffffu, (unsigned)mine[i] & 0xffffu);
+      whole += (long long)__reduce_add_sync(0xffffffffu, (unsigned)mine[i] >> 16) << 16;
     }
   }
-  s.cut(total);
+  s.cut(whole);
   s.b = 0;
   s.request_unit = 0;
 #pragma unroll
@@ -386,7 +387,7 @@ __device__ __forceinline__ PagedStart paged_start_cta(const PagedParams& p, long
   const int per = (p.batch + blockDim.x - 1) / blockDim.x;
   const int b0 = min(p.batch, (int)threadIdx.x * per), b1 = min(p.batch, b0 + per);
   long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += (long long)paged_head_units<NQ>(p, paged_request(p, b)) * p.heads_kv;
+  for (int b = b0; b < b1; ++b) mine += paged_head_units<NQ>(p, paged_request(p, b)) * p.heads_kv;
   long long total;
   const long long upto = block_scan<long long>(mine, scan, total);
   s.cut(total);
@@ -394,8 +395,8 @@ __device__ __forceinline__ PagedStart paged_start_cta(const PagedParams& p, long
   __syncthreads();  // scan is written again
   if (s.unit < s.end && at <= s.unit && s.unit < upto) {
     int b = b0;
-    while (true) {
-      const long long units = (long long)paged_head_units<NQ>(p, paged_request(p, b)) * p.heads_kv;
+    while (b + 1 < b1) {
+      const int units = paged_head_units<NQ>(p, paged_request(p, b)) * p.heads_kv;
       if (at + units > s.unit) break;
       at += units;
       ++b;
@@ -405,7 +406,7 @@ __device__ __forceinline__ PagedStart paged_start_cta(const PagedParams& p, long
   }
   __syncthreads();
   s.b = *found;
-  s.request_unit = scan[0];
+  s.request_unit = (int)scan[0];
   return s;
 }
 
@@ -657,7 +658,9 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     int g = 0;  // tiles so far
     uint32_t fills = 0;  // ring fills of the segments before
     auto split = [&](const PagedSegment& s, int n) {
-      split_query_rows<T, D, NQ, 1>(p, s, smem, n, warp, C::kSoftWarps);
+      // All of a warp's loads at once: 32 / (D / 16) rows per step.
+      constexpr int kSteps = NQ * (D / 16) / (32 * C::kSoftWarps);
+      split_query_rows<T, D, NQ, (kSteps > 1 ? kSteps : 1)>(p, s, smem, n, warp, C::kSoftWarps);
       ptx::named_bar_sync(15, 32 * C::kSoftWarps);
       if (threadIdx.x == 0) ptx::mbar_arrive(bar(C::kQFull + (n & 1)));
     };
@@ -702,6 +705,8 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
         const int lo = p.window >= 0 ? max(place - p.window, 0) : 0;
         float nm = 0.f, l = 0.f;  // kPagedTop - max; the row's sum over this thread's tokens
         bool set = false, force = true;
+        // Rows past the tile's last: nobody reads their S, weights or O.
+        const bool idle = quarter * 32 >= seg.rows;
 #pragma unroll 1
         for (int j = 0; j < seg.n; ++j, ++g) {
           const int sb = g & 1;
@@ -739,6 +744,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
               }
             }
           };
+          if (!idle) {
           float most = -INFINITY;
 #pragma unroll 1
           for (int c0 = 0; c0 < kTok; c0 += NC) {
@@ -795,11 +801,6 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
               load(tok0 + c0);
               scaled(tok0 + c0);
             }
-            if (c0 + NC == kTok) {  // S is in registers: the MMA warp may write the buffer again
-              ptx::tc_fence_before();
-              __syncwarp();
-              if (lane == 0) ptx::mbar_arrive(bar(C::kSFree + sb));
-            }
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               const int c16 = tok0 + c0 + 16 * half;
@@ -830,6 +831,11 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
                 ptx::st_shared_v4(dst + unit + i * C::kPTerm, term[i][0], term[i][1], term[i][2], term[i][3]);
             }
           }
+          }
+          // S is read: the MMA warp may write the buffer again.
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(bar(C::kSFree + sb));
           clear_unseen(j);
           ptx::fence_proxy_async_smem();
           ptx::tc_fence_before();

@@ -340,6 +340,11 @@ int forward_paged(const apex_attn_paged_args* a, void* workspace, size_t bytes, 
 
   const int group = a->heads_q / a->heads_kv;
   const int tile = query_tile(group * a->max_seqlen_q);
+  // The kernel counts its work in 31 bits: K/V heads x query tiles x (tiles of the cache and the
+  // fixed cost of an item).
+  const long long items = (long long)a->heads_kv * ((long long)a->total_q * group / tile + a->batch);
+  const long long units = (long long)a->table_width * a->block_size / apex::kPagedTile + 1 + apex::kPagedItemUnits<128>;
+  if (items * units > INT_MAX) return APEX_ATTN_ERR_TOO_LARGE;
   const Workspace w = workspace_plan(tile, a->head_dim);
   char* ws = static_cast<char*>(workspace);
   apex::PagedParams p{};
