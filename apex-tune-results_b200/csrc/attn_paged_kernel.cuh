@@ -564,6 +564,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = ptx::smem_u32(smem);
   if ((sbase & 1023u) != 0) {  // swizzled tiles need 1 KB alignment
+    ptx::wait_for_previous_grid();
     if (threadIdx.x == 0) report_error(p.status, p.host_flag, kStatusSmemAlign);
     if (threadIdx.x < 2) p.share[(2 * blockIdx.x + threadIdx.x) * kShareInts] = -1;
     return;
@@ -612,6 +613,8 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     ptx::prefetch_tmap(&tmK);
     ptx::prefetch_tmap(&tmV);
   }
+  // Launched while the kernel before may still run: up to here nothing of it was touched.
+  ptx::wait_for_previous_grid();
   PagedStart start{};
   if (p.batch > kPagedWarpBatch)
     start = paged_start_cta<NQ>(p, reinterpret_cast<long long*>(smem + C::kScan),
@@ -1416,40 +1419,90 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
 }
 
 // Joins the parts of the items that several CTAs shared: o = sum_k w_k o_k / sum_k w_k with
-// w_k = 2^(lse_k - max lse), in the CTAs' order. The CTAs c0 .. c1 of an item take its rows in
-// turn, a warp per row where few parts meet and all warps a share of the parts where many do.
+// w_k = 2^(lse_k - max lse), in the CTAs' order. The CTAs c0 .. c1 of an item share its rows out.
+// Bound: latency (three dependent loads). Few parts: a thread takes four columns of a row, so
+// that all its loads are under way at once. Many: a CTA takes a row, each warp a share of the
+// parts.
 constexpr int kCombineThreads = 256;
+constexpr int kCombineFew = 4;
 
 template <typename T, int D, int NQ>
 __global__ void __launch_bounds__(kCombineThreads) attn_paged_combine_kernel(const PagedParams p) {
   constexpr int kWarps = kCombineThreads / 32, E = D / 32;
   __shared__ float part[kWarps][D];
   __shared__ float stat[kWarps][2];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  ptx::launch_dependents();
   ptx::wait_for_previous_grid();
+  const int4* const share = reinterpret_cast<const int4*>(p.share + 2 * blockIdx.x * kShareInts);
+  const int4 entry[4] = {share[0], share[1], share[2], share[3]};
 #pragma unroll 1
   for (int side = 0; side < 2; ++side) {
-    const int4* at = reinterpret_cast<const int4*>(p.share + (2 * blockIdx.x + side) * kShareInts);
-    const int4 item = at[0], ctas = at[1];
+    const int4 item = side ? entry[2] : entry[0], ctas = side ? entry[3] : entry[1];
     if (item.x < 0) continue;
     const int h = item.y, rows = item.z, c0 = ctas.x, k_parts = ctas.y - ctas.x + 1;
-    const bool alone = k_parts <= 4;  // a warp joins a row by itself
-    const int lanes = alone ? kWarps : 1;
-    for (int c = ((int)blockIdx.x - c0) * lanes + (alone ? warp : 0); c < rows; c += k_parts * lanes) {
-      // Part k is CTA c0 + k's: the first left it behind, the others got it from before.
-      auto slot = [&](int k) { return (long long)(2 * (c0 + k) + (k == 0 ? 1 : 0)) * NQ + c; };
-      const int first = alone ? 0 : warp, step = alone ? 1 : kWarps;
+    // Part k is CTA c0 + k's: the first left it behind, the others got it from before.
+    auto slot = [&](int k, int c) { return (long long)(2 * (c0 + k) + (k == 0 ? 1 : 0)) * NQ + c; };
+    auto out = [&](int c, int d, long long& lse_at) {
+      int i, hq;
+      paged_row(p, item.w, ctas.z, c, i, hq);
+      i += item.x;
+      hq += h * p.group;
+      lse_at = (long long)hq * p.total_q + i;
+      return static_cast<T*>(p.o) + i * p.o_st + hq * p.o_sh + d;
+    };
+    auto put_lse = [&](long long at, float m, float sum) {
+      if (p.lse != nullptr) p.lse[at] = sum == 0.f ? -INFINITY : (m + __log2f(sum)) * 0.69314718055994531f;
+    };
+    if (k_parts <= kCombineFew) {
+      constexpr int kQuads = D / 4;  // threads per row
+      for (int x = ((int)blockIdx.x - c0) * kCombineThreads + (int)threadIdx.x; x < rows * kQuads;
+           x += k_parts * kCombineThreads) {
+        const int c = x / kQuads, d = x % kQuads * 4;
+        float lse[kCombineFew], m = -INFINITY, sum = 0.f;
+        float4 o[kCombineFew];
+#pragma unroll
+        for (int k = 0; k < kCombineFew; ++k) {
+          lse[k] = -INFINITY;
+          if (k < k_parts) {
+            lse[k] = p.part_lse[slot(k, c)];
+            o[k] = *reinterpret_cast<const float4*>(p.part_o + slot(k, c) * D + d);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kCombineFew; ++k) m = fmaxf(m, lse[k]);
+        const float base = m == -INFINITY ? 0.f : m;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < kCombineFew; ++k) {
+          if (k < k_parts) {
+            const float w = ptx::ex2(lse[k] - base);
+            sum += w;
+            acc = make_float4(fmaf(w, o[k].x, acc.x), fmaf(w, o[k].y, acc.y), fmaf(w, o[k].z, acc.z),
+                              fmaf(w, o[k].w, acc.w));
+          }
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        long long lse_at;
+        T* to = out(c, d, lse_at);
+        *reinterpret_cast<uint2*>(to) = make_uint2(DType<T>::pack(acc.x * inv, acc.y * inv),
+                                                   DType<T>::pack(acc.z * inv, acc.w * inv));
+        if (d == 0) put_lse(lse_at, m, sum);
+      }
+      continue;
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int c = (int)blockIdx.x - c0; c < rows; c += k_parts) {
       float m = -INFINITY, sum = 0.f, acc[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] = 0.f;
-      for (int k = first + lane * step; k < k_parts; k += 32 * step) m = fmaxf(m, p.part_lse[slot(k)]);
+      for (int k = warp + lane * kWarps; k < k_parts; k += 32 * kWarps) m = fmaxf(m, p.part_lse[slot(k, c)]);
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
       const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll 4
-      for (int k = first; k < k_parts; k += step) {
-        const float w = ptx::ex2(p.part_lse[slot(k)] - base);
-        const float* o = p.part_o + slot(k) * D + lane * E;
+      for (int k = warp; k < k_parts; k += kWarps) {
+        const float w = ptx::ex2(p.part_lse[slot(k, c)] - base);
+        const float* o = p.part_o + slot(k, c) * D + lane * E;
         sum += w;
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
@@ -1458,46 +1511,33 @@ __global__ void __launch_bounds__(kCombineThreads) attn_paged_combine_kernel(con
           acc[e + 1] = fmaf(w, v.y, acc[e + 1]);
         }
       }
-      if (!alone) {
-        if (lane == 0) {
-          stat[warp][0] = m;
-          stat[warp][1] = sum;
-        }
+      if (lane == 0) {
+        stat[warp][0] = m;
+        stat[warp][1] = sum;
+      }
 #pragma unroll
-        for (int e = 0; e < E; ++e) part[warp][lane * E + e] = acc[e];
-        __syncthreads();
+      for (int e = 0; e < E; ++e) part[warp][lane * E + e] = acc[e];
+      __syncthreads();
+      if (threadIdx.x < D / 2) {
         float all = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) all = fmaxf(all, stat[w][0]);
         const float base_all = all == -INFINITY ? 0.f : all;
-        if (warp == 0) {
-          sum = 0.f;
+        const int d = 2 * threadIdx.x;
+        float total = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) {
-            // A warp without parts has max -inf: weight 0.
-            const float f = ptx::ex2(stat[w][0] - base_all);
-            sum += f * stat[w][1];
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = fmaf(f, part[w][lane * E + e], acc[e]);
-          }
-          m = all;
+        for (int w = 0; w < kWarps; ++w) {
+          const float f = ptx::ex2(stat[w][0] - base_all);  // a warp without parts has -inf: 0
+          total = fmaf(f, stat[w][1], total);
+          x = fmaf(f, part[w][d], x);
+          y = fmaf(f, part[w][d + 1], y);
         }
-        __syncthreads();
-        if (warp != 0) continue;
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        long long lse_at;
+        *reinterpret_cast<uint32_t*>(out(c, d, lse_at)) = DType<T>::pack(x * inv, y * inv);
+        if (d == 0) put_lse(lse_at, all, total);
       }
-      int i, hq;
-      paged_row(p, item.w, ctas.z, c, i, hq);
-      i += item.x;
-      hq += h * p.group;
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      T* o = static_cast<T*>(p.o) + (long long)i * p.o_st + (long long)hq * p.o_sh + lane * E;
-#pragma unroll
-      for (int e = 0; e < E; e += 2)
-        *reinterpret_cast<uint32_t*>(o + e) = DType<T>::pack(acc[e] * inv, acc[e + 1] * inv);
-      if (p.lse != nullptr && lane == 0)
-        p.lse[(long long)hq * p.total_q + i] = sum == 0.f ? -INFINITY : (m + __log2f(sum)) * 0.69314718055994531f;
+      __syncthreads();
     }
   }
 }
