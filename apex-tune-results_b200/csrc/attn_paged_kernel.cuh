@@ -135,7 +135,8 @@ struct PagedCfg {
   static constexpr int kCol = kScales + kScaleRing * 8 * 16;  // two of, per query row: -m, q scale, factor, hi, lo
   static constexpr int kRed = kCol + 2 * 5 * NQ * 4;          // token-major [4 warps][NQ], query-major [14][128]
   static constexpr int kSegs = (kRed + (kQueryMajor ? 14 : 4) * NQ * 4 + 15) / 16 * 16;       // int4 [kSegRing][kSegVecs]
-  static constexpr int kScan = kSegs + kSegRing * 5 * 16;                // long long [32], found request
+  static constexpr int kBad = kSegs + kSegRing * 4 * 16;                 // unsigned [2][4]
+  static constexpr int kScan = kBad + 32;                // long long [32], found request
   static constexpr int kMisc = kScan + 32 * 8 + 16;
   static constexpr int kBytes = kMisc + 16;
   static_assert(kBytes <= kBudget, "shared-memory plan");
@@ -603,6 +604,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     }
     ptx::mbar_init(bar(C::kDrain), 1);
     *abort_flag = 0;
+    for (int k = 0; k < 8; ++k) reinterpret_cast<unsigned*>(smem + C::kBad)[k] = 0;
     ptx::fence_mbar_init();
   }
   if (warp == kWarpMma) {
@@ -672,19 +674,50 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       const bool more = next_segment(s);
       return !ptx::named_bar_or(15, 32 * C::kSoftWarps, !more);
     };
-    // Tokens of tile j that no row sees: their V rows hold anything (NaN, an older tile), and
-    // 0 * NaN would reach O. Clear them. Thread t of a tile's first warpgroup takes token t.
-    auto clear_unseen = [&](int j) {
+    // Before P V of tile j, the V rows that would carry NaN to rows that do not see their token
+    // (0 * NaN): those of tokens that no row sees hold anything (NaN, an older tile) and are
+    // cleared. Where some rows see a token and others do not, a V row with NaN in it is cleared
+    // too, and the rows that see it get a weight of NaN instead: `poison(token)` writes this
+    // thread's. Thread t of a tile's first warpgroup takes token t.
+    unsigned* const bad_tokens = reinterpret_cast<unsigned*>(smem + C::kBad);  // [2 tiles][128 bits]
+    auto clear_unseen = [&](int j, int tile_barrier, auto&& poison) {
       const int pos0 = (seg.tile + j) * kPagedTile, pos = pos0 + t;
-      if (pos0 >= seg.lo && pos0 + kPagedTile <= seg.hi) return;
+      const bool uneven = (pos0 < seg.lo_all && seg.lo < seg.lo_all) ||
+                          (pos0 + kPagedTile > seg.hi_all && seg.hi_all < seg.hi);
+      if (!uneven && pos0 >= seg.lo && pos0 + kPagedTile <= seg.hi) return;
       const uint32_t fill = fills + min(seg.n, j + 1 + C::kLead) + j;  // V(j)'s place in the ring
       const int slot = (int)(fill % NS);
       wait(C::kKvFull + slot, fill / NS);
-      if ((wg & 1) == 0 && (pos < seg.lo || pos >= seg.hi)) {
+      unsigned* const bad = bad_tokens + (g & 1) * 4;
+      const uint32_t row = sbase + slot * C::kSlotBytes + t * C::kRow;
+      auto at = [&](int k) { return row + (k / C::kRow) * (kPagedTile * C::kRow) + k % C::kRow; };
+      if ((wg & 1) == 0) {
+        const bool unseen = pos < seg.lo || pos >= seg.hi;
+        bool nan = false;
+        if (uneven && !unseen) {
 #pragma unroll 1
-        for (int k = 0; k < D; k += 16)
-          ptx::st_shared_v4(sbase + slot * C::kSlotBytes + (k / C::kRow) * (kPagedTile * C::kRow) + t * C::kRow +
-                                k % C::kRow, 0, 0, 0, 0);
+          for (int k = 0; k < D; k += 16) {
+            const uint4 v = ptx::ld_shared_v4(at(k));
+            // A byte of 7f or ff: its low seven bits carry when 1 is added.
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) nan |= (((w[x] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+          }
+          if (nan) atomicOr(bad + (t >> 5), 1u << (t & 31));
+        }
+        if (unseen || nan) {
+#pragma unroll 1
+          for (int k = 0; k < D; k += 16) ptx::st_shared_v4(at(k), 0, 0, 0, 0);
+        }
+      }
+      if (!uneven) return;
+      ptx::named_bar_sync(tile_barrier, 32 * C::kTileWarps);
+      if ((bad[0] | bad[1] | bad[2] | bad[3]) != 0) {
+#pragma unroll 1
+        for (int x = 0; x < kPagedTile; ++x)
+          if (bad[x >> 5] >> (x & 31) & 1) poison(x);
+        ptx::named_bar_sync(tile_barrier, 32 * C::kTileWarps);
+        if ((wg & 1) == 0 && t < 4) bad[t] = 0;  // before this pair's next barrier
       }
     };
     bool more = next_for_all(seg);
@@ -747,6 +780,11 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
               }
             }
           };
+          // The P buffer was read by an earlier tile's P V.
+          auto wait_p_buffer = [&]() {
+            if (g >= C::kPBufs) wait(C::kPvDone + ((g - C::kPBufs) & 1), (uint32_t)((g - C::kPBufs) >> 1));
+          };
+          if (idle) wait_p_buffer();  // (clear_unseen counts on it)
           if (!idle) {
           float most = -INFINITY;
 #pragma unroll 1
@@ -795,8 +833,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
               ptx::tmem_wait_st();
             }
           }
-          // The P buffer was read by an earlier tile's P V.
-          if (g >= C::kPBufs) wait(C::kPvDone + ((g - C::kPBufs) & 1), (uint32_t)((g - C::kPBufs) >> 1));
+          wait_p_buffer();
           const uint32_t dst = sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kTerms * C::kPTerm + t * 128;
 #pragma unroll 1
           for (int c0 = 0; c0 < kTok; c0 += NC) {
@@ -839,7 +876,12 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           ptx::tc_fence_before();
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive(bar(C::kSFree + sb));
-          clear_unseen(j);
+          clear_unseen(j, 13 + pair, [&](int x) {
+            const int pos = pos0 + x;
+            if (x >= tok0 && x < tok0 + kTok && pos >= lo && pos < hi)
+              ptx::st_shared_u8(sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kTerms * C::kPTerm + t * 128 +
+                                    (((x >> 4) ^ (t & 7)) << 4) + (x & 15), 0x7fu);
+          });
           ptx::fence_proxy_async_smem();
           ptx::tc_fence_before();
           __syncwarp();
@@ -1055,7 +1097,11 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           for (int j2 = 0; j2 < C::kTerms; ++j2)
             ptx::st_shared_v4(dst + c * 128 + j2 * C::kPTerm, term[j2][0], term[j2][1], term[j2][2], term[j2][3]);
         }
-        clear_unseen(j);
+        clear_unseen(j, 1 + wg, [&](int x) {  // columns 16-byte chunk by chunk, tokens within
+          if (x != t) return;
+          for (int c = 0; c < NC; ++c)
+            if (pos >= col_lo[c] && pos < col_hi[c]) ptx::st_shared_u8(dst + (c >> 4) * 2048 + (c & 15), 0x7fu);
+        });
         ptx::fence_proxy_async_smem();
         ptx::tc_fence_before();
         __syncwarp();

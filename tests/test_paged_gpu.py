@@ -458,6 +458,207 @@ def test_views_of_q():
     assert torch.equal(call(p), want)
 
 
+@pytest.mark.parametrize("hq,hkv,dim,q_len,window", [(4, 2, 128, 5, None), (8, 2, 64, 7, 3), (16, 2, 128, 30, None),
+                                                    (16, 2, 64, 200, 40), (16, 2, 256, 30, None), (4, 2, 256, 4, None),
+                                                    (40, 2, 128, 150, None)])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_nan_reaches_only_the_rows_that_see_it(hq, hkv, dim, q_len, window, which):
+    """A cached token that holds NaN: rows before it (and, under a window, behind) keep their values, the
+    others get NaN. Both layouts of the products, tokens at tile edges among them."""
+    lens = [q_len + 253, q_len + 1]
+    p = paged_problem(lens, hq, hkv, dim, 16, "bf16", [q_len, q_len], seed=dim + q_len)
+    want_o, want_lse, ob, lb = ref.attend(p["q"], *(c.double().nan_to_num() for c, _ in p["caches"]),
+                                          *(s.double().nan_to_num() for _, s in p["caches"]), p["table"], lens, p["cu"],
+                                          16, True, window)
+    bad = [lens[0] - q_len // 2 - 1, lens[1] - 1]  # token positions
+    column = 5
+    for b, pos in enumerate(bad):
+        codes = p["gpu"][0 if which == "k" else 1][0]
+        codes[p["table"][b][pos // 16], :, pos % 16, column] = float("nan")
+    o, lse = call(p, window_left=window, return_lse=True)
+    o, lse = o.double().cpu(), lse.double().cpu()
+    for b, pos in enumerate(bad):
+        for i in range(q_len):
+            r, place = p["cu"][b] + i, lens[b] - q_len + i
+            sees = pos <= place and (window is None or pos >= place - window)
+            if sees:
+                assert torch.isnan(o[r, :, column]).all()
+                assert which == "v" or torch.isnan(lse[:, r]).all()
+            else:
+                eps = torch.finfo(torch.bfloat16).eps / 2
+                assert ((o[r] - want_o[r]).abs() <= ob[r] + eps * (want_o[r].abs() + ob[r])).all()
+                assert ((lse[:, r] - want_lse[:, r]).abs() <= lb[:, r]).all()
+
+
+@pytest.mark.parametrize("batch", [129, 300, 1000])
+def test_large_batches(batch):
+    rng = random.Random(batch)
+    lens = [rng.choice([0, 1, rng.randint(1, 300)]) for _ in range(batch)]
+    check_attend(paged_problem(lens, 4, 1, 64, 16, "bf16", [1] * batch, seed=batch), decode=True)
+
+
+def test_ragged_queries_in_a_large_batch():
+    rng = random.Random(7)
+    lens = [rng.randint(1, 200) for _ in range(150)]
+    q_lens = [rng.choice([0, 1, 1, 2, 40]) for _ in lens]
+    check_attend(paged_problem(lens, 8, 2, 64, 32, "fp16", q_lens, seed=7, spare_rows=3))
+
+
+def test_heads_of_their_own_and_one_head_for_all():
+    check_attend(paged_problem([200, 64], 32, 32, 64, 16, "bf16", [1, 1], seed=1), decode=True)
+    check_attend(paged_problem([300, 129], 16, 16, 128, 32, "fp16", [9, 3], seed=2))
+    check_attend(paged_problem([513], 200, 1, 64, 16, "bf16", [3], seed=3))
+
+
+def test_scales_of_zero_and_of_far_apart_blocks():
+    p = paged_problem([300, 70], 8, 2, 128, 16, "bf16", [1, 1], seed=4)
+    for c, s in p["caches"]:
+        s.copy_(s * torch.exp2(torch.randint(-12, 13, s.shape, generator=torch.Generator().manual_seed(1)).float()))
+    k_scale, v_scale = p["caches"][0][1], p["caches"][1][1]
+    k_scale.clamp_(max=0.05)
+    k_scale[p["table"][0][2]] = 0.0
+    v_scale[p["table"][0][3]] = 0.0
+    v_scale[p["table"][1][0]] = 0.0
+    p["gpu"] = [(c.cuda(), s.cuda()) for c, s in p["caches"]]
+    check_attend(p, decode=True)
+
+
+def test_a_context_of_zeros():
+    """All V scales zero: o is zero (scales below 2^-100 count as 2^-100), the logsumexp is right."""
+    p = paged_problem([400], 8, 2, 64, 16, "bf16", [1], seed=5)
+    p["gpu"][1][1].zero_()
+    p["caches"][1][1].zero_()
+    o, lse = call(p, decode=True, return_lse=True)
+    assert o.float().abs().max() < 1e-25
+    _, want, _, bound = ref.attend(p["q"], *(c.double().nan_to_num() for c, _ in p["caches"]),
+                                   *(s.double().nan_to_num() for _, s in p["caches"]), p["table"], p["lens"], p["cu"], 16)
+    assert ((lse.double().cpu() - want).abs() <= bound).all()
+
+
+def test_infinite_and_nan_queries():
+    p = paged_problem([100, 200], 4, 2, 64, 16, "fp16", [1, 1], seed=6)
+    want = call(p, decode=True)
+    p["q"][0, 1, 3] = float("inf")
+    p["q"][1, 2, 0] = float("nan")
+    got = call(p, decode=True)
+    hurt = torch.zeros(2, 4, dtype=torch.bool, device="cuda")
+    hurt[0, 1] = hurt[1, 2] = True
+    assert torch.isnan(got[hurt]).all()
+    assert torch.isfinite(got[~hurt]).all()
+    assert torch.allclose(got[~hurt].float(), want[~hurt].float(), atol=2e-2)
+
+
+def test_two_calls_at_once():
+    """Two streams, two workspaces: each result is the one that the call gives alone."""
+    problems = [paged_problem([3000, 500], 16, 2, 128, 16, "bf16", [1, 1], seed=8),
+                paged_problem([900, 800, 40], 16, 2, 128, 32, "bf16", [60, 70, 40], seed=9)]
+    want = [call(p) for p in problems]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in problems]
+    got = [[], []]
+    for _ in range(20):
+        for i, (p, s) in enumerate(zip(problems, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(call(p))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+def test_offsets_that_overlap_or_fall_stay_in_bounds():
+    """cu_seqlens_q and lengths that no program should give: rows may be wrong, guards stay."""
+    p = paged_problem([100, 60, 30], 4, 2, 64, 16, "bf16", [2, 3, 2], seed=10)
+    out = torch.full((20, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    for cu in ([0, 7, 7, 7], [5, 2, 9, -4], [0, 2 ** 30, 3, 7], [7, 0, 7, 0]):
+        for lens in ([100, 60, 30], [10 ** 9, -5, 112]):
+            p["cu"], p["lens"] = cu, lens
+            call(p, out=out[:7])
+    torch.cuda.synchronize()
+    assert (out[7:] == 7).all()
+
+
+def test_caches_beyond_four_gigabytes():
+    """Offsets past 32 bits in append and attend: blocks at the far end of two 5 GB caches."""
+    from apex_attn import custom_attention_paged_forward, kv_cache_append
+    blocks, heads, block, dim = 20480, 8, 128, 256
+    kc, vc = (torch.empty(blocks, heads, block, dim, dtype=E4M3, device="cuda") for _ in range(2))
+    ks, vs = (torch.ones(blocks, heads, device="cuda") for _ in range(2))
+    g = torch.Generator().manual_seed(11)
+    k, v = (torch.randn(200, heads, dim, generator=g).bfloat16() for _ in range(2))
+    q = torch.randn(1, heads, dim, generator=g).bfloat16()
+    ids = [blocks - 1, blocks - 2]
+    slots = [ids[t // block] * block + t % block for t in range(200)]
+    kv_cache_append(k.cuda(), v.cuda(), kc, vc, ks, vs, torch.tensor(slots, device="cuda"))
+    o = custom_attention_paged_forward(q.cuda(), kc, vc, ks, vs, ints([ids]), ints([200]))
+    small = [[torch.zeros(2, heads, block, dim, dtype=torch.float64), torch.ones(2, heads, dtype=torch.float64)]
+             for _ in range(2)]
+    for x, (codes, scale) in zip((k, v), small):
+        ref.append(x, codes, scale, [t for t in range(200)], block)
+    assert torch.equal(as_values(kc[ids])[:, :, :72], small[0][0][:, :, :72])
+    ro, _, ob, _ = ref.attend(q, small[0][0], small[1][0], small[0][1], small[1][1], [[0, 1]], [200], [0, 1], block)
+    eps = torch.finfo(torch.bfloat16).eps / 2
+    assert ((o.double().cpu() - ro).abs() <= ob + eps * (ro.abs() + ob)).all()
+    del kc, vc
+    torch.cuda.empty_cache()
+
+
+# ---------------------------------------------------------------------- refusals --
+def test_python_refusals():
+    import apex_attn
+    p = paged_problem([40, 20], 4, 2, 64, 16, "bf16", [1, 1], seed=12)
+    (kc, ks), (vc, vs) = p["gpu"]
+    q, table, lens = p["q"].cuda(), ints(p["table"]), ints(p["lens"])
+    good = dict(q=q, k_cache=kc, v_cache=vc, k_scale=ks, v_scale=vs, block_table=table, seq_lens=lens)
+    run = apex_attn.custom_attention_paged_forward
+    run(**good)
+    for change, error in [
+        (dict(q=q[0]), ValueError), (dict(q=q.float()), TypeError), (dict(q=q.cpu()), ValueError),
+        (dict(q=q[:, :3]), ValueError), (dict(q=q[:, :, :32]), ValueError),
+        (dict(k_cache=kc[:, :1]), ValueError), (dict(k_cache=kc.float(), v_cache=vc.float()), TypeError),
+        (dict(k_cache=kc[..., :32], v_cache=vc[..., :32]), KeyError),
+        (dict(k_cache=kc[:, :, :8], v_cache=vc[:, :, :8]), ValueError),
+        (dict(k_cache=kc.transpose(2, 3).contiguous().transpose(2, 3)), ValueError),
+        (dict(k_scale=ks.double()), ValueError), (dict(v_scale=vs[:1]), ValueError), (dict(k_scale=ks.cpu()), ValueError),
+        (dict(block_table=table.long()), ValueError), (dict(block_table=table[0]), ValueError),
+        (dict(block_table=table.cpu()), ValueError), (dict(block_table=table[:, :0]), ValueError),
+        (dict(seq_lens=lens.long()), ValueError), (dict(seq_lens=lens[:1]), ValueError),
+        (dict(cu_seqlens_q=ints([0, 1, 2])), ValueError), (dict(cu_seqlens_q=ints([0, 1]), max_seqlen_q=1), ValueError),
+        (dict(max_seqlen_q=3), ValueError), (dict(q=q[:1]), ValueError), (dict(window_left=-1), ValueError),
+        (dict(window_left=4, causal=False), ValueError), (dict(out=q[:, :2]), ValueError), (dict(out=q.float()), ValueError),
+        (dict(sm_scale=0.0), RuntimeError), (dict(sm_scale=float("nan")), RuntimeError)]:
+        with pytest.raises(error):
+            run(**{**good, **change})
+    assert run(**{**good, "q": q[:0], "cu_seqlens_q": ints([0, 0, 0]), "max_seqlen_q": 1}).shape == (0, 4, 64)
+
+    k = torch.zeros(3, 2, 64, dtype=torch.bfloat16, device="cuda")
+    slots = torch.arange(3, device="cuda")
+    good = dict(k=k, v=k, k_cache=kc, v_cache=vc, k_scale=ks, v_scale=vs, slots=slots)
+    for change, error in [
+        (dict(k=k[:2]), ValueError), (dict(v=k.half()), TypeError), (dict(k=k.float(), v=k.float()), TypeError),
+        (dict(k=k[:, :1], v=k[:, :1]), ValueError), (dict(slots=slots.int()), ValueError), (dict(slots=slots[:2]), ValueError),
+        (dict(slots=slots.cpu()), ValueError), (dict(v_cache=vc.cpu()), ValueError)]:
+        with pytest.raises(error):
+            apex_attn.kv_cache_append(**{**good, **change})
+    apex_attn.kv_cache_append(**{**good, "k": k[:0], "v": k[:0]})
+
+    free, count = ints(range(9)), ints([9])
+    for change in [dict(block_size=20), dict(max_new_tokens=0), dict(new_lens=ints([1])), dict(free_count=ints([1, 2])),
+                   dict(free_blocks=free.long()), dict(block_table=table.cpu()), dict(seq_lens=lens.cpu())]:
+        with pytest.raises(ValueError):
+            apex_attn.kv_cache_plan(**{**dict(block_table=table, seq_lens=lens, new_lens=lens, free_blocks=free,
+                                              free_count=count, block_size=16, max_new_tokens=5), **change})
+    with pytest.raises(ValueError):
+        apex_attn.kv_cache_release(table, lens, lens[:1], free, count, 16)
+
+
+def test_release_keeps_to_the_stack():
+    """A stack without room for all returned blocks keeps what fits."""
+    from apex_attn import kv_cache_release
+    free = ints([9, -1, -1])
+    lens, count = kv_cache_release(ints([[1, 2, 3], [4, 5, 6]]), ints([33, 16]), ints([1, 1]), free, ints([1]), 16)
+    assert lens.tolist() == [0, 0] and count.tolist() == [3] and free.tolist() == [9, 1, 2]
+
+
 # -------------------------------------------------------------- a run of them all --
 @pytest.mark.parametrize("block,dim,dtype", [(16, 64, "bf16"), (32, 128, "fp16"), (64, 256, "bf16")])
 def test_serving_steps(block, dim, dtype):
