@@ -23,6 +23,7 @@ status text otherwise.
 """
 from __future__ import annotations
 
+import ctypes
 import functools
 import math
 from typing import NamedTuple
@@ -37,8 +38,28 @@ _INT32 = torch.int32
 _HEAD_DIMS = (64, 128, 256)
 _BLOCK_SIZES = (16, 32, 64, 128)
 
-# A decode step's kernels are short, so the host's share counts: these functions ask each tensor
-# for a property once and pack the arguments in one go.
+# A decode step's kernels are short, so the host's share counts. Well-formed calls go through the
+# native module _calls, which checks, allocates and calls the library in one step; it returns
+# None for anything else, and then the Python here copies what can be copied, raises what has
+# to be raised, and makes the same call. It asks each tensor for a property once, too.
+_calls = None
+
+
+def _load_calls():
+    """The native module with the library's addresses set, or False where it was not built."""
+    global _calls
+    lib = _lib.load()
+    try:
+        from . import _calls as module
+    except ImportError:
+        module = False
+    if module:
+        module.init(*(ctypes.cast(getattr(lib, "apex_attn_" + name), ctypes.c_void_p).value for name in (
+            "kv_plan", "kv_release", "kv_append", "fwd_paged_workspace_bytes", "fwd_paged")))
+    _calls = module
+    return module
+
+
 try:
     _raw_stream = torch._C._cuda_getCurrentRawStream
 except AttributeError:  # a build of torch without CUDA, or one that names it otherwise
@@ -115,6 +136,11 @@ def kv_cache_plan(block_table, seq_lens, new_lens, free_blocks, free_count, bloc
       array had no room for. It takes no block, keeps its length, and its slots are -1.
 
     At most 8192 requests. Asynchronous on the current CUDA stream of the table's device."""
+    calls = _load_calls() if _calls is None else _calls
+    if calls:
+        done = calls.plan(block_table, seq_lens, new_lens, free_blocks, free_count, block_size, max_new_tokens)
+        if done is not None:
+            return KVCachePlan._make(done)
     if max_new_tokens < 1:
         raise ValueError("max_new_tokens must be positive")
     batch = seq_lens.numel()
@@ -135,6 +161,11 @@ def kv_cache_release(block_table, seq_lens, finished, free_blocks, free_count,
     ``[batch]``) back on the stack ``free_blocks`` (behind its first ``free_count`` entries, in
     request order). Returns the lengths (0 for those requests) and the count after it, as
     new tensors; the table rows stay as they are. Arguments as for kv_cache_plan."""
+    calls = _load_calls() if _calls is None else _calls
+    if calls:
+        done = calls.release(block_table, seq_lens, finished, free_blocks, free_count, block_size)
+        if done is not None:
+            return done
     lens, count = torch.empty_like(seq_lens), torch.empty_like(free_count)
     _bookkeeping(_lib.load().apex_attn_kv_release, "kv_cache_release", block_table, seq_lens, None, finished,
                  free_blocks, free_count, block_size, 0, 0, lens.data_ptr(), count.data_ptr(), 0, 0)
@@ -206,6 +237,9 @@ def kv_cache_append(k, v, k_cache, v_cache, k_scale, v_scale, slots) -> None:
     not finite are stored as NaN and leave the scale alone. In one call at most one run may go
     to a block, and a block must belong to one request. ``slots`` may be longer than ``k``
     (then its first ``total`` entries count)."""
+    calls = _load_calls() if _calls is None else _calls
+    if calls and calls.append(k, v, k_cache, v_cache, k_scale, v_scale, slots) is not None:
+        return
     shape = k.shape
     if len(shape) != 3 or shape != v.shape:
         raise ValueError(f"k and v must be [total, H_kv, D] alike, got {tuple(k.shape)}, {tuple(v.shape)}")
@@ -250,6 +284,12 @@ def custom_attention_paged_forward(q, k_cache, v_cache, k_scale, v_scale, block_
     they hold.
 
     Head dims 64, 128, 256 (others: KeyError). Asynchronous on the current CUDA stream."""
+    calls = _load_calls() if _calls is None else _calls
+    if calls:
+        done = calls.attend(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens_q, max_seqlen_q,
+                            causal, sm_scale, return_lse, window_left, out)
+        if done is not None:
+            return done
     shape = q.shape
     if len(shape) != 3:
         raise ValueError(f"q must be [total_q, H, D], got {tuple(shape)}")

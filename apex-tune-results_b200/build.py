@@ -1,18 +1,22 @@
-"""Builds libapex_attn.so in-tree (next to the apex_attn package) with nvcc for sm_100a.
+"""Builds libapex_attn.so in-tree (next to the apex_attn package) with nvcc for sm_100a, and the
+Python module _calls.so beside it with g++.
 
 Usage: python apex-tune-results_b200/build.py [--verbose]
 Each source is compiled to an object under _build/ (side by side, and only when it or a
 header changed), then linked. The library links the CUDA runtime statically and resolves
 cuTensorMapEncodeTiled through cudaGetDriverEntryPoint, so it needs no -lcuda and loads on
-a machine without a GPU.
+a machine without a GPU. _calls.so uses the headers of the installed torch and links to its
+libraries.
 """
 from __future__ import annotations
 
 import argparse
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -27,6 +31,8 @@ HEADERS = {
     SOURCES[0]: _SHARED + [os.path.join(CSRC, f) for f in ("attn_fwd_tile_kernel.cuh", "attn_bwd_kernel.cuh")],
     SOURCES[1]: _SHARED + [os.path.join(CSRC, f) for f in ("attn_paged_kernel.cuh", "kv_cache_kernels.cuh")],
 }
+CALLS_SOURCE = os.path.join(CSRC, "torch_calls.cpp")
+CALLS_OUT = os.path.join(HERE, "apex_attn", "_calls.so")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo", "-Xptxas", "-v",
          "-Xcompiler", "-fPIC", "-I", os.path.join(ROOT, "include"), "-I", CSRC]
 
@@ -55,7 +61,30 @@ def up_to_date() -> bool:
     return newer(OUT, inputs)
 
 
+def calls_command(out: str) -> list[str]:
+    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    include = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include"),
+               os.path.join(ROOT, "include")]
+    libs = ["torch_python", "torch", "torch_cpu", "torch_cuda", "c10", "c10_cuda"]
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            "-D_GLIBCXX_USE_CXX11_ABI=1", *("-I" + p for p in include), "-o", out, CALLS_SOURCE,
+            "-L" + os.path.join(torch_dir, "lib"), *("-l" + name for name in libs)]
+
+
+def build_calls(force: bool = False) -> str:
+    if force or not newer(CALLS_OUT, [CALLS_SOURCE, API, __file__]):
+        tmp = CALLS_OUT + ".tmp"
+        proc = subprocess.run(calls_command(tmp), capture_output=True, text=True)
+        if proc.returncode != 0:
+            sys.stderr.write(proc.stdout + proc.stderr)
+            raise RuntimeError("g++ failed building _calls.so")
+        os.replace(tmp, CALLS_OUT)
+    return CALLS_OUT
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
+    build_calls(force)
     if not force and up_to_date():
         return OUT
     os.makedirs(OBJ, exist_ok=True)

@@ -743,3 +743,40 @@ def test_a_captured_step_replays_with_new_lengths():
             assert torch.equal(o2, want) and torch.equal(lse2, wl)
         state["lens"].copy_(plan.seq_lens)
         state["count"].copy_(plan.free_count)
+
+
+def test_native_and_python_ways_agree():
+    """Every call of a step through the native module and through Python: the same results."""
+    import apex_attn.paged as paged
+    if not (paged._calls or paged._load_calls()):
+        pytest.skip("_calls is not built")
+    native = paged._calls
+    used = []
+    results = []
+    for way in (native, False):
+        paged._calls = way
+        try:
+            table, free = ints([[0] * 8 for _ in range(3)]), ints(list(range(20)))
+            kc, ks = new_cache(20, 2, 16, 64, True, 1)
+            vc, vs = new_cache(20, 2, 16, 64, False, 2)
+            g = torch.Generator(device="cuda").manual_seed(5)
+            q = torch.randn(40, 8, 64, generator=g, device="cuda").half()
+            lens, count = paged.kv_cache_release(table, ints([0, 0, 0]), ints([0, 1, 0]), free, ints([20]), 16)
+            plan = paged.kv_cache_plan(table, lens, ints([20, 3, 17]), free, count, 16, 40)
+            assert isinstance(plan, paged.KVCachePlan)
+            paged.kv_cache_append(q[:, :2], q[:, 2:4], kc, vc, ks, vs, plan.slots)
+            out = torch.zeros_like(q)
+            got = [paged.custom_attention_paged_forward(q, kc, vc, ks, vs, table, plan.seq_lens, plan.cu_seqlens, 20,
+                                                        return_lse=True, window_left=7, sm_scale=0.2),
+                   paged.custom_attention_paged_forward(q, kc, vc, ks, vs, table, plan.seq_lens, plan.cu_seqlens, 20,
+                                                        causal=False, out=out),
+                   paged.custom_attention_paged_forward(q[:3], kc, vc, ks, vs, table, plan.seq_lens)]
+            assert got[1] is out
+            results.append([*plan, table, lens, kc.float(), vc.float(), ks, vs, *got[0], *got[1:]])
+            used.append(paged._calls)
+        finally:
+            paged._calls = native
+    for a, b in zip(*results):
+        assert a.shape == b.shape and a.dtype == b.dtype and a.stride() == b.stride()
+        assert torch.equal(a, b)
+    assert native.attend(q.float(), kc, vc, ks, vs, table, plan.seq_lens, None, None, True, None, False, None, None) is None
