@@ -7,13 +7,16 @@
 //
 // The codes never leave 8 bits: both products run on tcgen05.mma kind::f8f6f4 with the cache
 // tiles as the TMA wrote them to shared memory, so nothing converts the cache. What is not
-// e4m3 is split into e4m3 terms that add up to it, two for bf16 calls and three for fp16 ones:
+// e4m3 is split into terms that add up to it, two of e4m3 for bf16 calls, and a third of e5m2 for
+// fp16 ones:
 //   * q, scaled per row by a power of two so that its largest magnitude lies in (224, 448]: its
-//     8 or 11 significant bits in pieces of 4, exact but for values below 2^-9 of that range;
+//     8 or 11 significant bits in pieces of 4, 4 and 3, exact but for what lies below 2^-10 (two
+//     terms) or 2^-17;
 //   * the weight p'_ij = 2^(x_ij + log2 b_j - m_i) (the V scale goes into the exponent, one
-//     addition per token), rounded to fp16: off by 2^-8 (two terms) or 2^-12 of itself, or by
-//     2^-10 absolutely. With two terms an fp16 output was 3.3 times as far from its float64
-//     value as rounding alone puts it; a bf16 output's own rounding hides the difference.
+//     addition per token), rounded to fp16: off by 2^-8 of itself or 2^-10 (two terms), by 2^-11 of
+//     itself or 2^-17 (three). With two terms an fp16 output was 3.3 times as far from its float64
+//     value as rounding alone puts it; a bf16 output's own rounding hides the difference. With
+//     three terms of e4m3, 131k flat weights still made it 1.8 times as far.
 // fp32 accumulation of e4m3 products on this card is exact to 2^-23 of the magnitudes.
 //
 // Tokens, not query rows, are the M side: S^T = K Q^T and O^T = V^T P, M = 128 tokens resp. 128
@@ -411,6 +414,18 @@ __device__ __forceinline__ PagedStart paged_start_cta(const PagedParams& p, long
   return s;
 }
 
+// Four fp16 values to e5m2, a.x in the lowest byte.
+__device__ __forceinline__ uint32_t e5m2x4_of_half2(__half2 a, __half2 b) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\t"
+      "cvt.rn.satfinite.e5m2x2.f16x2 lo, %1;\n\t"
+      "cvt.rn.satfinite.e5m2x2.f16x2 hi, %2;\n\t"
+      "mov.b32 %0, {lo, hi};\n\t}"
+      : "=r"(r)
+      : "r"(*reinterpret_cast<uint32_t*>(&a)), "r"(*reinterpret_cast<uint32_t*>(&b)));
+  return r;
+}
+
 // Four fp16 values to e4m3 (a.x in the lowest byte) and back. One asm block each, so that the
 // halves are converted in place instead of being moved and merged.
 __device__ __forceinline__ uint32_t e4m3x4_of_half2(__half2 a, __half2 b) {
@@ -434,6 +449,26 @@ __device__ __forceinline__ void half2_of_e4m3x4(uint32_t v, __half2& a, __half2&
       : "r"(v));
   a = *reinterpret_cast<__half2*>(&x);
   b = *reinterpret_cast<__half2*>(&y);
+}
+
+// Splits four fp16 values into K terms that add up to them: e4m3, and of three the last e5m2, whose
+// smallest values lie 2^7 below e4m3's (a third piece has three bits left, as many as it holds).
+template <int K>
+__device__ __forceinline__ void split_terms(__half2 a, __half2 b, uint32_t (&term)[K]) {
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    if (i == 2) {
+      term[i] = e5m2x4_of_half2(a, b);
+      continue;
+    }
+    term[i] = e4m3x4_of_half2(a, b);
+    if (i + 1 < K) {
+      __half2 ra, rb;
+      half2_of_e4m3x4(term[i], ra, rb);
+      a = __hsub2(a, ra);
+      b = __hsub2(b, rb);
+    }
+  }
 }
 
 // Sums N (at most 32) values per lane over the warp; each lane ends with the sum of one in
@@ -525,16 +560,10 @@ __device__ __forceinline__ void split_query_rows(const PagedParams& p, const Pag
       const float2 f = __fmul2_rn(Elem<T>::to_float2(x[2 * k]), make_float2(inv, inv));
       const float2 g = __fmul2_rn(Elem<T>::to_float2(x[2 * k + 1]), make_float2(inv, inv));
       __half2 a = __floats2half2_rn(f.x, f.y), b = __floats2half2_rn(g.x, g.y);
+      uint32_t four[C::kTerms];
+      split_terms(a, b, four);
 #pragma unroll
-      for (int j = 0; j < C::kTerms; ++j) {
-        term[j][k] = e4m3x4_of_half2(a, b);
-        if (j + 1 < C::kTerms) {
-          __half2 ra, rb;
-          half2_of_e4m3x4(term[j][k], ra, rb);
-          a = __hsub2(a, ra);
-          b = __hsub2(b, rb);
-        }
-      }
+      for (int j = 0; j < C::kTerms; ++j) term[j][k] = four[j];
     }
 #pragma unroll
     for (int j = 0; j < C::kTerms; ++j)
@@ -853,16 +882,10 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
                 const float2 e1 = make_float2(ptx::ex2(d[x + 1].x), ptx::ex2(d[x + 1].y));
                 sum = __fadd2_rn(sum, __fadd2_rn(e0, e1));
                 __half2 a = __floats2half2_rn(e0.x, e0.y), b = __floats2half2_rn(e1.x, e1.y);
+                uint32_t four[C::kTerms];
+                split_terms(a, b, four);
 #pragma unroll
-                for (int i = 0; i < C::kTerms; ++i) {
-                  term[i][k] = e4m3x4_of_half2(a, b);
-                  if (i + 1 < C::kTerms) {
-                    __half2 ra, rb;
-                    half2_of_e4m3x4(term[i][k], ra, rb);
-                    a = __hsub2(a, ra);
-                    b = __hsub2(b, rb);
-                  }
-                }
+                for (int i = 0; i < C::kTerms; ++i) term[i][k] = four[i];
               }
               l = fmaf(sum.x + sum.y, sc[c16 >> p.block_shift].z, l);
               const uint32_t unit = (uint32_t)((c16 >> 4) ^ (t & 7)) << 4;
@@ -1082,16 +1105,10 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
             l[x] = __ffma2_rn(e0, i2, l[x]);
             l[x + 1] = __ffma2_rn(e1, i2, l[x + 1]);
             __half2 a = __floats2half2_rn(e0.x, e0.y), b = __floats2half2_rn(e1.x, e1.y);
+            uint32_t four[C::kTerms];
+            split_terms(a, b, four);
 #pragma unroll
-            for (int j2 = 0; j2 < C::kTerms; ++j2) {
-              term[j2][k >> 2] = e4m3x4_of_half2(a, b);
-              if (j2 + 1 < C::kTerms) {
-                __half2 ra, rb;
-                half2_of_e4m3x4(term[j2][k >> 2], ra, rb);
-                a = __hsub2(a, ra);
-                b = __hsub2(b, rb);
-              }
-            }
+            for (int j2 = 0; j2 < C::kTerms; ++j2) term[j2][k >> 2] = four[j2];
           }
 #pragma unroll
           for (int j2 = 0; j2 < C::kTerms; ++j2)
@@ -1272,6 +1289,10 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     constexpr uint32_t idS = kDesc | ((uint32_t)(NQ >> 3) << 17);
     constexpr uint32_t idPV = C::kQueryMajor ? kDesc | (1u << 16) | ((uint32_t)(D >> 3) << 17)
                                              : kDesc | (1u << 15) | (1u << 16) | ((uint32_t)(NQ >> 3) << 17);
+    // The operand that is split is e5m2 in its third term.
+    auto with_type = [](uint32_t id, int term) {
+      return term == 2 ? id | (1u << (C::kQueryMajor ? 7 : 10)) : id;
+    };
     uint32_t reads = 0;  // ring slots consumed
     int gs = 0, gp = 0;  // S and P V tiles issued
     auto acquire = [&]() -> int {
@@ -1300,10 +1321,10 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
               const uint32_t dS = tmem + (uint32_t)(sb * NQ);
               if constexpr (C::kQueryMajor) {
                 const uint64_t q = ptx::smem_desc(rows + ch * (NQ * C::kRow) + ks * 32, 16, 8 * C::kRow, C::kSwizzle);
-                ptx::umma_ss_f8_warp(dS, q, k, idS, acc);
+                ptx::umma_ss_f8_warp(dS, q, k, with_type(idS, j), acc);
               } else {
                 const uint64_t q = ptx::smem_desc(rows + (ch * (C::kRow / 16) + 2 * ks) * (NQ * 16), NQ * 16, 128, 0);
-                ptx::umma_ss_f8_warp(dS, k, q, idS, acc);
+                ptx::umma_ss_f8_warp(dS, k, q, with_type(idS, j), acc);
               }
               acc = 1;
             }
@@ -1330,7 +1351,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
 #pragma unroll
             for (int j = 0; j < C::kTerms; ++j) {
               const uint64_t w = ptx::smem_desc(weights + j * C::kPTerm + ks * 32, 16, 1024, 2);
-              ptx::umma_ss_f8_warp(dO, w, v, idPV, first && ks == 0 && j == 0 ? 0u : 1u);
+              ptx::umma_ss_f8_warp(dO, w, v, with_type(idPV, j), first && ks == 0 && j == 0 ? 0u : 1u);
             }
           }
         } else {
@@ -1345,7 +1366,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
 #pragma unroll
               for (int j = 0; j < C::kTerms; ++j) {
                 const uint64_t w = ptx::smem_desc(weights + j * C::kPTerm + ks * 32 * 16, 128, 2048, 0);
-                ptx::umma_ss_f8_warp(dO + (uint32_t)(ch * NQ), v, w, idPV, first && ks == 0 && j == 0 ? 0u : 1u);
+                ptx::umma_ss_f8_warp(dO + (uint32_t)(ch * NQ), v, w, with_type(idPV, j), first && ks == 0 && j == 0 ? 0u : 1u);
               }
             }
         }
