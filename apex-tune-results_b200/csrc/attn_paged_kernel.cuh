@@ -253,6 +253,7 @@ struct PagedWalk {
   int unit, end, share, more;
   int b, h, qt, qts;
   int item;  // first unit of the item (b, h, qt)
+  int tiles_begin = 0, tiles_end = 0;  // units of the tiles of the last segment's item
   PagedRequest r;
 
   __device__ __forceinline__ PagedWalk(const PagedParams& params, const PagedStart& s)
@@ -261,9 +262,10 @@ struct PagedWalk {
     if (unit >= end) return;
     r = paged_request(p, b);
     qts = paged_qtiles<NQ>(p, r);
-    const int per_head = paged_head_units<NQ>(p, r);
-    if (p.heads_kv > 1) {
-      h = (int)((unsigned)(unit - item) / (unsigned)per_head);
+    const int into = unit - item;
+    if (p.heads_kv > 1 && into > 0) {
+      const int per_head = paged_head_units<NQ>(p, r);
+      h = (int)((unsigned)into / (unsigned)per_head);
       item += h * per_head;
     }
     while (qt + 1 < qts) {
@@ -319,17 +321,21 @@ struct PagedWalk {
       s.hi_all = p.causal ? min(r.len, place + span.i0 + 1) : r.len;
       s.lo_all = p.window >= 0 ? max(0, place + span.i1 - p.window) : 0;
       s.slot = -1;
-      if (to - from < n) {
-        s.slot = 2 * (int)blockIdx.x + (from > first ? 0 : 1);
-        if ((threadIdx.x & 31) == 0) {
-          int4* at = reinterpret_cast<int4*>(p.share + s.slot * kShareInts);
-          at[0] = make_int4(r.q0, h, s.rows, s.token0);
-          at[1] = make_int4(cta_of(first), cta_of(last - 1), s.head0, 0);
-        }
-      }
+      if (to - from < n) s.slot = 2 * (int)blockIdx.x + (from > first ? 0 : 1);
+      tiles_begin = first;
+      tiles_end = last;
       return s;
     }
     return s;
+  }
+
+  // Leaves the joining kernel what it needs to know of a segment that is part of an item. (After
+  // the segment is published: nobody waits for this.)
+  __device__ __forceinline__ void share_out(const PagedSegment& s) const {
+    if (s.n < 0 || s.slot < 0 || (threadIdx.x & 31) != 0) return;
+    int4* at = reinterpret_cast<int4*>(p.share + s.slot * kShareInts);
+    at[0] = make_int4(s.q0, s.h, s.rows, s.token0);
+    at[1] = make_int4(cta_of(tiles_begin), cta_of(tiles_end - 1), s.head0, 0);
   }
 };
 
@@ -1418,10 +1424,12 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     int g = 0;
     seg = walk.next();
     publish(seg);
+    walk.share_out(seg);
     while (seg.n >= 0) {
       // One segment ahead of its scales, so that the other roles can look ahead too.
       const PagedSegment then = walk.next();
       publish(then);
+      walk.share_out(then);
 #pragma unroll 1
       for (int j0 = 0; j0 < seg.n; j0 += 4) {
         const int j = j0 + (lane >> 3), page = lane & 7;
