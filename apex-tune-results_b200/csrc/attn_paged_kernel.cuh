@@ -91,7 +91,10 @@ struct PagedCfg {
   static constexpr int kChunks = (D + 127) / 128;
   static constexpr uint32_t kSwizzle = kRow == 128 ? 2 : 4;
   static constexpr int kTerms = std::is_same<T, __half>::value ? 3 : 2;  // of q
-  static constexpr bool kQueryMajor = NQ == 128;
+  static constexpr bool kQueryMajor = NQ >= 64;
+  // Columns of an S buffer. (Query-major M is 128 for 64-row tiles too: the products read what lies
+  // behind the 64 rows of Q and of the weights, and nobody reads rows 64 .. 127 of the results.)
+  static constexpr int kSCols = kQueryMajor ? kPagedTile : NQ;
   static constexpr int kWG = kQueryMajor ? 4 : 1;        // softmax warpgroups
   // Query-major, d <= 128: two pairs of warpgroups take the tiles in turn, each pair with its own
   // maxima, sums and O, so that one's exponentials run while the other loads and converts.
@@ -107,7 +110,7 @@ struct PagedCfg {
   static constexpr int kQBytes = kTerms * NQ * D;        // one segment's query rows
   static constexpr int kPTerm = kPagedTile * NQ;         // one term of one P buffer
   static constexpr int kBudget = kCtas == 2 ? 115712 : 232448;
-  static constexpr int kMiscBytes = 2240 + NQ * (NQ == 128 ? 96 : 56);      // what the plan below adds
+  static constexpr int kMiscBytes = 2240 + NQ * 56 + (kQueryMajor ? 14 * 128 * 4 : 0);      // what the plan below adds
   static constexpr int slots(int q_bufs, int p_bufs) {
     return (kBudget - q_bufs * kQBytes - p_bufs * kTerms * kPTerm - kMiscBytes) / kSlotBytes;
   }
@@ -121,9 +124,9 @@ struct PagedCfg {
   static_assert(kNS > kLead, "the ring needs K(j + kLead) beside V(j)");
   static constexpr int kScaleRing = 8;
   static constexpr int kSegRing = 4;
-  // TMEM: S buffers at 0 and NQ, O from 2 NQ on (token-major: a block of NQ columns per 128 of
+  // TMEM: S buffers at 0 and kSCols, O from 2 kSCols on (token-major: a block of NQ columns per 128 of
   // the head dim; query-major: the head dim, for each pair).
-  static constexpr int kTmemUsed = kQueryMajor ? 2 * NQ + kPairs * D : (2 + kChunks) * NQ;
+  static constexpr int kTmemUsed = 2 * kSCols + (kQueryMajor ? kPairs * D : kChunks * NQ);
   static constexpr int kTmemCols = kTmemUsed <= 64 ? 64 : (kTmemUsed <= 128 ? 128 : (kTmemUsed <= 256 ? 256 : 512));
   static_assert(kTmemUsed <= 512 && kCtas * kTmemCols <= 512, "TMEM plan");
   // shared-memory plan
@@ -137,12 +140,13 @@ struct PagedCfg {
   static constexpr int kScales = (kBars + kNumBars * 8 + 15) / 16 * 16;  // float4 [kScaleRing][8 pages]
   static constexpr int kCol = kScales + kScaleRing * 8 * 16;  // two of, per query row: -m, q scale, factor, hi, lo
   static constexpr int kRed = kCol + 2 * 5 * NQ * 4;          // token-major [4 warps][NQ], query-major [14][128]
-  static constexpr int kSegs = (kRed + (kQueryMajor ? 14 : 4) * NQ * 4 + 15) / 16 * 16;       // int4 [kSegRing][kSegVecs]
+  static constexpr int kSegs = (kRed + (kQueryMajor ? 14 * 128 : 4 * NQ) * 4 + 15) / 16 * 16;       // int4 [kSegRing][kSegVecs]
   static constexpr int kBad = kSegs + kSegRing * 4 * 16;                 // unsigned [2][4]
   static constexpr int kScan = kBad + 32;                // long long [32], found request
   static constexpr int kMisc = kScan + 32 * 8 + 16;
   static constexpr int kBytes = kMisc + 16;
   static_assert(kBytes <= kBudget, "shared-memory plan");
+  static_assert(!kQueryMajor || kBytes - kBars >= (128 - NQ) * 128, "rows behind the last weights");
 };
 
 // The query rows of request b and where they stand.
@@ -790,7 +794,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           ptx::tc_fence_after();
           float2 d[NC / 2];
           auto load = [&](int c0) {  // 32 tokens' scores
-            const uint32_t at = tmem + lane_off + (uint32_t)(sb * NQ + c0);
+            const uint32_t at = tmem + lane_off + (uint32_t)(sb * C::kSCols + c0);
             ptx::tmem_ld16(at, reinterpret_cast<uint32_t*>(d));
             ptx::tmem_ld16(at + 16, reinterpret_cast<uint32_t*>(d) + 16);
             ptx::tmem_wait_ld();
@@ -833,12 +837,12 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           const bool move = force || left ? true : ptx::named_bar_or(vote, 32 * kWGs, most > kPagedMost);
           force = left;
           if (move) {
-            float* const tops = exchange + ((g / C::kPairs) & 1) * C::kWG * NQ;
-            tops[wg * NQ + t] = most;
+            float* const tops = exchange + ((g / C::kPairs) & 1) * C::kWG * 128;
+            tops[wg * 128 + t] = most;
             ptx::named_bar_sync(vote, 32 * kWGs);
             float top = most;
 #pragma unroll
-            for (int k = 0; k < kWGs; ++k) top = fmaxf(top, tops[(pair * kWGs + k) * NQ + t]);
+            for (int k = 0; k < kWGs; ++k) top = fmaxf(top, tops[(pair * kWGs + k) * 128 + t]);
             // By how much the maximum moves: up only, but freely the first time.
             const bool some = top != -INFINITY;
             const float by = some ? (set ? fmaxf(top - kPagedTop, 0.f) : top - kPagedTop) : 0.f;
@@ -856,7 +860,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
               ptx::tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < D / kWGs; c += 16) {
-                const uint32_t at = tmem + lane_off + (uint32_t)(2 * NQ + pair * D + wg % kWGs * (D / kWGs) + c);
+                const uint32_t at = tmem + lane_off + (uint32_t)(2 * C::kSCols + pair * D + wg % kWGs * (D / kWGs) + c);
                 uint32_t v[16];
                 ptx::tmem_ld16(at, v);
                 ptx::tmem_wait_ld();
@@ -907,7 +911,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           if (lane == 0) ptx::mbar_arrive(bar(C::kSFree + sb));
           clear_unseen(j, 13 + pair, [&](int x) {
             const int pos = pos0 + x;
-            if (x >= tok0 && x < tok0 + kTok && pos >= lo && pos < hi)
+            if (!idle && x >= tok0 && x < tok0 + kTok && pos >= lo && pos < hi)
               ptx::st_shared_u8(sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kTerms * C::kPTerm + t * 128 +
                                     (((x >> 4) ^ (t & 7)) << 4) + (x & 15), 0x7fu);
           });
@@ -927,23 +931,23 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
         if (more) split(then, n + 1);
 
         // ---- the segment's result: this thread's row, a quarter of its columns ----
-        float* const sums = exchange + 2 * C::kWG * NQ;
-        float* const refs = sums + C::kWG * NQ;
-        sums[wg * NQ + t] = l;
-        if (wg % kWGs == 0) refs[pair * NQ + t] = set ? nm : INFINITY;
+        float* const sums = exchange + 2 * C::kWG * 128;
+        float* const refs = sums + C::kWG * 128;
+        sums[wg * 128 + t] = l;
+        if (wg % kWGs == 0) refs[pair * 128 + t] = set ? nm : INFINITY;
         ptx::named_bar_sync(9 + quarter, 32 * C::kWG);
         float ref = refs[t];
 #pragma unroll
-        for (int k = 1; k < C::kPairs; ++k) ref = fminf(ref, refs[k * NQ + t]);
+        for (int k = 1; k < C::kPairs; ++k) ref = fminf(ref, refs[k * 128 + t]);
         // o = (sum_k f_k O_k) / (sum_k f_k l_k) over the pairs, f_k = 2^(m_k - max m).
         float f[C::kPairs], sum = 0.f;
 #pragma unroll
         for (int k = 0; k < C::kPairs; ++k) {
-          const float mine = refs[k * NQ + t];
+          const float mine = refs[k * 128 + t];
           f[k] = mine == INFINITY ? 0.f : ptx::ex2(ref - mine);
           float s = 0.f;
 #pragma unroll
-          for (int x = 0; x < kWGs; ++x) s += sums[(k * kWGs + x) * NQ + t];
+          for (int x = 0; x < kWGs; ++x) s += sums[(k * kWGs + x) * 128 + t];
           sum = fmaf(f[k], s, sum);
         }
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -969,7 +973,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
 #pragma unroll
           for (int k = 0; k < C::kPairs; ++k) {
             uint32_t v[16];
-            ptx::tmem_ld16(tmem + lane_off + (uint32_t)(2 * NQ + k * D + c), v);
+            ptx::tmem_ld16(tmem + lane_off + (uint32_t)(2 * C::kSCols + k * D + c), v);
             ptx::tmem_wait_ld();
             ptx::reg_fence16(v);
             // f = 0: the pair has nothing of this row, and TMEM may hold anything.
@@ -1292,7 +1296,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     // e4m3, fp32 sums, M = 128. S: both operands K-major. P V: V is always MN-major; the weights
     // are MN-major as the B operand (token-major), K-major as the A operand (query-major).
     constexpr uint32_t kDesc = (1u << 4) | ((uint32_t)(128 >> 4) << 24);
-    constexpr uint32_t idS = kDesc | ((uint32_t)(NQ >> 3) << 17);
+    constexpr uint32_t idS = kDesc | ((uint32_t)(C::kSCols >> 3) << 17);
     constexpr uint32_t idPV = C::kQueryMajor ? kDesc | (1u << 16) | ((uint32_t)(D >> 3) << 17)
                                              : kDesc | (1u << 15) | (1u << 16) | ((uint32_t)(NQ >> 3) << 17);
     // The operand that is split is e5m2 in its third term.
@@ -1324,7 +1328,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
 #pragma unroll
             for (int j = 0; j < C::kTerms; ++j) {
               const uint32_t rows = sbase + C::kQ + (n % C::kQBufs) * C::kQBytes + j * NQ * D;
-              const uint32_t dS = tmem + (uint32_t)(sb * NQ);
+              const uint32_t dS = tmem + (uint32_t)(sb * C::kSCols);
               if constexpr (C::kQueryMajor) {
                 const uint64_t q = ptx::smem_desc(rows + ch * (NQ * C::kRow) + ks * 32, 16, 8 * C::kRow, C::kSwizzle);
                 ptx::umma_ss_f8_warp(dS, q, k, with_type(idS, j), acc);
@@ -1348,7 +1352,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       ptx::tc_fence_after();
       if (ok) {
         const uint32_t weights = sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kTerms * C::kPTerm;
-        const uint32_t dO = tmem + (uint32_t)(2 * NQ + (C::kPairs == 2 ? sb * D : 0));
+        const uint32_t dO = tmem + (uint32_t)(2 * C::kSCols + (C::kPairs == 2 ? sb * D : 0));
         if constexpr (C::kQueryMajor) {
 #pragma unroll
           for (int ks = 0; ks < kPagedTile / 32; ++ks) {

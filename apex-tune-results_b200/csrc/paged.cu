@@ -200,9 +200,10 @@ int append(const apex_attn_kv_append_args* a, void* stream) {
 // -------------------------------------------------------------------- attention --
 constexpr int kMaxSms = 160;  // the workspace holds what this many SMs' CTAs may write
 
-// Query rows per tile: 16 or 32 (tokens as the M side of the products) where they hold all rows of
-// a request's K/V head, else 128 (query rows as the M side).
-int query_tile(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 128; }
+// Query rows per tile, the smallest that holds all rows of a request's K/V head: 16 or 32 with
+// tokens as the M side of the products, 64 with the query rows (half the shared memory for rows
+// and weights, so more of the cache under way), else 128.
+int query_tile(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
 struct Workspace {
   size_t share, lse, o, bytes;  // offsets and size
@@ -282,6 +283,7 @@ int launch_tile(int tile, const apex::PagedParams& p, const CUtensorMap& mk, con
   switch (tile) {
     case 16: return launch_paged<T, D, 16>(p, mk, mv, dev, num_sms, s);
     case 32: return launch_paged<T, D, 32>(p, mk, mv, dev, num_sms, s);
+    case 64: return launch_paged<T, D, 64>(p, mk, mv, dev, num_sms, s);
     default: return launch_paged<T, D, 128>(p, mk, mv, dev, num_sms, s);
   }
 }
