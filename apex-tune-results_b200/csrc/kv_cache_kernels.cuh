@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(1024) kv_release_kernel(const PlanParams p) {
 }
 
 // ----------------------------------------------------------------------- append --
-constexpr int kAppendWarps = 8;
+constexpr int kAppendWarps = 4;
 constexpr int kMinScaleExponent = -100;
 
 struct AppendParams {
@@ -269,11 +269,13 @@ struct Elem<__half> {
 // looks at one token of the window each, so that finding the runs is one load. A run of up to
 // 2048 values (16 tokens of 128) stays in registers between the pass for the maximum and the
 // one for the codes; a longer one is read again, from the L2.
-// Bound: DRAM for prompts (2 bytes read, 1 written per value), latency for a decode step.
+// Bound: DRAM for prompts (2 bytes read, 1 written per value): 25k tokens of 8 heads of 128 in
+// 29.5 us, 5.2 TB/s of 6.6; with 80 registers and three quarters of the warps it took 36 us, with
+// eight warps per CTA 30.4. Latency for a decode step: 3.3 us.
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * kAppendWarps, 3) kv_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(32 * kAppendWarps, 8) kv_append_kernel(const AppendParams p) {
   constexpr int kPerRow = D / 8;   // 8 values (16 bytes of input) per lane and step
-  constexpr int kAhead = 8;        // steps in registers at once
+    constexpr int kAhead = 8;        // steps in registers at once
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int unit = blockIdx.y * kAppendWarps + warp;
   if (unit >= 2 * p.heads) return;
@@ -375,26 +377,27 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 3) kv_append_kernel(const A
     const float inv = 1.f / s;
     unsigned char* to = dst + (o + row) * p.c_st[kv] + col;
     const long long to_step = kRows * p.c_st[kv];
-    auto codes_of = [&](uint32_t a, uint32_t b) -> uint32_t {
-      float2 f = Elem<T>::to_float2(a), g = Elem<T>::to_float2(b);
-      if (plain) {
-        f = __fmul2_rn(f, make_float2(inv, inv));
-        g = __fmul2_rn(g, make_float2(inv, inv));
-      } else {
-        auto quotient = [&](float q) { return isfinite(q) ? q / s : __int_as_float(0x7fffffff); };
-        f = make_float2(quotient(f.x), quotient(f.y));
-        g = make_float2(quotient(g.x), quotient(g.y));
-      }
-      return e4m3x4(f, g);
-    };
-    for (int base = 0; base < chunks; base += 32 * kAhead) {
-      if (chunks > 32 * kAhead) load(base);
-      unsigned char* at = to + base / 32 * to_step;
+    auto write = [&](auto&& quotient) {
+      for (int base = 0; base < chunks; base += 32 * kAhead) {
+        if (chunks > 32 * kAhead) load(base);
+        unsigned char* at = to + base / 32 * to_step;
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k)
-        if (base + 32 * k + lane < chunks)
-          *reinterpret_cast<uint2*>(at + k * to_step) =
-              make_uint2(codes_of(v[k].x, v[k].y), codes_of(v[k].z, v[k].w));
+        for (int k = 0; k < kAhead; ++k) {
+          if (base + 32 * k + lane < chunks) {
+            const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+            float2 f[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = quotient(Elem<T>::to_float2(w[e]));
+            *reinterpret_cast<uint2*>(at + k * to_step) = make_uint2(e4m3x4(f[0], f[1]), e4m3x4(f[2], f[3]));
+          }
+        }
+      }
+    };
+    if (plain) {
+      write([&](float2 f) { return __fmul2_rn(f, make_float2(inv, inv)); });
+    } else {
+      auto one = [&](float q) { return isfinite(q) ? q / s : __int_as_float(0x7fffffff); };
+      write([&](float2 f) { return make_float2(one(f.x), one(f.y)); });
     }
   }
 }

@@ -185,10 +185,10 @@ int append(const apex_attn_kv_append_args* a, void* stream) {
   p.total = a->total;
   p.heads = a->heads_kv;
   p.block_shift = shift;
-  // A window of one token while that leaves at most four CTAs for each of the device's places
-  // (decode: every token is a run of its own); else windows that a run mostly fills.
+  // A window of one token while that makes at most 32 CTAs per SM (decode: every token is a run of
+  // its own); else windows that a run mostly fills.
   const int groups = (2 * a->heads_kv + apex::kAppendWarps - 1) / apex::kAppendWarps;
-  const bool few = (long long)a->total * groups <= 4LL * 8 * d.num_sms;
+  const bool few = (long long)a->total * groups <= 32LL * d.num_sms;
   p.window = few ? 1 : std::min(a->block_size, 32);
   const dim3 grid((unsigned)((a->total + p.window - 1) / p.window), (unsigned)groups);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
