@@ -37,6 +37,7 @@ _E4M3 = torch.float8_e4m3fn
 _INT32 = torch.int32
 _HEAD_DIMS = (64, 128, 256)
 _BLOCK_SIZES = (16, 32, 64, 128)
+_INT_MAX = 2 ** 31 - 1
 
 # A decode step's kernels are short, so the host's share counts. Well-formed calls go through the
 # native module _calls, which checks, allocates and calls the library in one step; it returns
@@ -141,8 +142,8 @@ def kv_cache_plan(block_table, seq_lens, new_lens, free_blocks, free_count, bloc
         done = calls.plan(block_table, seq_lens, new_lens, free_blocks, free_count, block_size, max_new_tokens)
         if done is not None:
             return KVCachePlan._make(done)
-    if max_new_tokens < 1:
-        raise ValueError("max_new_tokens must be positive")
+    if not 1 <= max_new_tokens <= 2 ** 30:
+        raise ValueError(f"max_new_tokens must lie in [1, 2^30], got {max_new_tokens}")
     batch = seq_lens.numel()
     where = block_table.device
     slots = torch.empty(max_new_tokens, dtype=torch.int64, device=where)
@@ -220,6 +221,13 @@ def _rows(t):
     return t, st, sh
 
 
+def _distinct_rows(t, st, sh):
+    """Whether the (token, head) rows of an output do not overlap."""
+    total, heads, headdim = t.shape
+    return (total <= 1 or st >= headdim) and (heads <= 1 or sh >= headdim) and (
+        total <= 1 or heads <= 1 or st >= (heads - 1) * sh + headdim or sh >= (total - 1) * st + headdim)
+
+
 @functools.lru_cache(maxsize=256)
 def _workspace_bytes(nheads, kv_heads, max_seqlen_q, headdim):
     return _lib.load().apex_attn_fwd_paged_workspace_bytes(nheads, kv_heads, max_seqlen_q, headdim)
@@ -279,9 +287,13 @@ def custom_attention_paged_forward(q, k_cache, v_cache, k_scale, v_scale, block_
     query tokens' own among them: append first. Causal (default): query token i of n sees the
     positions up to ``seq_len - n + i``, from ``window_left`` before it on if a window is given;
     otherwise all. Returns o like q (rows outside every request are zeros) and, with
-    ``return_lse``, the fp32 natural logsumexp ``[H, total_q]``. A row that sees nothing gives 0
-    and -inf. ``out``: a tensor like q to write o into; its rows outside every request keep what
-    they hold.
+    ``return_lse``, the fp32 natural logsumexp ``[H, total_q]`` (0 outside every request). A row that
+    sees nothing gives 0 and -inf. ``out``: a tensor like q to write o into, whose rows do not
+    overlap; those outside every request keep what they hold.
+
+    Scales are not negative; V scales below 2^-100 count as 2^-100. A code or scale of NaN, or an
+    infinite or NaN value of q, makes the rows that see it NaN and no others. Table entries
+    outside the cache read as blocks of zeros.
 
     Head dims 64, 128, 256 (others: KeyError). Asynchronous on the current CUDA stream."""
     calls = _load_calls() if _calls is None else _calls
@@ -315,6 +327,7 @@ def custom_attention_paged_forward(q, k_cache, v_cache, k_scale, v_scale, block_
         cu_at = _int32(cu_seqlens_q, "cu_seqlens_q", batch + 1, device)
         if max_seqlen_q is None or max_seqlen_q < 1:
             raise ValueError("cu_seqlens_q needs a positive max_seqlen_q")
+        max_seqlen_q = min(max_seqlen_q, max(total, 1))
     elif total % batch != 0 or (max_seqlen_q is not None and max_seqlen_q * batch != total):
         raise ValueError(f"without cu_seqlens_q, q's {total} rows must be max_seqlen_q for each of {batch} requests")
     else:
@@ -327,9 +340,14 @@ def custom_attention_paged_forward(q, k_cache, v_cache, k_scale, v_scale, block_
         o_st, o_sh = nheads * headdim, headdim
     else:
         o, o_st, o_sh = _rows(out)
-        if o is not out or o.shape != shape or o.dtype is not q.dtype or o.get_device() != device:
-            raise ValueError("out must be like q, with unit stride along D and other strides multiples of 8")
-    lse = torch.empty(nheads, total, dtype=torch.float32, device=where) if return_lse else None
+        if o is not out or o.shape != shape or o.dtype is not q.dtype or o.get_device() != device \
+                or not _distinct_rows(o, o_st, o_sh):
+            raise ValueError("out must be like q, with unit stride along D, other strides multiples of 8, and rows "
+                             "that do not overlap")
+    lse = None
+    if return_lse:  # the kernel clears the rows outside every request unless `out` keeps its own
+        new = torch.empty if out is None or cu_seqlens_q is None else torch.zeros
+        lse = new(nheads, total, dtype=torch.float32, device=where)
     if total == 0:
         return (o, lse) if return_lse else o
     q, q_st, q_sh = _rows(q)
@@ -340,7 +358,7 @@ def custom_attention_paged_forward(q, k_cache, v_cache, k_scale, v_scale, block_
     args = _lib.PAGED_ARGS.pack(
         q.data_ptr(), *at, block_table.data_ptr(), lens_at, cu_at, o.data_ptr(), 0 if lse is None else lse.data_ptr(),
         table_stride, q_st, q_sh, o_st, o_sh, *cache_strides, batch, nheads, kv_heads, total, max_seqlen_q, headdim,
-        dtype, blocks, block_size, width, 1 if causal else 0, -1 if window_left is None else window_left,
+        dtype, blocks, block_size, width, 1 if causal else 0, -1 if window_left is None else min(window_left, _INT_MAX),
         1 if out is None else 0, sm_scale, device + 1)
     rc = _lib.load().apex_attn_fwd_paged(args, workspace.data_ptr(), ws_bytes, _raw_stream(device))
     if rc:

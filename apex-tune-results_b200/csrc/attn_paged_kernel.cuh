@@ -19,13 +19,16 @@
 //     three terms of e4m3, 131k flat weights still made it 1.8 times as far.
 // fp32 accumulation of e4m3 products on this card is exact to 2^-23 of the magnitudes.
 //
-// Tokens, not query rows, are the M side: S^T = K Q^T and O^T = V^T P, M = 128 tokens resp. 128
-// columns of the head dim, N = 16 .. 128 query rows. A decode step has 1 to 16 query rows per
-// K/V head; as the M side they would leave most of a 128-row tile empty. Thread t owns token t of a
-// tile: its scales are per-thread scalars and its row of P is 16 contiguous bytes per 16 query
-// rows. The price is that a row's maximum runs across threads; so the running maximum is only
-// moved when some p' would pass 2^8.75 (one vote per tile), which is rare after a row's
-// first tile.
+// Up to 32 query rows per K/V head, tokens are the M side ("token-major"): S^T = K Q^T and O^T = V^T P,
+// M = 128 tokens resp. 128 columns of the head dim, N = 16 or 32 query rows. A decode step has 1 to
+// 16 query rows per K/V head; as the M side they would leave most of a 128-row tile empty. Thread t
+// owns token t of a tile: its scales are per-thread scalars and its row of P is 16 contiguous bytes
+// per 16 query rows. The price is that a row's maximum runs across threads; so the running
+// maximum is only moved when some p' would pass 2^8.75 (one vote per tile), which is rare after
+// a row's first tile.
+// More rows, in tiles of 64 or 128, are the M side themselves ("query-major"): S = Q K^T, O = P V, a
+// thread owns part of a row, and a maximum takes one exchange between warps. (Measured: two
+// 32-row token-major tiles for 33 to 96 rows are 10 to 60 % slower than one of 64 or 128.)
 //
 // m_i tracks the maximum of x_ij + log2 b_j, kept 2^6 below p's top so that small weights stay
 // above e4m3's floor: the largest weight of a row is held at 2^6 .. 2^8.75 (e4m3's largest is 448).
@@ -63,7 +66,7 @@ struct PagedParams {
   const int* block_table;  // [batch, table_width], row stride table_stride
   const int* seq_lens;     // [batch] tokens in the cache
   const int* cu_seqlens_q; // [batch + 1]; null: total_q / batch query tokens each
-  float* part_o;    // [2 * CTAs][NQ][D], see PagedShare
+  float* part_o;    // [2 * CTAs][NQ][D]: of CTA c's entries in `share`
   float* part_lse;  // [2 * CTAs][NQ]
   int* share;       // [2 * CTAs][kShareInts]
   int* status;
@@ -209,7 +212,7 @@ __device__ __forceinline__ int paged_qtiles(const PagedParams& p, const PagedReq
 // A CTA that begins an item spends about as long on it as on this many tiles: units of an item
 // are these and then its tiles, at least one (an item that sees nothing still has rows to
 // write). Without them the CTAs that got short requests finished last: 48 requests of 129 to
-// 8191 tokens took 115 us instead of TODO us.
+// 8191 tokens take 92 us instead of 80, and three of 1024 new tokens each 600 instead of 553.
 template <int NQ>
 constexpr int kPagedItemUnits = NQ <= 32 ? 4 : 8;
 
@@ -688,7 +691,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     if (lane == 0) ptx::mbar_arrive(bar(C::kSegEmpty + at));
     return ok && seg.n >= 0;  // after a failed wait the ring may hold anything
   };
-  PagedSegment seg;
+  PagedSegment seg{};
 
   if (warp < C::kSoftWarps) {
     // =========================================================== softmax ===
@@ -825,85 +828,85 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           };
           if (idle) wait_p_buffer();  // (clear_unseen counts on it)
           if (!idle) {
-          float most = -INFINITY;
+            float most = -INFINITY;
 #pragma unroll 1
-          for (int c0 = 0; c0 < kTok; c0 += NC) {
-            load(tok0 + c0);
-            scaled(tok0 + c0);
-#pragma unroll
-            for (int c = 0; c < NC / 2; ++c) most = ptx::fmax3(most, d[c].x, d[c].y);
-          }
-          const bool left = pos0 < seg.lo_all;
-          const bool move = force || left ? true : ptx::named_bar_or(vote, 32 * kWGs, most > kPagedMost);
-          force = left;
-          if (move) {
-            float* const tops = exchange + ((g / C::kPairs) & 1) * C::kWG * 128;
-            tops[wg * 128 + t] = most;
-            ptx::named_bar_sync(vote, 32 * kWGs);
-            float top = most;
-#pragma unroll
-            for (int k = 0; k < kWGs; ++k) top = fmaxf(top, tops[(pair * kWGs + k) * 128 + t]);
-            // By how much the maximum moves: up only, but freely the first time.
-            const bool some = top != -INFINITY;
-            const float by = some ? (set ? fmaxf(top - kPagedTop, 0.f) : top - kPagedTop) : 0.f;
-            const float f = set ? ptx::ex2(-by) : 0.f;
-            set = set || some;
-            nm -= by;
-            l *= f;
-            if (C::kPairs == 1) {  // d is still here; else it is loaded again below
-              const float2 by2 = make_float2(-by, -by);
-#pragma unroll
-              for (int c = 0; c < NC / 2; ++c) d[c] = __fadd2_rn(d[c], by2);
-            }
-            if (j >= C::kPairs) {
-              wait(C::kPvDone + ((g - C::kPairs) & 1), (uint32_t)((g - C::kPairs) >> 1));
-              ptx::tc_fence_after();
-#pragma unroll 1
-              for (int c = 0; c < D / kWGs; c += 16) {
-                const uint32_t at = tmem + lane_off + (uint32_t)(2 * C::kSCols + pair * D + wg % kWGs * (D / kWGs) + c);
-                uint32_t v[16];
-                ptx::tmem_ld16(at, v);
-                ptx::tmem_wait_ld();
-                ptx::reg_fence16(v);
-#pragma unroll
-                for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
-                ptx::tmem_st16(at, v);
-              }
-              ptx::tmem_wait_st();
-            }
-          }
-          wait_p_buffer();
-          const uint32_t dst = sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kTerms * C::kPTerm + t * 128;
-#pragma unroll 1
-          for (int c0 = 0; c0 < kTok; c0 += NC) {
-            if (C::kPairs == 2) {
+            for (int c0 = 0; c0 < kTok; c0 += NC) {
               load(tok0 + c0);
               scaled(tok0 + c0);
+#pragma unroll
+              for (int c = 0; c < NC / 2; ++c) most = ptx::fmax3(most, d[c].x, d[c].y);
             }
+            const bool left = pos0 < seg.lo_all;
+            const bool move = force || left ? true : ptx::named_bar_or(vote, 32 * kWGs, most > kPagedMost);
+            force = left;
+            if (move) {
+              float* const tops = exchange + ((g / C::kPairs) & 1) * C::kWG * 128;
+              tops[wg * 128 + t] = most;
+              ptx::named_bar_sync(vote, 32 * kWGs);
+              float top = most;
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const int c16 = tok0 + c0 + 16 * half;
-              uint32_t term[C::kTerms][4];
-              float2 sum = make_float2(0.f, 0.f);
+              for (int k = 0; k < kWGs; ++k) top = fmaxf(top, tops[(pair * kWGs + k) * 128 + t]);
+              // By how much the maximum moves: up only, but freely the first time.
+              const bool some = top != -INFINITY;
+              const float by = some ? (set ? fmaxf(top - kPagedTop, 0.f) : top - kPagedTop) : 0.f;
+              const float f = set ? ptx::ex2(-by) : 0.f;
+              set = set || some;
+              nm -= by;
+              l *= f;
+              if (C::kPairs == 1) {  // d is still here; else it is loaded again below
+                const float2 by2 = make_float2(-by, -by);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const int x = 8 * half + 2 * k;
-                const float2 e0 = make_float2(ptx::ex2(d[x].x), ptx::ex2(d[x].y));
-                const float2 e1 = make_float2(ptx::ex2(d[x + 1].x), ptx::ex2(d[x + 1].y));
-                sum = __fadd2_rn(sum, __fadd2_rn(e0, e1));
-                __half2 a = __floats2half2_rn(e0.x, e0.y), b = __floats2half2_rn(e1.x, e1.y);
-                uint32_t four[C::kTerms];
-                split_terms(a, b, four);
-#pragma unroll
-                for (int i = 0; i < C::kTerms; ++i) term[i][k] = four[i];
+                for (int c = 0; c < NC / 2; ++c) d[c] = __fadd2_rn(d[c], by2);
               }
-              l = fmaf(sum.x + sum.y, sc[c16 >> p.block_shift].z, l);
-              const uint32_t unit = (uint32_t)((c16 >> 4) ^ (t & 7)) << 4;
+              if (j >= C::kPairs) {
+                wait(C::kPvDone + ((g - C::kPairs) & 1), (uint32_t)((g - C::kPairs) >> 1));
+                ptx::tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < D / kWGs; c += 16) {
+                  const uint32_t at = tmem + lane_off + (uint32_t)(2 * C::kSCols + pair * D + wg % kWGs * (D / kWGs) + c);
+                  uint32_t v[16];
+                  ptx::tmem_ld16(at, v);
+                  ptx::tmem_wait_ld();
+                  ptx::reg_fence16(v);
 #pragma unroll
-              for (int i = 0; i < C::kTerms; ++i)
-                ptx::st_shared_v4(dst + unit + i * C::kPTerm, term[i][0], term[i][1], term[i][2], term[i][3]);
+                  for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
+                  ptx::tmem_st16(at, v);
+                }
+                ptx::tmem_wait_st();
+              }
             }
-          }
+            wait_p_buffer();
+            const uint32_t dst = sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kTerms * C::kPTerm + t * 128;
+#pragma unroll 1
+            for (int c0 = 0; c0 < kTok; c0 += NC) {
+              if (C::kPairs == 2) {
+                load(tok0 + c0);
+                scaled(tok0 + c0);
+              }
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                const int c16 = tok0 + c0 + 16 * half;
+                uint32_t term[C::kTerms][4];
+                float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const int x = 8 * half + 2 * k;
+                  const float2 e0 = make_float2(ptx::ex2(d[x].x), ptx::ex2(d[x].y));
+                  const float2 e1 = make_float2(ptx::ex2(d[x + 1].x), ptx::ex2(d[x + 1].y));
+                  sum = __fadd2_rn(sum, __fadd2_rn(e0, e1));
+                  __half2 a = __floats2half2_rn(e0.x, e0.y), b = __floats2half2_rn(e1.x, e1.y);
+                  uint32_t four[C::kTerms];
+                  split_terms(a, b, four);
+#pragma unroll
+                  for (int i = 0; i < C::kTerms; ++i) term[i][k] = four[i];
+                }
+                l = fmaf(sum.x + sum.y, sc[c16 >> p.block_shift].z, l);
+                const uint32_t unit = (uint32_t)((c16 >> 4) ^ (t & 7)) << 4;
+#pragma unroll
+                for (int i = 0; i < C::kTerms; ++i)
+                  ptx::st_shared_v4(dst + unit + i * C::kPTerm, term[i][0], term[i][1], term[i][2], term[i][3]);
+              }
+            }
           }
           // S is read: the MMA warp may write the buffer again.
           ptx::tc_fence_before();
@@ -1000,202 +1003,206 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
         seg = then;
       }
     } else {
-    // The first rows are split here in any case: these warps have nothing else to do yet.
+      // The first rows are split here in any case: these warps have nothing else to do yet.
 #pragma unroll 1
-    for (int n = 0; more; ++n) {
-      const int rows = seg.rows - c_first;  // of this warpgroup; may be <= 0
-      float* const col_nm = reinterpret_cast<float*>(smem + C::kCol) + (n & 1) * 5 * NQ + c_first;  // kPagedTop - max
-      const float* const col_q = col_nm + NQ;  // q's scale
-      float* const col_f = col_nm + 2 * NQ;    // factor of a moved maximum, -1 before the first; 1 / sum at the end
-      const int* const col_hi = reinterpret_cast<const int*>(col_nm + 3 * NQ);  // tokens [lo, hi) are seen
-      const int* const col_lo = reinterpret_cast<const int*>(col_nm + 4 * NQ);
-      if (n == 0) split(seg, 0);
-      wait(C::kQFull + (n & 1), (uint32_t)(n >> 1));
-      float2 l[NC / 2];
+      for (int n = 0; more; ++n) {
+        const int rows = seg.rows - c_first;  // of this warpgroup; may be <= 0
+        float* const col_nm = reinterpret_cast<float*>(smem + C::kCol) + (n & 1) * 5 * NQ + c_first;  // kPagedTop - max
+        const float* const col_q = col_nm + NQ;  // q's scale
+        float* const col_f = col_nm + 2 * NQ;    // factor of a moved maximum, -1 before the first; 1 / sum at the end
+        const int* const col_hi = reinterpret_cast<const int*>(col_nm + 3 * NQ);  // tokens [lo, hi) are seen
+        const int* const col_lo = reinterpret_cast<const int*>(col_nm + 4 * NQ);
+        if (n == 0) split(seg, 0);
+        wait(C::kQFull + (n & 1), (uint32_t)(n >> 1));
+        float2 l[NC / 2];
 #pragma unroll
-      for (int c = 0; c < NC / 2; ++c) l[c] = make_float2(0.f, 0.f);
-      bool force = true;  // a row's maximum may not be set: first tile, or behind one left of a row's window
+        for (int c = 0; c < NC / 2; ++c) l[c] = make_float2(0.f, 0.f);
+        bool force = true;  // a row's maximum may not be set: first tile, or behind one left of a row's window
 
 #pragma unroll 1
-      for (int j = 0; j < seg.n; ++j, ++g) {
-        const int sb = g & 1;
-        const int pos0 = (seg.tile + j) * kPagedTile, pos = pos0 + t;
-        wait(C::kScFull + g % C::kScaleRing, (uint32_t)(g / C::kScaleRing));
-        const float4 sc = scales[(g % C::kScaleRing) * 8 + page];  // a * scale_log2, log2 b, 1 / b
-        wait(C::kSFull + sb, (uint32_t)(g >> 1));
-        ptx::tc_fence_after();
-        float2 d[NC / 2];
+        for (int j = 0; j < seg.n; ++j, ++g) {
+          const int sb = g & 1;
+          const int pos0 = (seg.tile + j) * kPagedTile, pos = pos0 + t;
+          wait(C::kScFull + g % C::kScaleRing, (uint32_t)(g / C::kScaleRing));
+          const float4 sc = scales[(g % C::kScaleRing) * 8 + page];  // a * scale_log2, log2 b, 1 / b
+          wait(C::kSFull + sb, (uint32_t)(g >> 1));
+          ptx::tc_fence_after();
+          float2 d[NC / 2];
 #pragma unroll
-        for (int c = 0; c < NC; c += 16)
-          ptx::tmem_ld16(tmem + lane_off + (uint32_t)(sb * NQ + c_first + c), reinterpret_cast<uint32_t*>(d) + c);
-        ptx::tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < NC; c += 16) ptx::reg_fence16(reinterpret_cast<uint32_t*>(d) + c);
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          ptx::mbar_arrive(bar(C::kScEmpty + g % C::kScaleRing));
-          ptx::mbar_arrive(bar(C::kSFree + sb));
-        }
-        // d = x + log2 b - m; -inf where the row does not see the token.
-        const float2 a2 = make_float2(sc.x, sc.x), b2 = make_float2(sc.y, sc.y), i2 = make_float2(sc.z, sc.z);
-        float most = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < NC / 2; c += 2) {
-          const float4 q4 = *reinterpret_cast<const float4*>(col_q + 2 * c);
-          const float4 n4 = *reinterpret_cast<const float4*>(col_nm + 2 * c);
-          d[c] = __ffma2_rn(d[c], __fmul2_rn(a2, make_float2(q4.x, q4.y)), __fadd2_rn(b2, make_float2(n4.x, n4.y)));
-          d[c + 1] =
-              __ffma2_rn(d[c + 1], __fmul2_rn(a2, make_float2(q4.z, q4.w)), __fadd2_rn(b2, make_float2(n4.z, n4.w)));
-          most = ptx::fmax3(most, d[c].x, d[c].y);
-          most = ptx::fmax3(most, d[c + 1].x, d[c + 1].y);
-        }
-        const bool masked = pos0 < seg.lo_all || pos0 + kPagedTile > seg.hi_all;
-        if (masked) {
-#pragma unroll
-          for (int c = 0; c < NC; ++c)
-            if (pos < col_lo[c] || pos >= col_hi[c]) (c & 1 ? d[c / 2].y : d[c / 2].x) = -INFINITY;
-        }
-        const bool left = pos0 < seg.lo_all;
-        const bool move = force || left ? true : ptx::named_bar_or(1 + wg, 128, most > kPagedMost);
-        force = left;
-        if (move) {
-          // Move the maxima: over the warp, over the warps; then rescale the sums and O.
-#pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            const float top = ptx::warp_max(c & 1 ? d[c / 2].y : d[c / 2].x);
-            if (lane == c) red[(warp & 3) * NC + c] = top;
-          }
-          ptx::named_bar_sync(1 + wg, 128);
-          if (t < NC) {
-            const float top = fmaxf(fmaxf(red[t], red[NC + t]), fmaxf(red[2 * NC + t], red[3 * NC + t]));
-            // By how much the maximum moves: up only, but freely the first time.
-            const bool set = col_f[t] >= 0.f;
-            const float by = top == -INFINITY ? 0.f : (set ? fmaxf(top - kPagedTop, 0.f) : top - kPagedTop);
-            if (set || top != -INFINITY) col_f[t] = set ? ptx::ex2(-by) : 0.f;
-            col_nm[t] -= by;
-            red[t] = by;
-          }
-          ptx::named_bar_sync(1 + wg, 128);
-#pragma unroll
-          for (int c = 0; c < NC / 2; ++c) {
-            const float2 by = *reinterpret_cast<const float2*>(red + 2 * c);
-            d[c] = make_float2(d[c].x - by.x, d[c].y - by.y);
-            l[c] = __fmul2_rn(l[c], *reinterpret_cast<const float2*>(col_f + 2 * c));
-          }
-          if (j > 0) {
-            wait(C::kPvDone + (sb ^ 1), (uint32_t)((g - 1) >> 1));
-            ptx::tc_fence_after();
-#pragma unroll 1
-            for (int c = 0; c < C::kChunks * NC; c += 16) {
-              const int cc = c % NC;
-              const uint32_t at = tmem + lane_off + (uint32_t)(2 * NQ + (c / NC) * NQ + c_first + cc);
-              uint32_t v[16];
-              ptx::tmem_ld16(at, v);
-              ptx::tmem_wait_ld();
-              ptx::reg_fence16(v);
-#pragma unroll
-              for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * col_f[cc + k]);
-              ptx::tmem_st16(at, v);
-            }
-            ptx::tmem_wait_st();
-          }
-        }
-        // P buffer sb was read by P V of tile g - 2.
-        if (g >= 2) wait(C::kPvDone + sb, (uint32_t)((g - 2) >> 1));
-        const uint32_t dst = sbase + C::kP + sb * C::kTerms * C::kPTerm + t * 16 + c_first * 128;
-#pragma unroll
-        for (int c = 0; c < NC; c += 16) {
-          uint32_t term[C::kTerms][4];
-#pragma unroll
-          for (int k = 0; k < 16; k += 4) {
-            const int x = (c + k) / 2;
-            const float2 e0 = make_float2(ptx::ex2(d[x].x), ptx::ex2(d[x].y));
-            const float2 e1 = make_float2(ptx::ex2(d[x + 1].x), ptx::ex2(d[x + 1].y));
-            l[x] = __ffma2_rn(e0, i2, l[x]);
-            l[x + 1] = __ffma2_rn(e1, i2, l[x + 1]);
-            __half2 a = __floats2half2_rn(e0.x, e0.y), b = __floats2half2_rn(e1.x, e1.y);
-            uint32_t four[C::kTerms];
-            split_terms(a, b, four);
-#pragma unroll
-            for (int j2 = 0; j2 < C::kTerms; ++j2) term[j2][k >> 2] = four[j2];
-          }
-#pragma unroll
-          for (int j2 = 0; j2 < C::kTerms; ++j2)
-            ptx::st_shared_v4(dst + c * 128 + j2 * C::kPTerm, term[j2][0], term[j2][1], term[j2][2], term[j2][3]);
-        }
-        clear_unseen(j, 1 + wg, [&](int x) {  // columns 16-byte chunk by chunk, tokens within
-          if (x != t) return;
-          for (int c = 0; c < NC; ++c)
-            if (pos >= col_lo[c] && pos < col_hi[c]) ptx::st_shared_u8(dst + (c >> 4) * 2048 + (c & 15), 0x7fu);
-        });
-        ptx::fence_proxy_async_smem();
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(bar(C::kPFull + sb));
-      }
-      fills += 2 * seg.n;
-
-      // ---- the segment's result ----
-      {
-        float sums[NC];
-#pragma unroll
-        for (int c = 0; c < NC / 2; ++c) sums[2 * c] = l[c].x, sums[2 * c + 1] = l[c].y;
-        const int c = warp_column_sums<NC>(sums);
-        if (NC == 32 || (lane & 1) == 0) red[(warp & 3) * NC + c] = sums[0];
-      }
-      ptx::named_bar_sync(1 + wg, 128);
-      if (t < NC && t < rows) {
-        const float sum = red[t] + red[NC + t] + red[2 * NC + t] + red[3 * NC + t];
-        const float lse2 = sum == 0.f ? -INFINITY : __log2f(sum) - col_nm[t];
-        col_f[t] = sum == 0.f ? 0.f : 1.f / sum;
-        if (seg.slot >= 0) {
-          p.part_lse[(long long)seg.slot * NQ + c_first + t] = lse2;
-        } else if (p.lse != nullptr) {
-          int token, head;
-          paged_row(p, seg.token0, seg.head0, c_first + t, token, head);
-          p.lse[(long long)(seg.h * p.group + head) * p.total_q + seg.q0 + token] = lse2 * 0.69314718055994531f;
-        }
-      }
-      if (seg.n > 0) wait(C::kPvDone + ((g - 1) & 1), (uint32_t)((g - 1) >> 1));
-      ptx::tc_fence_after();
-      ptx::named_bar_sync(1 + wg, 128);
-#pragma unroll 1
-      for (int ch = 0; ch < C::kChunks; ++ch) {
-        const int d = ch * 128 + t;
-#pragma unroll 1
-        for (int c = 0; c < NC; c += 16) {
-          if (c >= rows) break;
-          uint32_t v[16];
-          ptx::tmem_ld16(tmem + lane_off + (uint32_t)(2 * NQ + ch * NQ + c_first + c), v);
+          for (int c = 0; c < NC; c += 16)
+            ptx::tmem_ld16(tmem + lane_off + (uint32_t)(sb * NQ + c_first + c), reinterpret_cast<uint32_t*>(d) + c);
           ptx::tmem_wait_ld();
-          ptx::reg_fence16(v);
-          int token, head;
-          paged_row(p, seg.token0, seg.head0, c_first + c, token, head);
-          T* o = static_cast<T*>(p.o) + (seg.q0 + token) * p.o_st + (seg.h * p.group + head) * p.o_sh + d;
-          float* part = p.part_o + ((long long)seg.slot * NQ + c_first + c) * D + d;
-          const long long wrap = p.o_st - (p.group - 1) * p.o_sh;  // from a token's last head to the next's first
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            if (c + k >= rows) break;
-            const float inv = col_f[c + k];
-            // A row that saw nothing has no O (its tiles may not have run): 0, whatever TMEM holds.
-            const float val = inv == 0.f ? 0.f : __uint_as_float(v[k]) * inv;
-            if (d < D) {
-              if (seg.slot >= 0) part[k * D] = val;
-              else *o = (T)val;
+          for (int c = 0; c < NC; c += 16) ptx::reg_fence16(reinterpret_cast<uint32_t*>(d) + c);
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            ptx::mbar_arrive(bar(C::kScEmpty + g % C::kScaleRing));
+            ptx::mbar_arrive(bar(C::kSFree + sb));
+          }
+          // d = x + log2 b - m; -inf where the row does not see the token.
+          const float2 a2 = make_float2(sc.x, sc.x), b2 = make_float2(sc.y, sc.y), i2 = make_float2(sc.z, sc.z);
+          float most = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < NC / 2; c += 2) {
+            const float4 q4 = *reinterpret_cast<const float4*>(col_q + 2 * c);
+            const float4 n4 = *reinterpret_cast<const float4*>(col_nm + 2 * c);
+            d[c] = __ffma2_rn(d[c], __fmul2_rn(a2, make_float2(q4.x, q4.y)), __fadd2_rn(b2, make_float2(n4.x, n4.y)));
+            d[c + 1] =
+                __ffma2_rn(d[c + 1], __fmul2_rn(a2, make_float2(q4.z, q4.w)), __fadd2_rn(b2, make_float2(n4.z, n4.w)));
+            most = ptx::fmax3(most, d[c].x, d[c].y);
+            most = ptx::fmax3(most, d[c + 1].x, d[c + 1].y);
+          }
+          const bool masked = pos0 < seg.lo_all || pos0 + kPagedTile > seg.hi_all;
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+              if (pos < col_lo[c] || pos >= col_hi[c]) (c & 1 ? d[c / 2].y : d[c / 2].x) = -INFINITY;
+            // What nobody sees has no say in where the maxima move: not one bit of the result is its.
+            most = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < NC / 2; ++c) most = ptx::fmax3(most, d[c].x, d[c].y);
+          }
+          const bool left = pos0 < seg.lo_all;
+          const bool move = force || left ? true : ptx::named_bar_or(1 + wg, 128, most > kPagedMost);
+          force = left;
+          if (move) {
+            // Move the maxima: over the warp, over the warps; then rescale the sums and O.
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+              const float top = ptx::warp_max(c & 1 ? d[c / 2].y : d[c / 2].x);
+              if (lane == c) red[(warp & 3) * NC + c] = top;
             }
-            const bool last = ++head == p.group;
-            o += last ? wrap : p.o_sh;
-            head = last ? 0 : head;
+            ptx::named_bar_sync(1 + wg, 128);
+            if (t < NC) {
+              const float top = fmaxf(fmaxf(red[t], red[NC + t]), fmaxf(red[2 * NC + t], red[3 * NC + t]));
+              // By how much the maximum moves: up only, but freely the first time.
+              const bool set = col_f[t] >= 0.f;
+              const float by = top == -INFINITY ? 0.f : (set ? fmaxf(top - kPagedTop, 0.f) : top - kPagedTop);
+              if (set || top != -INFINITY) col_f[t] = set ? ptx::ex2(-by) : 0.f;
+              col_nm[t] -= by;
+              red[t] = by;
+            }
+            ptx::named_bar_sync(1 + wg, 128);
+#pragma unroll
+            for (int c = 0; c < NC / 2; ++c) {
+              const float2 by = *reinterpret_cast<const float2*>(red + 2 * c);
+              d[c] = make_float2(d[c].x - by.x, d[c].y - by.y);
+              l[c] = __fmul2_rn(l[c], *reinterpret_cast<const float2*>(col_f + 2 * c));
+            }
+            if (j > 0) {
+              wait(C::kPvDone + (sb ^ 1), (uint32_t)((g - 1) >> 1));
+              ptx::tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < C::kChunks * NC; c += 16) {
+                const int cc = c % NC;
+                const uint32_t at = tmem + lane_off + (uint32_t)(2 * NQ + (c / NC) * NQ + c_first + cc);
+                uint32_t v[16];
+                ptx::tmem_ld16(at, v);
+                ptx::tmem_wait_ld();
+                ptx::reg_fence16(v);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * col_f[cc + k]);
+                ptx::tmem_st16(at, v);
+              }
+              ptx::tmem_wait_st();
+            }
+          }
+          // P buffer sb was read by P V of tile g - 2.
+          if (g >= 2) wait(C::kPvDone + sb, (uint32_t)((g - 2) >> 1));
+          const uint32_t dst = sbase + C::kP + sb * C::kTerms * C::kPTerm + t * 16 + c_first * 128;
+#pragma unroll
+          for (int c = 0; c < NC; c += 16) {
+            uint32_t term[C::kTerms][4];
+#pragma unroll
+            for (int k = 0; k < 16; k += 4) {
+              const int x = (c + k) / 2;
+              const float2 e0 = make_float2(ptx::ex2(d[x].x), ptx::ex2(d[x].y));
+              const float2 e1 = make_float2(ptx::ex2(d[x + 1].x), ptx::ex2(d[x + 1].y));
+              l[x] = __ffma2_rn(e0, i2, l[x]);
+              l[x + 1] = __ffma2_rn(e1, i2, l[x + 1]);
+              __half2 a = __floats2half2_rn(e0.x, e0.y), b = __floats2half2_rn(e1.x, e1.y);
+              uint32_t four[C::kTerms];
+              split_terms(a, b, four);
+#pragma unroll
+              for (int j2 = 0; j2 < C::kTerms; ++j2) term[j2][k >> 2] = four[j2];
+            }
+#pragma unroll
+            for (int j2 = 0; j2 < C::kTerms; ++j2)
+              ptx::st_shared_v4(dst + c * 128 + j2 * C::kPTerm, term[j2][0], term[j2][1], term[j2][2], term[j2][3]);
+          }
+          clear_unseen(j, 1 + wg, [&](int x) {  // columns 16-byte chunk by chunk, tokens within
+            if (x != t) return;
+            for (int c = 0; c < NC; ++c)
+              if (pos >= col_lo[c] && pos < col_hi[c]) ptx::st_shared_u8(dst + (c >> 4) * 2048 + (c & 15), 0x7fu);
+          });
+          ptx::fence_proxy_async_smem();
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(bar(C::kPFull + sb));
+        }
+        fills += 2 * seg.n;
+
+        // ---- the segment's result ----
+        {
+          float sums[NC];
+#pragma unroll
+          for (int c = 0; c < NC / 2; ++c) sums[2 * c] = l[c].x, sums[2 * c + 1] = l[c].y;
+          const int c = warp_column_sums<NC>(sums);
+          if (NC == 32 || (lane & 1) == 0) red[(warp & 3) * NC + c] = sums[0];
+        }
+        ptx::named_bar_sync(1 + wg, 128);
+        if (t < NC && t < rows) {
+          const float sum = red[t] + red[NC + t] + red[2 * NC + t] + red[3 * NC + t];
+          const float lse2 = sum == 0.f ? -INFINITY : __log2f(sum) - col_nm[t];
+          col_f[t] = sum == 0.f ? 0.f : 1.f / sum;
+          if (seg.slot >= 0) {
+            p.part_lse[(long long)seg.slot * NQ + c_first + t] = lse2;
+          } else if (p.lse != nullptr) {
+            int token, head;
+            paged_row(p, seg.token0, seg.head0, c_first + t, token, head);
+            p.lse[(long long)(seg.h * p.group + head) * p.total_q + seg.q0 + token] = lse2 * 0.69314718055994531f;
           }
         }
+        if (seg.n > 0) wait(C::kPvDone + ((g - 1) & 1), (uint32_t)((g - 1) >> 1));
+        ptx::tc_fence_after();
+        ptx::named_bar_sync(1 + wg, 128);
+#pragma unroll 1
+        for (int ch = 0; ch < C::kChunks; ++ch) {
+          const int d = ch * 128 + t;
+#pragma unroll 1
+          for (int c = 0; c < NC; c += 16) {
+            if (c >= rows) break;
+            uint32_t v[16];
+            ptx::tmem_ld16(tmem + lane_off + (uint32_t)(2 * NQ + ch * NQ + c_first + c), v);
+            ptx::tmem_wait_ld();
+            ptx::reg_fence16(v);
+            int token, head;
+            paged_row(p, seg.token0, seg.head0, c_first + c, token, head);
+            T* o = static_cast<T*>(p.o) + (seg.q0 + token) * p.o_st + (seg.h * p.group + head) * p.o_sh + d;
+            float* part = p.part_o + ((long long)seg.slot * NQ + c_first + c) * D + d;
+            const long long wrap = p.o_st - (p.group - 1) * p.o_sh;  // from a token's last head to the next's first
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              if (c + k >= rows) break;
+              const float inv = col_f[c + k];
+              // A row that saw nothing has no O (its tiles may not have run): 0, whatever TMEM holds.
+              const float val = inv == 0.f ? 0.f : __uint_as_float(v[k]) * inv;
+              if (d < D) {
+                if (seg.slot >= 0) part[k * D] = val;
+                else *o = (T)val;
+              }
+              const bool last = ++head == p.group;
+              o += last ? wrap : p.o_sh;
+              head = last ? 0 : head;
+            }
+          }
+        }
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar(C::kColEmpty + (n & 1)));
+        more = next_for_all(seg);
       }
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(bar(C::kColEmpty + (n & 1)));
-      more = next_for_all(seg);
-    }
     }
   } else if (warp == kWarpProd) {
     // ========================================================== producer ===
@@ -1444,8 +1451,10 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           const int id = __ldg(p.block_table + (long long)seg.b * p.table_stride + (at >> p.block_shift));
           if (id >= 0 && id < p.num_blocks) {
             const float a = __ldg(p.k_scale + (long long)id * p.heads_kv + seg.h);
-            const float b = fmaxf(__ldg(p.v_scale + (long long)id * p.heads_kv + seg.h), kPagedLeastScale);
-            sc = make_float4(a * p.scale_log2, __log2f(b), 1.f / b, 0.f);
+            const float given = __ldg(p.v_scale + (long long)id * p.heads_kv + seg.h);
+            const float b = fmaxf(given, kPagedLeastScale);
+            // A scale of NaN goes on in the exponent, which is masked; 1 / b is not, and stays a number.
+            sc = make_float4(a * p.scale_log2, given != given ? given : __log2f(b), 1.f / b, 0.f);
           }
         }
         const int take = min(4, seg.n - j0);

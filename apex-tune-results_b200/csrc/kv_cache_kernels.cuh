@@ -275,7 +275,7 @@ struct Elem<__half> {
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * kAppendWarps, 8) kv_append_kernel(const AppendParams p) {
   constexpr int kPerRow = D / 8;   // 8 values (16 bytes of input) per lane and step
-    constexpr int kAhead = 8;        // steps in registers at once
+  constexpr int kAhead = 8;        // steps in registers at once
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int unit = blockIdx.y * kAppendWarps + warp;
   if (unit >= 2 * p.heads) return;

@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <exception>
 
@@ -47,6 +48,13 @@ uintptr_t address(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.da
 bool rows_ready(const at::Tensor& t) {
   return t.dim() == 3 && t.stride(2) == 1 && ((t.stride(0) | t.stride(1)) & 7) == 0 && t.stride(1) >= t.size(2) &&
          (address(t) & 15) == 0;
+}
+
+// Whether the (token, head) rows of an output do not overlap.
+bool rows_distinct(const at::Tensor& t) {
+  const int64_t n = t.size(0), h = t.size(1), d = t.size(2), st = t.stride(0), sh = t.stride(1);
+  return (n <= 1 || st >= d) && (h <= 1 || sh >= d) &&
+         (n <= 1 || h <= 1 || st >= (h - 1) * sh + d || sh >= (n - 1) * st + d);
 }
 
 int dtype_of(const at::Tensor& t) {
@@ -161,6 +169,7 @@ PyObject* attend(PyObject*, PyObject* const* o, Py_ssize_t n) {
       const at::Tensor* cu = cuda_tensor(o[7], device);
       if (!vector_of(cu, at::kInt, (int64_t)a.batch + 1) || !whole(o[8], max_q) || max_q < 1) return nullptr;
       a.cu_seqlens_q = static_cast<const int*>(cu->data_ptr());
+      max_q = (int)std::min<int64_t>(max_q, total);
     }
     if ((o[9] != Py_True && o[9] != Py_False) || (o[11] != Py_True && o[11] != Py_False)) return nullptr;
     a.causal = o[9] == Py_True;
@@ -177,12 +186,15 @@ PyObject* attend(PyObject*, PyObject* const* o, Py_ssize_t n) {
       a.zero_rest = 1;
     } else {
       const at::Tensor* given = cuda_tensor(o[13], device);
-      if (!given || given->scalar_type() != q->scalar_type() || given->sizes() != q->sizes() || !rows_ready(*given))
+      if (!given || given->scalar_type() != q->scalar_type() || given->sizes() != q->sizes() || !rows_ready(*given) ||
+          !rows_distinct(*given))
         return nullptr;
       out = *given;
     }
     at::Tensor lse;
     if (o[11] == Py_True) {
+      // The kernel clears the rows outside every request, unless `out` keeps its own: the other way.
+      if (a.zero_rest == 0 && a.cu_seqlens_q != nullptr) return nullptr;
       lse = new_tensor({heads, total}, at::kFloat, device);
       a.lse = static_cast<float*>(lse.data_ptr());
     }

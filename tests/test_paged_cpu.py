@@ -207,3 +207,30 @@ def test_oracle_plan_and_release_return_to_the_start():
     assert slots[:16] == [8 * 16 + i for i in range(16)] and slots[20] == 6 * 16 and slots[54:] == [-1] * 6
     lens, count = ref.release(table, lens, [1, 1, 1], free, count, 16)
     assert lens == [0, 0, 0] and count == 9 and sorted(free) == list(range(9))
+
+
+@pytest.mark.parametrize("i,value", [(4, 0), (4, 1024), (7, 2032), (5, 0), (5, 1008), (8, 64)])
+def test_append_refuses_caches_that_overlap_themselves(lib, i, value):
+    """Blocks, heads or tokens that share bytes (an expanded cache) would be written twice at once."""
+    args = append_args(with_stride(i, value))
+    assert lib.apex_attn_kv_append(ctypes.byref(args), None) == LAYOUT
+
+
+@pytest.mark.parametrize("kv", [0, 1])
+def test_append_takes_caches_in_any_order_of_dimensions(lib, kv):
+    """Heads outside the blocks, tokens outside the heads, K and V in one storage: past the layout's
+    checks, where the made-up pointers are refused."""
+    for sb, sh, st in [(1024, 4096, 64), (128, 64, 512), (4096, 64, 256), (64, 16 * 256, 256)]:
+        strides = [256, 64, 256, 64, 2048, 1024, 64, 2048, 1024, 64]
+        strides[4 + 3 * kv:7 + 3 * kv] = [sb, sh, st]
+        assert lib.apex_attn_kv_append(ctypes.byref(append_args(tuple(strides))), None) == NODEV
+
+
+@pytest.mark.parametrize("tokens,heads,ok", [(256, 64, True), (64, 192, True), (0, 64, False), (128, 64, False),
+                                             (64, 128, False), (192, 64, False), (1024, 256, True)])
+def test_attention_refuses_outputs_whose_rows_overlap(lib, tokens, heads, ok):
+    """Three tokens of four heads of 64."""
+    strides = (256, 64, tokens, heads, 2048, 1024, 64, 2048, 1024, 64)
+    got = paged(lib, total_q=3, heads_q=4, heads_kv=2, head_dim=64, batch=3, max_seqlen_q=1,
+                strides=(ctypes.c_longlong * 10)(*strides))
+    assert got == (NODEV if ok else LAYOUT)

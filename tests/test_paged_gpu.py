@@ -780,3 +780,85 @@ def test_native_and_python_ways_agree():
         assert a.shape == b.shape and a.dtype == b.dtype and a.stride() == b.stride()
         assert torch.equal(a, b)
     assert native.attend(q.float(), kc, vc, ks, vs, table, plan.seq_lens, None, None, True, None, False, None, None) is None
+
+
+# ------------------------------------------------------------ calls at the edges --
+@pytest.mark.parametrize("hq,hkv,dim,q_len,window", [(4, 2, 128, 5, None), (8, 2, 64, 7, 3), (16, 2, 64, 200, 40),
+                                                    (40, 2, 128, 150, None), (4, 2, 256, 4, None)])
+@pytest.mark.parametrize("which", [0, 1])
+def test_a_scale_of_nan_reaches_only_the_rows_that_see_its_block(hq, hkv, dim, q_len, window, which):
+    lens = [q_len + 253, q_len + 1]
+    p = paged_problem(lens, hq, hkv, dim, 16, "bf16", [q_len, q_len], seed=dim + q_len)
+    want_o, want_lse, ob, lb = ref.attend(p["q"], *(c.double().nan_to_num() for c, _ in p["caches"]),
+                                          *(s.double().nan_to_num() for _, s in p["caches"]), p["table"], lens, p["cu"],
+                                          16, True, window)
+    blocks = [(lens[0] - q_len // 2 - 1) // 16, (lens[1] - 1) // 16]
+    for b, j in enumerate(blocks):
+        p["gpu"][which][1][p["table"][b][j]] = float("nan")
+    o, lse = call(p, window_left=window, return_lse=True)
+    o, lse = o.double().cpu(), lse.double().cpu()
+    some = [0, 0]
+    for b, j in enumerate(blocks):
+        for i in range(q_len):
+            r, place = p["cu"][b] + i, lens[b] - q_len + i
+            sees = 16 * j <= place and (window is None or 16 * j + 15 >= place - window)
+            some[sees] += 1
+            if sees:
+                assert torch.isnan(o[r]).all() and torch.isnan(lse[:, r]).all()
+            else:
+                eps = torch.finfo(torch.bfloat16).eps / 2
+                assert ((o[r] - want_o[r]).abs() <= ob[r] + eps * (want_o[r].abs() + ob[r])).all()
+                assert ((lse[:, r] - want_lse[:, r]).abs() <= lb[:, r]).all()
+    assert some[1]
+
+
+@pytest.mark.parametrize("hq,hkv,dim,q_len", [(16, 2, 64, 1), (16, 1, 128, 1), (32, 1, 128, 1), (16, 2, 256, 1),
+                                              (16, 2, 64, 5), (16, 2, 128, 20)])
+def test_what_nobody_sees_changes_no_bit(hq, hkv, dim, q_len):
+    """Old codes behind a request's last token, small, of the largest magnitude and NaN. (They must not
+    even move a row's running maximum, which its weights are rounded against.)"""
+    lens = [150, 135, 260, 131, 300, 145]
+    p = paged_problem(lens, hq, hkv, dim, 64, "bf16", [q_len] * len(lens), seed=dim, spread=3.0)
+    results = []
+    for value in (0.0, 448.0, -448.0, float("nan")):
+        for (codes, _), _ in zip(p["gpu"], p["caches"]):
+            for b, n in enumerate(lens):
+                codes[p["table"][b][n // 64], :, n % 64:] = value
+        results.append(call(p, return_lse=True))
+    for o, lse in results[1:]:
+        assert torch.equal(o, results[0][0]) and torch.equal(lse, results[0][1])
+
+
+def test_limits_that_reach_past_everything():
+    """A window or a bound on the rows above what 31 bits hold is the same as none."""
+    p = paged_problem([90, 33], 4, 2, 64, 16, "bf16", [3, 2], seed=9)
+    want = call(p)
+    assert torch.equal(call(p, window_left=2 ** 40), want)
+    p["max_q"] = 2 ** 40
+    assert torch.equal(call(p), want)
+    from apex_attn import kv_cache_plan
+    one = ints([1])
+    with pytest.raises(ValueError):
+        kv_cache_plan(ints([[0, 1]]), one, one, ints([2, 3]), one, 16, 2 ** 40)
+
+
+def test_lse_outside_the_requests_is_zero_with_a_given_out():
+    p = paged_problem([100, 50], 4, 2, 64, 16, "bf16", [2, 3], seed=5, spare_rows=9)
+    torch.full((4, 14), 3.0, device="cuda")  # what a new tensor may find in its place
+    out = torch.full(p["q"].shape, 7.0, dtype=p["q"].dtype, device="cuda")
+    o, lse = call(p, out=out, return_lse=True)
+    assert (o[5:] == 7).all() and not lse[:, 5:].any()
+    assert torch.equal(lse, call(p, return_lse=True)[1])
+
+
+def test_outputs_and_caches_that_overlap_themselves_are_refused():
+    import apex_attn
+    p = paged_problem([40, 20], 4, 2, 64, 16, "bf16", [1, 1], seed=12)
+    with pytest.raises(ValueError):
+        call(p, out=torch.zeros(1, 4, 64, dtype=torch.bfloat16, device="cuda").expand(2, 4, 64))
+    heads_first = torch.zeros(4, 2, 64, dtype=torch.bfloat16, device="cuda").transpose(0, 1)
+    assert torch.equal(call(p, out=heads_first), call(p))
+    (kc, ks), (vc, vs) = p["gpu"]
+    k = torch.zeros(1, 2, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError):
+        apex_attn.kv_cache_append(k, k, kc[:1].expand_as(kc), vc, ks, vs, torch.zeros(1, dtype=torch.int64, device="cuda"))
