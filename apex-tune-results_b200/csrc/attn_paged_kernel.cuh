@@ -95,25 +95,29 @@ struct PagedCfg {
   static constexpr uint32_t kSwizzle = kRow == 128 ? 2 : 4;
   static constexpr int kTerms = std::is_same<T, __half>::value ? 3 : 2;  // of q
   static constexpr bool kQueryMajor = NQ >= 64;
-  // Columns of an S buffer. (Query-major M is 128 for 64-row tiles too: the products read what lies
-  // behind the 64 rows of Q and of the weights, and nobody reads rows 64 .. 127 of the results.)
+  // Columns of an S buffer.
   static constexpr int kSCols = kQueryMajor ? kPagedTile : NQ;
   static constexpr int kWG = kQueryMajor ? 4 : 1;        // softmax warpgroups
   // Query-major, d <= 128: two pairs of warpgroups take the tiles in turn, each pair with its own
   // maxima, sums and O, so that one's exponentials run while the other loads and converts.
   static constexpr int kPairs = kQueryMajor && D <= 128 ? 2 : 1;
   static constexpr int kLead = kPairs;                   // S runs this many tiles ahead of P V
-  static constexpr int kNC = 32 < NQ ? 32 : NQ;          // S values per thread at once: query rows, or tokens
   static constexpr int kSoftWarps = 4 * kWG;
   static constexpr int kTileWarps = kSoftWarps / kPairs; // softmax warps per tile
   static constexpr int kThreads = 128 * (kWG + 1);
   // Two CTAs per SM cover each other's latencies where their shared memory fits.
   static constexpr int kCtas = (D <= 128 && NQ <= 32) ? 2 : 1;
   static constexpr int kSlotBytes = kPagedTile * D;      // one K or V tile
-  static constexpr int kQBytes = kTerms * NQ * D;        // one segment's query rows
   static constexpr int kPTerm = kPagedTile * NQ;         // one term of one P buffer
   static constexpr int kBudget = kCtas == 2 ? 115712 : 232448;
-  static constexpr int kMiscBytes = 2240 + NQ * 56 + (kQueryMajor ? 14 * 128 * 4 : 0);      // what the plan below adds
+  static constexpr int kMiscBytes = 2240 + NQ * 56 + (kQueryMajor ? 14 * 128 * 4 : 0);  // what the plan below adds
+  // Query-major M is 128 for 64-row tiles too. Where shared memory holds Q twice, rows 64 .. 127 of S
+  // repeat the first 64 and their threads take half of the tokens: TMEM lanes belong to warps by
+  // their quarter, so two of the SM's four schedulers would do nothing otherwise. Of O, rows 64 .. 127
+  // are never read; the weights that they come from are what lies behind the 64 rows.
+  static constexpr int kCopies =
+      NQ == 64 && 2 * kTerms * NQ * D + kTerms * kPTerm + kMiscBytes + 3 * kSlotBytes <= kBudget ? 2 : 1;
+  static constexpr int kQBytes = kTerms * NQ * D * kCopies;  // one segment's query rows
   static constexpr int slots(int q_bufs, int p_bufs) {
     return (kBudget - q_bufs * kQBytes - p_bufs * kTerms * kPTerm - kMiscBytes) / kSlotBytes;
   }
@@ -125,6 +129,11 @@ struct PagedCfg {
   static constexpr int kQBufs = !kSelfSplit && slots(2, kPBufs) >= 4 ? 2 : 1;
   static constexpr int kNS = slots(kQBufs, kPBufs) > 12 ? 12 : slots(kQBufs, kPBufs);  // ring slots
   static_assert(kNS > kLead, "the ring needs K(j + kLead) beside V(j)");
+  // Query-major: threads per row and tile, and the tokens of each.
+  static constexpr int kParts = kWG / kPairs * kCopies;
+  static constexpr int kTok = kPagedTile / kParts;
+  // S values per thread at once: query rows, or tokens.
+  static constexpr int kNC = kQueryMajor ? (kTok < 32 ? kTok : 32) : NQ;
   static constexpr int kScaleRing = 8;
   static constexpr int kSegRing = 4;
   // TMEM: S buffers at 0 and kSCols, O from 2 kSCols on (token-major: a block of NQ columns per 128 of
@@ -529,7 +538,7 @@ __device__ __forceinline__ void split_query_rows(const PagedParams& p, const Pag
     if constexpr (!C::kQueryMajor) return dst + chunk * (NQ * 16) + c * 16;
     constexpr int kUnits = C::kRow / 16;
     const uint32_t off = (uint32_t)(c * C::kRow + chunk % kUnits * 16);
-    return dst + chunk / kUnits * (NQ * C::kRow) + (off ^ (((off >> 7) & (kUnits - 1)) << 4));
+    return dst + chunk / kUnits * (C::kCopies * NQ * C::kRow) + (off ^ (((off >> 7) & (kUnits - 1)) << 4));
   };
   const T* const q = static_cast<const T*>(p.q) + (long long)seg.q0 * p.q_st +
                      (long long)(seg.h * p.group) * p.q_sh + chunk * 16;
@@ -579,8 +588,11 @@ __device__ __forceinline__ void split_query_rows(const PagedParams& p, const Pag
       for (int j = 0; j < C::kTerms; ++j) term[j][k] = four[j];
     }
 #pragma unroll
-    for (int j = 0; j < C::kTerms; ++j)
-      ptx::st_shared_v4(place_of(c) + j * NQ * D, term[j][0], term[j][1], term[j][2], term[j][3]);
+    for (int j = 0; j < C::kTerms; ++j) {
+      const uint32_t at = place_of(c) + j * C::kCopies * NQ * D;
+      ptx::st_shared_v4(at, term[j][0], term[j][1], term[j][2], term[j][3]);
+      if (C::kCopies == 2) ptx::st_shared_v4(at + NQ * C::kRow, term[j][0], term[j][1], term[j][2], term[j][3]);
+    }
     if (C::kQueryMajor) {
       if (chunk == 0) col_nm[NQ + c] = s;
     } else if (chunk == 0) {
@@ -764,27 +776,31 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     };
     bool more = next_for_all(seg);
     if constexpr (C::kQueryMajor) {
-      // Thread: row `t` of the tile, tokens tok0 .. tok0 + kTok - 1 of the tiles of its pair; the warps
-      // of a pair that share a TMEM quarter share its rows and agree on their maxima.
+      // Thread: row `row` of the tile, tokens tok0 .. tok0 + kTok - 1 of the tiles of its pair; the warps
+      // of a pair that share rows (one TMEM quarter's, or two with the same rows) agree on their maxima.
       constexpr int kWGs = C::kWG / C::kPairs;     // warpgroups per pair
-      constexpr int kTok = kPagedTile / kWGs;      // tokens per thread, 32 at a time
-      const int quarter = warp & 3, pair = wg / kWGs, tok0 = wg % kWGs * kTok;
-      const int vote = 1 + pair * 4 + quarter;     // barrier of the quarter's warps in the pair
+      constexpr int kTok = C::kTok, kParts = C::kParts, kQuarters = 4 / C::kCopies;
+      const int quarter = warp & 3, pair = wg / kWGs, rows_of = quarter % kQuarters;
+      const int row = rows_of * 32 + lane, copy = quarter / kQuarters;
+      const int tok0 = (wg % kWGs * C::kCopies + copy) * kTok;
+      const int vote = 1 + pair * 4 + rows_of;     // barrier of the pair's warps that share the rows
+      // What part k of a row's threads in pair q wrote to an exchange array at [wg * 128 + t].
+      auto part_at = [&](int q, int k) { return (q * kWGs + k / C::kCopies) * 128 + k % C::kCopies * NQ + row; };
       // Exchange: maxima [2 tiles][kWG][128], sums [kWG][128], references [pairs][128].
       float* const exchange = reinterpret_cast<float*>(smem + C::kRed);
 #pragma unroll 1
       for (int n = 0; more; ++n) {
         if (n == 0) split(seg, 0);
-        const float qs = reinterpret_cast<const float*>(smem + C::kCol)[(n & 1) * 5 * NQ + NQ + t];
+        const float qs = reinterpret_cast<const float*>(smem + C::kCol)[(n & 1) * 5 * NQ + NQ + row];
         int token, head;
-        paged_row(p, seg.token0, seg.head0, t, token, head);
+        paged_row(p, seg.token0, seg.head0, row, token, head);
         const int place = seg.len - seg.nq + min(token, seg.nq - 1);
         const int hi = p.causal ? min(place + 1, seg.len) : seg.len;
         const int lo = p.window >= 0 ? max(place - p.window, 0) : 0;
         float nm = 0.f, l = 0.f;  // kPagedTop - max; the row's sum over this thread's tokens
         bool set = false, force = true;
         // Rows past the tile's last: nobody reads their S, weights or O.
-        const bool idle = quarter * 32 >= seg.rows;
+        const bool idle = rows_of * 32 >= seg.rows;
 #pragma unroll 1
         for (int j = 0; j < seg.n; ++j, ++g) {
           const int sb = g & 1;
@@ -796,18 +812,18 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           wait(C::kSFull + sb, (uint32_t)(g >> 1));
           ptx::tc_fence_after();
           float2 d[NC / 2];
-          auto load = [&](int c0) {  // 32 tokens' scores
+          auto load = [&](int c0) {  // NC tokens' scores
             const uint32_t at = tmem + lane_off + (uint32_t)(sb * C::kSCols + c0);
-            ptx::tmem_ld16(at, reinterpret_cast<uint32_t*>(d));
-            ptx::tmem_ld16(at + 16, reinterpret_cast<uint32_t*>(d) + 16);
+#pragma unroll
+            for (int c = 0; c < NC; c += 16) ptx::tmem_ld16(at + c, reinterpret_cast<uint32_t*>(d) + c);
             ptx::tmem_wait_ld();
-            ptx::reg_fence16(reinterpret_cast<uint32_t*>(d));
-            ptx::reg_fence16(reinterpret_cast<uint32_t*>(d) + 16);
+#pragma unroll
+            for (int c = 0; c < NC; c += 16) ptx::reg_fence16(reinterpret_cast<uint32_t*>(d) + c);
           };
           // d = x + log2 b - m; -inf where the row does not see the token.
           auto scaled = [&](int c0) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
+            for (int half = 0; half < NC / 16; ++half) {
               const float4 s = sc[(c0 + 16 * half) >> p.block_shift];
               const float a = s.x * qs, b = s.y + nm;
               const float2 a2 = make_float2(a, a), b2 = make_float2(b, b);
@@ -837,15 +853,15 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
               for (int c = 0; c < NC / 2; ++c) most = ptx::fmax3(most, d[c].x, d[c].y);
             }
             const bool left = pos0 < seg.lo_all;
-            const bool move = force || left ? true : ptx::named_bar_or(vote, 32 * kWGs, most > kPagedMost);
+            const bool move = force || left ? true : ptx::named_bar_or(vote, 32 * kParts, most > kPagedMost);
             force = left;
             if (move) {
               float* const tops = exchange + ((g / C::kPairs) & 1) * C::kWG * 128;
               tops[wg * 128 + t] = most;
-              ptx::named_bar_sync(vote, 32 * kWGs);
+              ptx::named_bar_sync(vote, 32 * kParts);
               float top = most;
 #pragma unroll
-              for (int k = 0; k < kWGs; ++k) top = fmaxf(top, tops[(pair * kWGs + k) * 128 + t]);
+              for (int k = 0; k < kParts; ++k) top = fmaxf(top, tops[part_at(pair, k)]);
               // By how much the maximum moves: up only, but freely the first time.
               const bool some = top != -INFINITY;
               const float by = some ? (set ? fmaxf(top - kPagedTop, 0.f) : top - kPagedTop) : 0.f;
@@ -853,12 +869,12 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
               set = set || some;
               nm -= by;
               l *= f;
-              if (C::kPairs == 1) {  // d is still here; else it is loaded again below
+              if (kTok == NC) {  // d is still here; else it is loaded again below
                 const float2 by2 = make_float2(-by, -by);
 #pragma unroll
                 for (int c = 0; c < NC / 2; ++c) d[c] = __fadd2_rn(d[c], by2);
               }
-              if (j >= C::kPairs) {
+              if (j >= C::kPairs && copy == 0) {
                 wait(C::kPvDone + ((g - C::kPairs) & 1), (uint32_t)((g - C::kPairs) >> 1));
                 ptx::tc_fence_after();
 #pragma unroll 1
@@ -876,15 +892,15 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
               }
             }
             wait_p_buffer();
-            const uint32_t dst = sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kTerms * C::kPTerm + t * 128;
+            const uint32_t dst = sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kTerms * C::kPTerm + row * 128;
 #pragma unroll 1
             for (int c0 = 0; c0 < kTok; c0 += NC) {
-              if (C::kPairs == 2) {
+              if (kTok > NC) {
                 load(tok0 + c0);
                 scaled(tok0 + c0);
               }
 #pragma unroll
-              for (int half = 0; half < 2; ++half) {
+              for (int half = 0; half < NC / 16; ++half) {
                 const int c16 = tok0 + c0 + 16 * half;
                 uint32_t term[C::kTerms][4];
                 float2 sum = make_float2(0.f, 0.f);
@@ -901,7 +917,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
                   for (int i = 0; i < C::kTerms; ++i) term[i][k] = four[i];
                 }
                 l = fmaf(sum.x + sum.y, sc[c16 >> p.block_shift].z, l);
-                const uint32_t unit = (uint32_t)((c16 >> 4) ^ (t & 7)) << 4;
+                const uint32_t unit = (uint32_t)((c16 >> 4) ^ (row & 7)) << 4;
 #pragma unroll
                 for (int i = 0; i < C::kTerms; ++i)
                   ptx::st_shared_v4(dst + unit + i * C::kPTerm, term[i][0], term[i][1], term[i][2], term[i][3]);
@@ -915,8 +931,8 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           clear_unseen(j, 13 + pair, [&](int x) {
             const int pos = pos0 + x;
             if (!idle && x >= tok0 && x < tok0 + kTok && pos >= lo && pos < hi)
-              ptx::st_shared_u8(sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kTerms * C::kPTerm + t * 128 +
-                                    (((x >> 4) ^ (t & 7)) << 4) + (x & 15), 0x7fu);
+              ptx::st_shared_u8(sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kTerms * C::kPTerm + row * 128 +
+                                    (((x >> 4) ^ (row & 7)) << 4) + (x & 15), 0x7fu);
           });
           ptx::fence_proxy_async_smem();
           ptx::tc_fence_before();
@@ -938,25 +954,25 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
         float* const refs = sums + C::kWG * 128;
         sums[wg * 128 + t] = l;
         if (wg % kWGs == 0) refs[pair * 128 + t] = set ? nm : INFINITY;
-        ptx::named_bar_sync(9 + quarter, 32 * C::kWG);
-        float ref = refs[t];
+        ptx::named_bar_sync(9 + rows_of, 32 * C::kWG * C::kCopies);
+        float ref = refs[row];
 #pragma unroll
-        for (int k = 1; k < C::kPairs; ++k) ref = fminf(ref, refs[k * 128 + t]);
+        for (int k = 1; k < C::kPairs; ++k) ref = fminf(ref, refs[k * 128 + row]);
         // o = (sum_k f_k O_k) / (sum_k f_k l_k) over the pairs, f_k = 2^(m_k - max m).
         float f[C::kPairs], sum = 0.f;
 #pragma unroll
         for (int k = 0; k < C::kPairs; ++k) {
-          const float mine = refs[k * 128 + t];
+          const float mine = refs[k * 128 + row];
           f[k] = mine == INFINITY ? 0.f : ptx::ex2(ref - mine);
           float s = 0.f;
 #pragma unroll
-          for (int x = 0; x < kWGs; ++x) s += sums[(k * kWGs + x) * 128 + t];
+          for (int x = 0; x < kParts; ++x) s += sums[part_at(k, x)];
           sum = fmaf(f[k], s, sum);
         }
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
         for (int k = 0; k < C::kPairs; ++k) f[k] *= inv;
-        const bool real = t < seg.rows;
+        const bool real = copy == 0 && row < seg.rows;
         if (wg == 0 && real) {
           const float lse2 = sum == 0.f ? -INFINITY : __log2f(sum) - ref;
           if (seg.slot >= 0)
@@ -1334,10 +1350,11 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
                                               8 * C::kRow, C::kSwizzle);
 #pragma unroll
             for (int j = 0; j < C::kTerms; ++j) {
-              const uint32_t rows = sbase + C::kQ + (n % C::kQBufs) * C::kQBytes + j * NQ * D;
+              const uint32_t rows = sbase + C::kQ + (n % C::kQBufs) * C::kQBytes + j * C::kCopies * NQ * D;
               const uint32_t dS = tmem + (uint32_t)(sb * C::kSCols);
               if constexpr (C::kQueryMajor) {
-                const uint64_t q = ptx::smem_desc(rows + ch * (NQ * C::kRow) + ks * 32, 16, 8 * C::kRow, C::kSwizzle);
+                const uint64_t q = ptx::smem_desc(rows + ch * (C::kCopies * NQ * C::kRow) + ks * 32, 16,
+                                                  8 * C::kRow, C::kSwizzle);
                 ptx::umma_ss_f8_warp(dS, q, k, with_type(idS, j), acc);
               } else {
                 const uint64_t q = ptx::smem_desc(rows + (ch * (C::kRow / 16) + 2 * ks) * (NQ * 16), NQ * 16, 128, 0);
