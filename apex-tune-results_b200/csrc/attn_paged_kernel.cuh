@@ -656,7 +656,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       ptx::mbar_init(bar(C::kSegFull + s), 1);
       ptx::mbar_init(bar(C::kSegEmpty + s), C::kSoftWarps + 3);  // softmax, producer, MMA, query rows
     }
-    ptx::mbar_init(bar(C::kDrain), 1);
+    ptx::mbar_init(bar(C::kDrain), C::kQueryMajor ? 2 : 1);  // warps that issue products
     *abort_flag = 0;
     for (int k = 0; k < 8; ++k) reinterpret_cast<unsigned*>(smem + C::kBad)[k] = 0;
     ptx::fence_mbar_init();
@@ -842,12 +842,19 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           auto wait_p_buffer = [&]() {
             if (g >= C::kPBufs) wait(C::kPvDone + ((g - C::kPBufs) & 1), (uint32_t)((g - C::kPBufs) >> 1));
           };
+          // S is read: the MMA warp may write the buffer again.
+          auto release = [&]() {
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(bar(C::kSFree + sb));
+          };
           if (idle) wait_p_buffer();  // (clear_unseen counts on it)
           if (!idle) {
             float most = -INFINITY;
 #pragma unroll 1
             for (int c0 = 0; c0 < kTok; c0 += NC) {
               load(tok0 + c0);
+              if (kTok == NC) release();
               scaled(tok0 + c0);
 #pragma unroll
               for (int c = 0; c < NC / 2; ++c) most = ptx::fmax3(most, d[c].x, d[c].y);
@@ -924,10 +931,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
               }
             }
           }
-          // S is read: the MMA warp may write the buffer again.
-          ptx::tc_fence_before();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(bar(C::kSFree + sb));
+          if (idle || kTok > NC) release();
           clear_unseen(j, 13 + pair, [&](int x) {
             const int pos = pos0 + x;
             if (!idle && x >= tok0 && x < tok0 + kTok && pos >= lo && pos < hi)
@@ -1015,7 +1019,9 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
             *reinterpret_cast<uint4*>(o + c + 8) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
           }
         }
+        // Every warp has read its part of O before anyone's weights let the next P V write it.
         ptx::tc_fence_before();
+        ptx::named_bar_sync(15, 32 * C::kSoftWarps);
         seg = then;
       }
     } else {
@@ -1314,8 +1320,10 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       }
     }
     __syncwarp();
-  } else if (warp == kWarpMma) {
+  } else if (warp == kWarpMma || (C::kQueryMajor && warp == kWarpQ)) {
     // =============================================================== MMA ===
+    // Query-major, one warp issues S and another P V: the waits and the issue of a tile's products
+    // take a warp some 2500 cycles, the products themselves 1000.
     // e4m3, fp32 sums, M = 128. S: both operands K-major. P V: V is always MN-major; the weights
     // are MN-major as the B operand (token-major), K-major as the A operand (query-major).
     constexpr uint32_t kDesc = (1u << 4) | ((uint32_t)(128 >> 4) << 24);
@@ -1326,19 +1334,17 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     auto with_type = [](uint32_t id, int term) {
       return term == 2 ? id | (1u << (C::kQueryMajor ? 7 : 10)) : id;
     };
-    uint32_t reads = 0;  // ring slots consumed
     int gs = 0, gp = 0;  // S and P V tiles issued
-    auto acquire = [&]() -> int {
-      const int slot = (int)(reads % NS);
-      wait(C::kKvFull + slot, reads / NS);
-      ++reads;
+    auto acquire = [&](uint32_t fill) -> int {
+      const int slot = (int)(fill % NS);
+      wait(C::kKvFull + slot, fill / NS);
       return slot;
     };
     int n = 0;  // segments so far
-    auto issue_S = [&](bool last) {
+    auto issue_S = [&](uint32_t fill, bool last) {
       const int sb = gs & 1;
       if (gs >= 2) wait(C::kSFree + sb, (uint32_t)((gs >> 1) - 1));
-      const int slot = acquire();
+      const int slot = acquire(fill);
       ptx::tc_fence_after();
       if (ok) {
         uint32_t acc = 0;
@@ -1365,14 +1371,14 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           }
         ptx::tc_commit_warp(bar(C::kKvEmpty + slot));
         ptx::tc_commit_warp(bar(C::kSFull + sb));
-        if (last) ptx::tc_commit_warp(bar(C::kQEmpty + n % C::kQBufs));
+        if (!C::kQueryMajor && last) ptx::tc_commit_warp(bar(C::kQEmpty + n % C::kQBufs));
       }
       ++gs;
     };
-    auto issue_PV = [&](bool first) {
+    auto issue_PV = [&](uint32_t fill, bool first) {
       const int sb = gp & 1;
       wait(C::kPFull + sb, (uint32_t)(gp >> 1));
-      const int slot = acquire();
+      const int slot = acquire(fill);
       ptx::tc_fence_after();
       if (ok) {
         const uint32_t weights = sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kTerms * C::kPTerm;
@@ -1409,19 +1415,31 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       }
       ++gp;
     };
+    uint32_t fills = 0;  // of the segments before
     for (; next_segment(seg); ++n) {
-      wait(C::kQFull + (n & 1), (uint32_t)(n >> 1));
-      if (seg.n == 0) {
-        if (lane == 0) ptx::mbar_arrive(bar(C::kQEmpty + n % C::kQBufs));
-        continue;
-      }
+      // Places in the ring as the producer fills it.
+      auto k_at = [&](int j) { return fills + j + max(0, j - C::kLead); };
+      auto v_at = [&](int j) { return fills + j + min(seg.n, j + 1 + C::kLead); };
+      if (C::kQueryMajor && warp == kWarpQ) {
 #pragma unroll 1
-      for (int j = 0; j < min(seg.n, C::kLead); ++j) issue_S(j + 1 == seg.n);
+        for (int j = 0; j < seg.n; ++j) issue_PV(v_at(j), j < C::kPairs);
+      } else {
+        wait(C::kQFull + (n & 1), (uint32_t)(n >> 1));
+        if (C::kQueryMajor) {
 #pragma unroll 1
-      for (int j = 0; j < seg.n; ++j) {
-        if (j + C::kLead < seg.n) issue_S(j + C::kLead + 1 == seg.n);
-        issue_PV(j < C::kPairs);
+          for (int j = 0; j < seg.n; ++j) issue_S(k_at(j), false);
+        } else if (seg.n == 0) {
+          if (lane == 0) ptx::mbar_arrive(bar(C::kQEmpty + n % C::kQBufs));
+        } else {
+          issue_S(k_at(0), seg.n == 1);
+#pragma unroll 1
+          for (int j = 0; j < seg.n; ++j) {
+            if (j + 1 < seg.n) issue_S(k_at(j + 1), j + 2 == seg.n);
+            issue_PV(v_at(j), j == 0);
+          }
+        }
       }
+      fills += 2 * seg.n;
     }
     ptx::tc_commit_warp(bar(C::kDrain));
     if (lane == 0) drain_wait(bar(C::kDrain), 0, p.timeout_ns, p.status, p.host_flag);
@@ -1508,7 +1526,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     // ======================================================== query rows ===
     // Ahead of the softmax, from the second segment on.
     for (int n = 0; next_segment(seg); ++n) {
-      if (n == 0 || C::kSelfSplit) continue;
+      if (n == 0) continue;
       if (n >= C::kQBufs) wait(C::kQEmpty + n % C::kQBufs, (uint32_t)(n / C::kQBufs - 1));
       if (n >= 2) wait(C::kColEmpty + (n & 1), (uint32_t)((n >> 1) - 1));
       split_query_rows<T, D, NQ, 4>(p, seg, smem, n, 0, 1);
