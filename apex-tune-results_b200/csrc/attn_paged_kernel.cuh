@@ -904,6 +904,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
             for (int c0 = 0; c0 < kTok; c0 += NC) {
               if (kTok > NC) {
                 load(tok0 + c0);
+                if (c0 + NC == kTok) release();
                 scaled(tok0 + c0);
               }
 #pragma unroll
@@ -931,7 +932,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
               }
             }
           }
-          if (idle || kTok > NC) release();
+          if (idle) release();
           clear_unseen(j, 13 + pair, [&](int x) {
             const int pos = pos0 + x;
             if (!idle && x >= tok0 && x < tok0 + kTok && pos >= lo && pos < hi)
