@@ -5,7 +5,7 @@
 // the C ABI, whose addresses `init` gets, so this file links to nothing of the library.
 //
 // Measured on the host of a B200, Python alone / this: attention 15.9 / 7.4 us per call, append 8.0 /
-// 3.4 us, plan and release together 24 / 13 us; the kernels of a small decode step take as long.
+// 3.4 us, plan and release together 24 / 11 us; the kernels of a small decode step take as long.
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <Python.h>
@@ -63,6 +63,16 @@ int dtype_of(const at::Tensor& t) {
 
 at::Tensor new_tensor(at::IntArrayRef size, at::ScalarType type, int device) {
   return at::detail::empty_cuda(size, type, at::Device(at::kCUDA, (at::DeviceIndex)device), std::nullopt);
+}
+
+// `n` entries of a vector from `first` on, as a tensor of its own over the same storage. (Several small
+// outputs share an allocation: one of their own each took about half a microsecond.)
+at::Tensor part_of(const at::Tensor& t, int64_t first, int64_t n) {
+  at::Tensor part = at::detail::make_tensor<at::TensorImpl>(at::TensorImpl::VIEW, c10::Storage(t.storage()),
+                                                            t.key_set(), t.dtype());
+  part.unsafeGetTensorImpl()->set_storage_offset(first);
+  part.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return part;
 }
 
 // The cache of append and attend: pointers, sizes, and byte strides at strides[4 .. 9].
@@ -293,17 +303,17 @@ PyObject* wrapped(std::initializer_list<at::Tensor> tensors) {
 }
 
 // (..., max_new_tokens): (slots, cu_seqlens, seq_lens, free_count, placed)
-PyObject* plan(PyObject*, PyObject* const* o, Py_ssize_t n) {
+PyObject* plan(PyObject*, PyObject* const* o, Py_ssize_t given) {
   return guarded([&]() -> PyObject* {
-    if (n != 7 || !g.plan) return nullptr;
+    if (given != 7 || !g.plan) return nullptr;
     apex_attn_kv_plan_args a{};
     int device = -1;
     if (!bookkeeping_args(a, o, true, device) || !whole(o[6], a.max_new_tokens) || a.max_new_tokens < 1) return nullptr;
     const at::Tensor slots = new_tensor({a.max_new_tokens}, at::kLong, device);
-    const at::Tensor cu = new_tensor({(int64_t)a.batch + 1}, at::kInt, device);
-    const at::Tensor lens = new_tensor({a.batch}, at::kInt, device);
-    const at::Tensor count = new_tensor({1}, at::kInt, device);
-    const at::Tensor placed = new_tensor({a.batch}, at::kInt, device);
+    const int64_t n = a.batch;
+    const at::Tensor ints = new_tensor({3 * n + 2}, at::kInt, device);
+    const at::Tensor cu = part_of(ints, 0, n + 1), lens = part_of(ints, n + 1, n);
+    const at::Tensor placed = part_of(ints, 2 * n + 1, n), count = part_of(ints, 3 * n + 1, 1);
     a.slots = reinterpret_cast<long long*>(slots.data_ptr());
     a.cu_seqlens = static_cast<int*>(cu.data_ptr());
     a.seq_lens_out = static_cast<int*>(lens.data_ptr());
@@ -322,8 +332,8 @@ PyObject* release(PyObject*, PyObject* const* o, Py_ssize_t n) {
     apex_attn_kv_plan_args a{};
     int device = -1;
     if (!bookkeeping_args(a, o, false, device)) return nullptr;
-    const at::Tensor lens = new_tensor({a.batch}, at::kInt, device);
-    const at::Tensor count = new_tensor({1}, at::kInt, device);
+    const at::Tensor both = new_tensor({(int64_t)a.batch + 1}, at::kInt, device);
+    const at::Tensor lens = part_of(both, 0, a.batch), count = part_of(both, a.batch, 1);
     a.seq_lens_out = static_cast<int*>(lens.data_ptr());
     a.free_count_out = static_cast<int*>(count.data_ptr());
     void* stream = stream_of(device);
