@@ -408,7 +408,10 @@ int apex_attn_kv_release(const apex_attn_kv_plan_args* args, void* stream);
  * but for codes that leave e4m3's normal range). Codes are x / scale rounded to nearest even.
  * Values that are not finite do not count for the scale and are stored as NaN. Slots
  * outside [0, num_blocks * block_size) are skipped; rows of the block after the run stay as
- * they were. At most one run may go to a block in one call (what apex_attn_kv_plan gives).
+ * they were. At most one run may go to a block in one call (what apex_attn_kv_plan gives); two
+ * would write its scale at once, and one of them would win. A cache whose (block, head, token)
+ * rows overlap one another is refused (APEX_ATTN_ERR_BAD_LAYOUT). At most 2^30 tokens and 65535
+ * heads.
  *
  * strides: k token, head; v token, head (elements, multiples of 8); k_cache block, head,
  * token; v_cache block, head, token (bytes, multiples of 16). Pointers 16-byte aligned.
@@ -452,9 +455,17 @@ int apex_attn_kv_append(const apex_attn_kv_append_args* args, void* stream);
  * A row that sees nothing (an empty request, a position before the cache) gives o = 0 and
  * lse = -infinity. Table entries outside [0, num_blocks) read as zeros; entries of blocks that
  * no row of a request sees are not read, and what the cache holds there or behind the last
- * token (NaN codes too) does not matter. Scores, softmax statistics and sums are fp32.
+ * token (NaN codes too) changes no bit of the result. Scores, softmax statistics and sums are
+ * fp32. Scales are not negative; V scales below 2^-100 count as 2^-100. A code or scale of NaN,
+ * or a value of q that is not finite, gives NaN to the rows that see it and to no others.
+ * Offsets that fall or overlap give wrong rows, but nothing outside q and o is touched.
+ * Refused: rows of o that overlap one another (APEX_ATTN_ERR_BAD_LAYOUT); above 2^30 query rows
+ * over all heads or cached tokens per request, 65535 requests or 32767 heads, or where
+ * heads_kv * (total_q * group / query rows per tile + batch) * (tiles of 128 tokens of the table's
+ * width + 9) passes 2^31 (APEX_ATTN_ERR_TOO_LARGE).
  * workspace: device memory of at least apex_attn_fwd_paged_workspace_bytes(...) bytes, 16-byte
- * aligned, used only during the call; calls that can overlap need one each.
+ * aligned, used only during the call; calls that can overlap, two captured graphs among them,
+ * need one each. The first call per device sets up the library there: make it before a capture.
  */
 typedef struct apex_attn_paged_args {
   const void* q;
