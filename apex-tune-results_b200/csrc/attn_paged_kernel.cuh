@@ -167,6 +167,14 @@ struct PagedCfg {
   static_assert(!kQueryMajor || kBytes - kBars >= (128 - NQ) * 128, "rows behind the last weights");
 };
 
+// Inputs are read by plain loads. The kernel may start while the one that writes them still runs
+// (it waits for that before it reads), and then they are not constant for its lifetime, as the
+// non-coherent path takes them to be.
+template <typename V>
+__device__ __forceinline__ V read_input(const V* at) {
+  return *at;
+}
+
 // The query rows of request b and where they stand.
 struct PagedRequest {
   int q0, nq, len;  // first row, rows, cached tokens
@@ -175,14 +183,14 @@ struct PagedRequest {
 __device__ __forceinline__ PagedRequest paged_request(const PagedParams& p, int b) {
   PagedRequest r;
   if (p.cu_seqlens_q != nullptr) {
-    r.q0 = min(max(__ldg(p.cu_seqlens_q + b), 0), p.total_q);
-    r.nq = min(max(__ldg(p.cu_seqlens_q + b + 1), r.q0), p.total_q) - r.q0;
+    r.q0 = min(max(read_input(p.cu_seqlens_q + b), 0), p.total_q);
+    r.nq = min(max(read_input(p.cu_seqlens_q + b + 1), r.q0), p.total_q) - r.q0;
     r.nq = min(r.nq, p.max_q);
   } else {
     r.nq = p.max_q;
     r.q0 = b * r.nq;
   }
-  r.len = min(max(__ldg(p.seq_lens + b), 0), p.table_width << p.block_shift);
+  r.len = min(max(read_input(p.seq_lens + b), 0), p.table_width << p.block_shift);
   return r;
 }
 
@@ -276,13 +284,18 @@ struct PagedWalk {
   int b, h, qt, qts;
   int item;  // first unit of the item (b, h, qt)
   int tiles_begin = 0, tiles_end = 0;  // units of the tiles of the last segment's item
-  PagedRequest r;
+  PagedRequest r, ahead;  // of b, and of b + 1, read before it is needed
+
+  __device__ __forceinline__ void look_ahead() {
+    if (b + 1 < p.batch) ahead = paged_request(p, b + 1);
+  }
 
   __device__ __forceinline__ PagedWalk(const PagedParams& params, const PagedStart& s)
       : p(params), unit(s.unit), end(s.end), share(s.share), more(s.more), b(s.b), h(0), qt(0), qts(0),
         item(s.request_unit) {
     if (unit >= end) return;
     r = paged_request(p, b);
+    look_ahead();
     qts = paged_qtiles<NQ>(p, r);
     const int into = unit - item;
     if (p.heads_kv > 1 && into > 0) {
@@ -314,7 +327,8 @@ struct PagedWalk {
         if (++h == p.heads_kv || qts == 0) {
           h = 0;
           if (++b >= p.batch) return s;  // (units and requests always end together)
-          r = paged_request(p, b);
+          r = ahead;
+          look_ahead();
           qts = paged_qtiles<NQ>(p, r);
         }
       }
@@ -555,8 +569,8 @@ __device__ __forceinline__ void split_query_rows(const PagedParams& p, const Pag
       int token, head;
       paged_row(p, seg.token0, seg.head0, c, token, head);
       const uint4* src = reinterpret_cast<const uint4*>(q + token * p.q_st + head * p.q_sh);
-      a = __ldg(src);
-      b = __ldg(src + 1);
+      a = read_input(src);
+      b = read_input(src + 1);
     }
   };
   const int first = w * kStep + lane / kPerRow, step = warps * kStep;
@@ -1245,7 +1259,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     auto page_ids = [&](const PagedSegment& s, int tile) -> int {
       const int at = (tile + (lane >> 3)) * kPagedTile + ((lane & 7) << p.block_shift);
       if ((lane & 7) >= pages || at >= s.hi || at + (1 << p.block_shift) <= s.lo) return -2;
-      const int id = __ldg(p.block_table + (long long)s.b * p.table_stride + (at >> p.block_shift));
+      const int id = read_input(p.block_table + (long long)s.b * p.table_stride + (at >> p.block_shift));
       return id >= 0 && id < p.num_blocks ? id : -1;
     };
     // The next K tile, V tile or both, from the block ids in lanes 0 .. pages - 1 and V's in lanes
@@ -1500,10 +1514,10 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
         // Pages that are not there: zero scores and values, and a V scale too small to move a maximum.
         float4 sc = make_float4(0.f, -100.f, 1.f / kPagedLeastScale, 0.f);
         if (j < seg.n && page < pages && at < seg.hi && at + (1 << p.block_shift) > seg.lo) {
-          const int id = __ldg(p.block_table + (long long)seg.b * p.table_stride + (at >> p.block_shift));
+          const int id = read_input(p.block_table + (long long)seg.b * p.table_stride + (at >> p.block_shift));
           if (id >= 0 && id < p.num_blocks) {
-            const float a = __ldg(p.k_scale + (long long)id * p.heads_kv + seg.h);
-            const float given = __ldg(p.v_scale + (long long)id * p.heads_kv + seg.h);
+            const float a = read_input(p.k_scale + (long long)id * p.heads_kv + seg.h);
+            const float given = read_input(p.v_scale + (long long)id * p.heads_kv + seg.h);
             const float b = fmaxf(given, kPagedLeastScale);
             // A scale of NaN goes on in the exponent, which is masked; 1 / b is not, and stays a number.
             sc = make_float4(a * p.scale_log2, given != given ? given : __log2f(b), 1.f / b, 0.f);

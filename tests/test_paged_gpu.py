@@ -862,3 +862,31 @@ def test_outputs_and_caches_that_overlap_themselves_are_refused():
     k = torch.zeros(1, 2, 64, dtype=torch.bfloat16, device="cuda")
     with pytest.raises(RuntimeError):
         apex_attn.kv_cache_append(k, k, kc[:1].expand_as(kc), vc, ks, vs, torch.zeros(1, dtype=torch.int64, device="cuda"))
+
+
+def test_outputs_that_are_the_next_call_s_queries():
+    """A chain of calls, each reading what the one before wrote, on one stream and captured: every call
+    may start while the last is still running, and waits for it before it reads."""
+    p = paged_problem([700, 33, 2100], 16, 4, 128, 32, "bf16", [1, 1, 1], seed=21)
+    step = lambda x: call({**p, "q": x}, decode=True)
+    want = [p["q"].cuda()]
+    for _ in range(6):
+        want.append(step(want[-1]))
+        torch.cuda.synchronize()
+    x = p["q"].cuda()
+    for _ in range(6):
+        x = step(x)
+    assert torch.equal(x, want[-1])
+
+    from apex_attn import custom_attention_paged_forward
+    (kc, ks), (vc, vs) = p["gpu"]
+    table, lens, q = ints(p["table"]), ints(p["lens"]), p["q"].cuda()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = q
+        for _ in range(6):
+            y = custom_attention_paged_forward(y, kc, vc, ks, vs, table, lens)
+    for _ in range(3):
+        y.fill_(float("nan"))
+        graph.replay()
+        assert torch.equal(y, want[-1])
