@@ -41,8 +41,8 @@
 // Lengths are read on the device only.
 //
 // Warps: 4 to 16 softmax (32 rows of TMEM each), then TMA producer, MMA issuer, scales and work
-// list, and a fourth: token-major it splits the next segment's query rows, query-major it issues
-// P V. The scales' warp alone walks the work list and publishes the segments
+// list, and a fourth: token-major it splits the next segment's query rows, with
+// 64-row tiles it issues P V. The scales' warp alone walks the work list and publishes the segments
 // in shared memory: a warp on its own takes some 4 cycles per dependent instruction, and all
 // warps walking cost each of them about 2 us at the start and 1 us per segment.
 //
@@ -132,6 +132,11 @@ struct PagedCfg {
   // leaves four ring slots; a query-major tile's are too many for one warp, and the softmax
   // warps split them between segments.
   static constexpr bool kSelfSplit = kQueryMajor;
+  // 64-row tiles: one warp issues S and another P V. The waits and the issue of a tile's products
+  // take a warp some 2500 cycles, the products themselves 1000, and the softmax of half a
+  // tile's rows no longer covers that (32 requests of 40 rows, fp16: 33.7 -> 31.6 us; with 128
+  // rows it does, and two warps make 3 x 1024 new tokens 562 us instead of 520).
+  static constexpr bool kTwoIssuers = NQ == 64;
   static constexpr int kQBufs = !kSelfSplit && slots(2, kPBufs) >= 4 ? 2 : 1;
   static constexpr int kNS = slots(kQBufs, kPBufs) > 12 ? 12 : slots(kQBufs, kPBufs);  // ring slots
   static_assert(kNS > kLead, "the ring needs K(j + kLead) beside V(j)");
@@ -676,7 +681,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       ptx::mbar_init(bar(C::kSegFull + s), 1);
       ptx::mbar_init(bar(C::kSegEmpty + s), C::kSoftWarps + 3);  // softmax, producer, MMA, query rows
     }
-    ptx::mbar_init(bar(C::kDrain), C::kQueryMajor ? 2 : 1);  // warps that issue products
+    ptx::mbar_init(bar(C::kDrain), C::kTwoIssuers ? 2 : 1);  // warps that issue products
     *abort_flag = 0;
     for (int k = 0; k < 8; ++k) reinterpret_cast<unsigned*>(smem + C::kBad)[k] = 0;
     ptx::fence_mbar_init();
@@ -1351,10 +1356,8 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       }
     }
     __syncwarp();
-  } else if (warp == kWarpMma || (C::kQueryMajor && warp == kWarpQ)) {
+  } else if (warp == kWarpMma || (C::kTwoIssuers && warp == kWarpQ)) {
     // =============================================================== MMA ===
-    // Query-major, one warp issues S and another P V: the waits and the issue of a tile's products
-    // take a warp some 2500 cycles, the products themselves 1000.
     // e4m3, fp32 sums, M = 128. S: both operands K-major. P V: V is always MN-major; the weights
     // are MN-major as the B operand (token-major), K-major as the A operand (query-major).
     constexpr uint32_t kDesc = (1u << 4) | ((uint32_t)(128 >> 4) << 24);
@@ -1451,22 +1454,23 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       // Places in the ring as the producer fills it.
       auto k_at = [&](int j) { return fills + j + max(0, j - C::kLead); };
       auto v_at = [&](int j) { return fills + j + min(seg.n, j + 1 + C::kLead); };
-      if (C::kQueryMajor && warp == kWarpQ) {
+      if (C::kTwoIssuers && warp == kWarpQ) {
 #pragma unroll 1
         for (int j = 0; j < seg.n; ++j) issue_PV(v_at(j), j < C::kPairs);
       } else {
         wait(C::kQFull + (n & 1), (uint32_t)(n >> 1));
-        if (C::kQueryMajor) {
+        if (C::kTwoIssuers) {
 #pragma unroll 1
           for (int j = 0; j < seg.n; ++j) issue_S(k_at(j), false);
-        } else if (seg.n == 0) {
-          if (lane == 0) ptx::mbar_arrive(bar(C::kQEmpty + n % C::kQBufs));
         } else {
-          issue_S(k_at(0), seg.n == 1);
+          if (!C::kQueryMajor && seg.n == 0 && lane == 0) ptx::mbar_arrive(bar(C::kQEmpty + n % C::kQBufs));
+#pragma unroll 1
+          for (int j = 0; j < min(seg.n, C::kLead); ++j) issue_S(k_at(j), j + 1 == seg.n);
 #pragma unroll 1
           for (int j = 0; j < seg.n; ++j) {
-            if (j + 1 < seg.n) issue_S(k_at(j + 1), j + 2 == seg.n);
-            issue_PV(v_at(j), j == 0);
+            const int next = j + C::kLead;
+            if (next < seg.n) issue_S(k_at(next), next + 1 == seg.n);
+            issue_PV(v_at(j), j < C::kPairs);
           }
         }
       }
@@ -1557,7 +1561,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     // ======================================================== query rows ===
     // Ahead of the softmax, from the second segment on.
     for (int n = 0; next_segment(seg); ++n) {
-      if (n == 0) continue;
+      if (n == 0 || C::kSelfSplit) continue;
       if (n >= C::kQBufs) wait(C::kQEmpty + n % C::kQBufs, (uint32_t)(n / C::kQBufs - 1));
       if (n >= 2) wait(C::kColEmpty + (n & 1), (uint32_t)((n >> 1) - 1));
       split_query_rows<T, D, NQ, 4>(p, seg, smem, n, 0, 1);
