@@ -46,9 +46,9 @@
 // in shared memory: a warp on its own takes some 4 cycles per dependent instruction, and all
 // warps walking cost each of them about 2 us at the start and 1 us per segment.
 //
-// Bound: a decode step by the cache's bytes (48 requests of up to 8191 tokens, 410 MB: 76 us, 5.4
+// Bound: a decode step by the cache's bytes (48 requests of up to 8191 tokens, 410 MB: 73 us, 5.6
 // TB/s; about 7 us of them pass before the first scores are there, 4 in the joining kernel);
-// calls with many new tokens by the softmax warps' issue (3 x 1024 tokens on 16k: 561 us, 775
+// calls with many new tokens by the softmax warps' issue (3 x 1024 tokens on 5k to 16k: 520 us, 838
 // TFLOP/s; schedulers busy 48 %, tensor pipe 28 %).
 #pragma once
 
@@ -240,7 +240,7 @@ __device__ __forceinline__ int paged_qtiles(const PagedParams& p, const PagedReq
 // A CTA that begins an item spends about as long on it as on this many tiles: units of an item
 // are these and then its tiles, at least one (an item that sees nothing still has rows to
 // write). Without them the CTAs that got short requests finished last: 48 requests of 129 to
-// 8191 tokens take 92 us instead of 76, and three of 1024 new tokens each 588 instead of 561.
+// 8191 tokens take 88 us instead of 73, and three of 1024 new tokens each 565 instead of 520.
 template <int NQ>
 constexpr int kPagedItemUnits = NQ <= 32 ? 4 : 8;
 
