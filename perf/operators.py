@@ -28,19 +28,13 @@ MIN_EXPONENT = -100  # the smallest scale that an append writes is 2^-100
 _DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 
 
-_package = None
-
-
 def _library():
-    """The framework's package (kept below the repository's root), imported once."""
-    global _package
-    if _package is None:
-        path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "apex-tune-results_b200")
-        if path not in sys.path:
-            sys.path.insert(0, path)
-        import apex_attn
-        _package = apex_attn
-    return _package
+    """The framework's package (kept below the repository's root)."""
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "apex-tune-results_b200")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import apex_attn
+    return apex_attn
 
 
 # ------------------------------------------------------------------------- cases --
