@@ -116,7 +116,7 @@ struct PagedCfg {
   static constexpr int kSlotBytes = kPagedTile * D;      // one K or V tile
   static constexpr int kPTerm = kPagedTile * NQ;         // one term of one P buffer
   static constexpr int kBudget = kCtas == 2 ? 115712 : 232448;
-  static constexpr int kMiscBytes = 2240 + NQ * 56 + (kQueryMajor ? 14 * 128 * 4 : 0);  // what the plan below adds
+  static constexpr int kMiscBytes = 2240 + NQ * 60 + (kQueryMajor ? 14 * 128 * 4 : 0);  // what the plan below adds
   // Query-major M is 128 for 64-row tiles too. Where shared memory holds Q twice, rows 64 .. 127 of S
   // repeat the first 64 and their threads take half of the tokens: TMEM lanes belong to warps by
   // their quarter, so two of the SM's four schedulers would do nothing otherwise. Of O, rows 64 .. 127
@@ -162,8 +162,8 @@ struct PagedCfg {
                        kSegEmpty = kSegFull + kSegRing, kDrain = kSegEmpty + kSegRing, kNumBars = kDrain + 1;
   static constexpr int kScales = (kBars + kNumBars * 8 + 15) / 16 * 16;  // float4 [kScaleRing][8 pages]
   static constexpr int kCol = kScales + kScaleRing * 8 * 16;  // two of, per query row: -m, q scale, factor, hi, lo
-  static constexpr int kRed = kCol + 2 * 5 * NQ * 4;          // token-major [4 warps][NQ], query-major [14][128]
-  static constexpr int kSegs = (kRed + (kQueryMajor ? 14 * 128 : 4 * NQ) * 4 + 15) / 16 * 16;       // int4 [kSegRing][kSegVecs]
+  static constexpr int kRed = kCol + 2 * 5 * NQ * 4;          // token-major [4 warps + 1][NQ], query-major [14][128]
+  static constexpr int kSegs = (kRed + (kQueryMajor ? 14 * 128 : 5 * NQ) * 4 + 15) / 16 * 16;       // int4 [kSegRing][kSegVecs]
   static constexpr int kBad = kSegs + kSegRing * 4 * 16;                 // unsigned [2][4]
   static constexpr int kScan = kBad + 32;                // long long [32], found request
   static constexpr int kMisc = kScan + 32 * 8 + 16;
@@ -736,7 +736,11 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     const int t = (warp & 3) * 32 + lane;  // token of the tile; column of the head dim
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     const int c_first = wg * NC;           // this warpgroup's query rows of the tile
-    float* const red = reinterpret_cast<float*>(smem + C::kRed) + wg * 4 * NC;
+    // The warps' maxima or sums of each query row (token-major), and by how much a row's maximum
+    // moves. That has a place of its own: a warp may still read it while another, with no barrier
+    // between, writes its sums at the segment's end or the maxima of the next move.
+    float* const red = reinterpret_cast<float*>(smem + C::kRed) + wg * 5 * NC;
+    float* const moved = red + 4 * NC;
     const float4* const scales = reinterpret_cast<const float4*>(smem + C::kScales);
     const int page = t >> p.block_shift;
     int g = 0;  // tiles so far
@@ -1129,12 +1133,12 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
               const float by = top == -INFINITY ? 0.f : (set ? fmaxf(top - kPagedTop, 0.f) : top - kPagedTop);
               if (set || top != -INFINITY) col_f[t] = set ? ptx::ex2(-by) : 0.f;
               col_nm[t] -= by;
-              red[t] = by;
+              moved[t] = by;
             }
             ptx::named_bar_sync(1 + wg, 128);
 #pragma unroll
             for (int c = 0; c < NC / 2; ++c) {
-              const float2 by = *reinterpret_cast<const float2*>(red + 2 * c);
+              const float2 by = *reinterpret_cast<const float2*>(moved + 2 * c);
               d[c] = make_float2(d[c].x - by.x, d[c].y - by.y);
               l[c] = __fmul2_rn(l[c], *reinterpret_cast<const float2*>(col_f + 2 * c));
             }
