@@ -7,32 +7,36 @@
 //
 // The codes never leave 8 bits: both products run on tcgen05.mma kind::f8f6f4 with the cache
 // tiles as the TMA wrote them to shared memory, so nothing converts the cache. What is not
-// e4m3 is split into terms that add up to it, two of e4m3 for bf16 calls, and a third of e5m2 for
-// fp16 ones:
-//   * q, scaled per row by a power of two so that its largest magnitude lies in (224, 448]: its
-//     8 or 11 significant bits in pieces of 4, 4 and 3, exact but for what lies below 2^-10 (two
-//     terms) or 2^-17;
+// 8 bits wide is split into terms that add up to it:
+//   * q, scaled per row by a power of two so that its largest magnitude lies in (224, 448]: two
+//     terms of e4m3 for bf16 calls, and a third of e5m2 for fp16 ones. Its 8 or 11 significant bits
+//     in pieces of 4, 4 and 3, exact but for what lies below 2^-10 (two terms) or 2^-17;
 //   * the weight p'_ij = 2^(x_ij + log2 b_j - m_i) (the V scale goes into the exponent, one
-//     addition per token), rounded to fp16: off by 2^-8 of itself or 2^-10 (two terms), by 2^-11 of
-//     itself or 2^-17 (three). With two terms an fp16 output was 3.3 times as far from its float64
-//     value as rounding alone puts it; a bf16 output's own rounding hides the difference. With
-//     three terms of e4m3, 131k flat weights still made it 1.8 times as far.
-// fp32 accumulation of e4m3 products on this card is exact to 2^-23 of the magnitudes.
+//     addition per token), rounded to fp16: three terms of e5m2 for either type. Each is the nearest to
+//     what the ones before it left, with a sign of its own, so that the 11 bits come in pieces of 3, 4
+//     and 4: exact for weights from 2^-6 on, off by at most 2^-17 below. So a weight is off by 2^-11
+//     of itself, or by 2^-30 of the row's largest.
+// The weights need e5m2's exponents more than e4m3's bits. A row may have most of its weight on one
+// token whose V is small, and its output is then the mean of many small weights: with two terms of
+// e4m3, which end 2^-16 below the largest, 8192 tokens behind one of share 0.95 vanished from the
+// output (and not from the sum); with a third of e5m2 they were off by 4 % where all were alike.
+// fp32 accumulation of 8-bit products on this card is exact to 2^-23 of the magnitudes.
 //
 // Up to 32 query rows per K/V head, tokens are the M side ("token-major"): S^T = K Q^T and O^T = V^T P,
 // M = 128 tokens resp. 128 columns of the head dim, N = 16 or 32 query rows. A decode step has 1 to
 // 16 query rows per K/V head; as the M side they would leave most of a 128-row tile empty. Thread t
 // owns token t of a tile: its scales are per-thread scalars and its row of P is 16 contiguous bytes
 // per 16 query rows. The price is that a row's maximum runs across threads; so the running
-// maximum is only moved when some p' would pass 2^8.75 (one vote per tile), which is rare after
+// maximum is only moved when some p' would pass 2^15.75 (one vote per tile), which is rare after
 // a row's first tile.
 // More rows, in tiles of 64 or 128, are the M side themselves ("query-major"): S = Q K^T, O = P V, a
 // thread owns part of a row, and a maximum takes one exchange between warps. (Measured: two
 // 32-row token-major tiles for 33 to 96 rows are 10 to 60 % slower than one of 64 or 128.)
 //
-// m_i tracks the maximum of x_ij + log2 b_j, kept 2^6 below p's top so that small weights stay
-// above e4m3's floor: the largest weight of a row is held at 2^6 .. 2^8.75 (e4m3's largest is 448).
-// The row sum sum_j 2^(x_ij - m_i) = sum_j p'_ij / b_j is taken from the fp32 p'.
+// m_i tracks the maximum of x_ij + log2 b_j, kept 2^13 below p's top so that small weights stay
+// above e5m2's floor: the largest weight of a row is held at 2^13 .. 2^15.75 (e5m2's largest is
+// 57344 = 2^15.81). The row sum sum_j 2^(x_ij - m_i) = sum_j p'_ij / b_j is taken from the fp32 p', and
+// scaled by 2^-13: with b = 2^-100 throughout (a context of zeros) it would overflow.
 //
 // Work: an item is (request, K/V head, query-row tile); its tiles of 128 tokens line up with all
 // other items' in one sequence, which is cut into equal ranges, one per CTA, whatever the
@@ -58,8 +62,9 @@
 namespace apex {
 
 constexpr int kPagedTile = 128;      // cached tokens per tile
-constexpr float kPagedTop = 6.0f;    // log2 of the weight that a row's maximum maps to
-constexpr float kPagedMost = 8.75f;  // a weight above 2^this moves the maximum (448 = 2^8.807)
+constexpr float kPagedTop = 13.0f;    // log2 of the weight that a row's maximum maps to
+constexpr float kPagedMost = 15.75f;  // a weight above 2^this moves the maximum (57344 = 2^15.807)
+constexpr float kPagedSumUnit = 1.f / 8192.f;  // 2^-kPagedTop: row sums are in these
 // V scales below 2^-100 (0 among them) count as 2^-100, so that 1 / b stays in range.
 constexpr float kPagedLeastScale = 7.888609052210118e-31f;
 
@@ -99,7 +104,8 @@ struct PagedCfg {
   static constexpr int kRow = D < 128 ? D : 128;         // bytes of a token row in a column chunk
   static constexpr int kChunks = (D + 127) / 128;
   static constexpr uint32_t kSwizzle = kRow == 128 ? 2 : 4;
-  static constexpr int kTerms = std::is_same<T, __half>::value ? 3 : 2;  // of q
+  static constexpr int kQTerms = std::is_same<T, __half>::value ? 3 : 2;  // of a query value
+  static constexpr int kWTerms = 3;                                       // of a weight
   static constexpr bool kQueryMajor = NQ >= 64;
   // Columns of an S buffer.
   static constexpr int kSCols = kQueryMajor ? kPagedTile : NQ;
@@ -122,10 +128,10 @@ struct PagedCfg {
   // their quarter, so two of the SM's four schedulers would do nothing otherwise. Of O, rows 64 .. 127
   // are never read; the weights that they come from are what lies behind the 64 rows.
   static constexpr int kCopies =
-      NQ == 64 && 2 * kTerms * NQ * D + kTerms * kPTerm + kMiscBytes + 3 * kSlotBytes <= kBudget ? 2 : 1;
-  static constexpr int kQBytes = kTerms * NQ * D * kCopies;  // one segment's query rows
+      NQ == 64 && 2 * kQTerms * NQ * D + kWTerms * kPTerm + kMiscBytes + 3 * kSlotBytes <= kBudget ? 2 : 1;
+  static constexpr int kQBytes = kQTerms * NQ * D * kCopies;  // one segment's query rows
   static constexpr int slots(int q_bufs, int p_bufs) {
-    return (kBudget - q_bufs * kQBytes - p_bufs * kTerms * kPTerm - kMiscBytes) / kSlotBytes;
+    return (kBudget - q_bufs * kQBytes - p_bufs * kWTerms * kPTerm - kMiscBytes) / kSlotBytes;
   }
   static constexpr int kPBufs = slots(1, 2) >= 3 ? 2 : 1;
   // The next segment's query rows are split ahead of time, by a warp of their own, where that
@@ -155,7 +161,7 @@ struct PagedCfg {
   // shared-memory plan
   static constexpr int kQ = kNS * kSlotBytes;
   static constexpr int kP = kQ + kQBufs * kQBytes;
-  static constexpr int kBars = kP + kPBufs * kTerms * kPTerm;
+  static constexpr int kBars = kP + kPBufs * kWTerms * kPTerm;
   static constexpr int kKvFull = 0, kKvEmpty = kNS, kQFull = 2 * kNS, kQEmpty = kQFull + 2,
                        kColEmpty = kQEmpty + 2, kSFull = kColEmpty + 2, kSFree = kSFull + 2, kPFull = kSFree + 2, kPvDone = kPFull + 2, kScFull = kPvDone + 2,
                        kScEmpty = kScFull + kScaleRing, kSegFull = kScEmpty + kScaleRing,
@@ -498,10 +504,32 @@ __device__ __forceinline__ void half2_of_e4m3x4(uint32_t v, __half2& a, __half2&
   b = *reinterpret_cast<__half2*>(&y);
 }
 
-// Splits four fp16 values into K terms that add up to them: e4m3, and of three the last e5m2, whose
+// e5m2 is fp16's upper byte.
+__device__ __forceinline__ void half2_of_e5m2x4(uint32_t v, __half2& a, __half2& b) {
+  const uint32_t x = __byte_perm(v, 0, 0x1404), y = __byte_perm(v, 0, 0x3424);
+  a = *reinterpret_cast<const __half2*>(&x);
+  b = *reinterpret_cast<const __half2*>(&y);
+}
+
+// Splits four weights (fp16, below 57344) into terms of e5m2 that add up to them.
+template <int K>
+__device__ __forceinline__ void split_weights(__half2 a, __half2 b, uint32_t (&term)[K]) {
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    term[i] = e5m2x4_of_half2(a, b);
+    if (i + 1 < K) {
+      __half2 ra, rb;
+      half2_of_e5m2x4(term[i], ra, rb);
+      a = __hsub2(a, ra);
+      b = __hsub2(b, rb);
+    }
+  }
+}
+
+// Splits four query values (fp16) into K terms that add up to them: e4m3, and of three the last e5m2, whose
 // smallest values lie 2^7 below e4m3's (a third piece has three bits left, as many as it holds).
 template <int K>
-__device__ __forceinline__ void split_terms(__half2 a, __half2 b, uint32_t (&term)[K]) {
+__device__ __forceinline__ void split_query(__half2 a, __half2 b, uint32_t (&term)[K]) {
 #pragma unroll
   for (int i = 0; i < K; ++i) {
     if (i == 2) {
@@ -546,7 +574,7 @@ __device__ __forceinline__ int warp_column_sums(float (&v)[N]) {
 }
 
 // Splits a segment's query rows: each is scaled by a power of two to (224, 448], split into
-// e4m3 terms and stored as the B operand of S^T, [term][16-byte chunk of the head dim][row]; the
+// 8-bit terms and stored as the B operand of S^T, [term][16-byte chunk of the head dim][row]; the
 // rows' column arrays are set up. Warp `w` of `warps` takes its share of the rows.
 template <typename T, int D, int NQ, int kAhead>
 __device__ __forceinline__ void split_query_rows(const PagedParams& p, const PagedSegment& seg, uint8_t* smem,
@@ -600,20 +628,20 @@ __device__ __forceinline__ void split_query_rows(const PagedParams& p, const Pag
     for (int d = 1; d < kPerRow; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
     const float s = append_scale(Elem<T>::to_float2(top).x);
     const float inv = 1.f / s;  // a power of two
-    uint32_t term[C::kTerms][4];
+    uint32_t term[C::kQTerms][4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       // Scaled values fit fp16 exactly (11 bits; below 2^-13 fewer, far under e4m3's floor).
       const float2 f = __fmul2_rn(Elem<T>::to_float2(x[2 * k]), make_float2(inv, inv));
       const float2 g = __fmul2_rn(Elem<T>::to_float2(x[2 * k + 1]), make_float2(inv, inv));
       __half2 a = __floats2half2_rn(f.x, f.y), b = __floats2half2_rn(g.x, g.y);
-      uint32_t four[C::kTerms];
-      split_terms(a, b, four);
+      uint32_t four[C::kQTerms];
+      split_query(a, b, four);
 #pragma unroll
-      for (int j = 0; j < C::kTerms; ++j) term[j][k] = four[j];
+      for (int j = 0; j < C::kQTerms; ++j) term[j][k] = four[j];
     }
 #pragma unroll
-    for (int j = 0; j < C::kTerms; ++j) {
+    for (int j = 0; j < C::kQTerms; ++j) {
       const uint32_t at = place_of(c) + j * C::kCopies * NQ * D;
       ptx::st_shared_v4(at, term[j][0], term[j][1], term[j][2], term[j][3]);
       if (C::kCopies == 2) ptx::st_shared_v4(at + NQ * C::kRow, term[j][0], term[j][1], term[j][2], term[j][3]);
@@ -928,7 +956,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
               }
             }
             wait_p_buffer();
-            const uint32_t dst = sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kTerms * C::kPTerm + row * 128;
+            const uint32_t dst = sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kWTerms * C::kPTerm + row * 128;
 #pragma unroll 1
             for (int c0 = 0; c0 < kTok; c0 += NC) {
               if (kTok > NC) {
@@ -939,7 +967,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
 #pragma unroll
               for (int half = 0; half < NC / 16; ++half) {
                 const int c16 = tok0 + c0 + 16 * half;
-                uint32_t term[C::kTerms][4];
+                uint32_t term[C::kWTerms][4];
                 float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -948,15 +976,15 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
                   const float2 e1 = make_float2(ptx::ex2(d[x + 1].x), ptx::ex2(d[x + 1].y));
                   sum = __fadd2_rn(sum, __fadd2_rn(e0, e1));
                   __half2 a = __floats2half2_rn(e0.x, e0.y), b = __floats2half2_rn(e1.x, e1.y);
-                  uint32_t four[C::kTerms];
-                  split_terms(a, b, four);
+                  uint32_t four[C::kWTerms];
+                  split_weights(a, b, four);
 #pragma unroll
-                  for (int i = 0; i < C::kTerms; ++i) term[i][k] = four[i];
+                  for (int i = 0; i < C::kWTerms; ++i) term[i][k] = four[i];
                 }
                 l = fmaf(sum.x + sum.y, sc[c16 >> p.block_shift].z, l);
                 const uint32_t unit = (uint32_t)((c16 >> 4) ^ (row & 7)) << 4;
 #pragma unroll
-                for (int i = 0; i < C::kTerms; ++i)
+                for (int i = 0; i < C::kWTerms; ++i)
                   ptx::st_shared_v4(dst + unit + i * C::kPTerm, term[i][0], term[i][1], term[i][2], term[i][3]);
               }
             }
@@ -965,7 +993,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           clear_unseen(j, 13 + pair, [&](int x) {
             const int pos = pos0 + x;
             if (!idle && x >= tok0 && x < tok0 + kTok && pos >= lo && pos < hi)
-              ptx::st_shared_u8(sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kTerms * C::kPTerm + row * 128 +
+              ptx::st_shared_u8(sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kWTerms * C::kPTerm + row * 128 +
                                     (((x >> 4) ^ (row & 7)) << 4) + (x & 15), 0x7fu);
           });
           ptx::fence_proxy_async_smem();
@@ -1003,12 +1031,12 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           for (int x = 0; x < kParts; ++x) s += sums[part_at(k, x)];
           sum = fmaf(f[k], s, sum);
         }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const float inv = sum == 0.f ? 0.f : kPagedSumUnit / sum;
 #pragma unroll
         for (int k = 0; k < C::kPairs; ++k) f[k] *= inv;
         const bool real = copy == 0 && row < seg.rows;
         if (wg == 0 && real) {
-          const float lse2 = sum == 0.f ? -INFINITY : __log2f(sum) - ref;
+          const float lse2 = sum == 0.f ? -INFINITY : __log2f(sum) + (kPagedTop - ref);
           if (seg.slot >= 0)
             p.part_lse[(long long)seg.slot * NQ + t] = lse2;
           else if (p.lse != nullptr)
@@ -1076,7 +1104,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           const int sb = g & 1;
           const int pos0 = (seg.tile + j) * kPagedTile, pos = pos0 + t;
           wait(C::kScFull + g % C::kScaleRing, (uint32_t)(g / C::kScaleRing));
-          const float4 sc = scales[(g % C::kScaleRing) * 8 + page];  // a * scale_log2, log2 b, 1 / b
+          const float4 sc = scales[(g % C::kScaleRing) * 8 + page];  // a * scale_log2, log2 b, 2^-13 / b
           wait(C::kSFull + sb, (uint32_t)(g >> 1));
           ptx::tc_fence_after();
           float2 d[NC / 2];
@@ -1162,10 +1190,10 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
           }
           // P buffer sb was read by P V of tile g - 2.
           if (g >= 2) wait(C::kPvDone + sb, (uint32_t)((g - 2) >> 1));
-          const uint32_t dst = sbase + C::kP + sb * C::kTerms * C::kPTerm + t * 16 + c_first * 128;
+          const uint32_t dst = sbase + C::kP + sb * C::kWTerms * C::kPTerm + t * 16 + c_first * 128;
 #pragma unroll
           for (int c = 0; c < NC; c += 16) {
-            uint32_t term[C::kTerms][4];
+            uint32_t term[C::kWTerms][4];
 #pragma unroll
             for (int k = 0; k < 16; k += 4) {
               const int x = (c + k) / 2;
@@ -1174,13 +1202,13 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
               l[x] = __ffma2_rn(e0, i2, l[x]);
               l[x + 1] = __ffma2_rn(e1, i2, l[x + 1]);
               __half2 a = __floats2half2_rn(e0.x, e0.y), b = __floats2half2_rn(e1.x, e1.y);
-              uint32_t four[C::kTerms];
-              split_terms(a, b, four);
+              uint32_t four[C::kWTerms];
+              split_weights(a, b, four);
 #pragma unroll
-              for (int j2 = 0; j2 < C::kTerms; ++j2) term[j2][k >> 2] = four[j2];
+              for (int j2 = 0; j2 < C::kWTerms; ++j2) term[j2][k >> 2] = four[j2];
             }
 #pragma unroll
-            for (int j2 = 0; j2 < C::kTerms; ++j2)
+            for (int j2 = 0; j2 < C::kWTerms; ++j2)
               ptx::st_shared_v4(dst + c * 128 + j2 * C::kPTerm, term[j2][0], term[j2][1], term[j2][2], term[j2][3]);
           }
           clear_unseen(j, 1 + wg, [&](int x) {  // columns 16-byte chunk by chunk, tokens within
@@ -1206,8 +1234,8 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
         ptx::named_bar_sync(1 + wg, 128);
         if (t < NC && t < rows) {
           const float sum = red[t] + red[NC + t] + red[2 * NC + t] + red[3 * NC + t];
-          const float lse2 = sum == 0.f ? -INFINITY : __log2f(sum) - col_nm[t];
-          col_f[t] = sum == 0.f ? 0.f : 1.f / sum;
+          const float lse2 = sum == 0.f ? -INFINITY : __log2f(sum) + (kPagedTop - col_nm[t]);
+          col_f[t] = sum == 0.f ? 0.f : kPagedSumUnit / sum;
           if (seg.slot >= 0) {
             p.part_lse[(long long)seg.slot * NQ + c_first + t] = lse2;
           } else if (p.lse != nullptr) {
@@ -1362,16 +1390,15 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     __syncwarp();
   } else if (warp == kWarpMma || (C::kTwoIssuers && warp == kWarpQ)) {
     // =============================================================== MMA ===
-    // e4m3, fp32 sums, M = 128. S: both operands K-major. P V: V is always MN-major; the weights
+    // 8 bits, fp32 sums, M = 128. S: both operands K-major. P V: V is always MN-major; the weights
     // are MN-major as the B operand (token-major), K-major as the A operand (query-major).
     constexpr uint32_t kDesc = (1u << 4) | ((uint32_t)(128 >> 4) << 24);
     constexpr uint32_t idS = kDesc | ((uint32_t)(C::kSCols >> 3) << 17);
-    constexpr uint32_t idPV = C::kQueryMajor ? kDesc | (1u << 16) | ((uint32_t)(D >> 3) << 17)
-                                             : kDesc | (1u << 15) | (1u << 16) | ((uint32_t)(NQ >> 3) << 17);
-    // The operand that is split is e5m2 in its third term.
-    auto with_type = [](uint32_t id, int term) {
-      return term == 2 ? id | (1u << (C::kQueryMajor ? 7 : 10)) : id;
-    };
+    // The operand that is split (query-major A, token-major B) is e5m2 where it is a weight, or the third
+    // term of q.
+    constexpr uint32_t kE5m2 = 1u << (C::kQueryMajor ? 7 : 10);
+    constexpr uint32_t idPV = kE5m2 | (C::kQueryMajor ? kDesc | (1u << 16) | ((uint32_t)(D >> 3) << 17)
+                                                      : kDesc | (1u << 15) | (1u << 16) | ((uint32_t)(NQ >> 3) << 17));
     int gs = 0, gp = 0;  // S and P V tiles issued
     auto acquire = [&](uint32_t fill) -> int {
       const int slot = (int)(fill % NS);
@@ -1393,16 +1420,16 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
             const uint64_t k = ptx::smem_desc(sbase + slot * C::kSlotBytes + ch * (kPagedTile * C::kRow) + ks * 32, 16,
                                               8 * C::kRow, C::kSwizzle);
 #pragma unroll
-            for (int j = 0; j < C::kTerms; ++j) {
+            for (int j = 0; j < C::kQTerms; ++j) {
               const uint32_t rows = sbase + C::kQ + (n % C::kQBufs) * C::kQBytes + j * C::kCopies * NQ * D;
               const uint32_t dS = tmem + (uint32_t)(sb * C::kSCols);
               if constexpr (C::kQueryMajor) {
                 const uint64_t q = ptx::smem_desc(rows + ch * (C::kCopies * NQ * C::kRow) + ks * 32, 16,
                                                   8 * C::kRow, C::kSwizzle);
-                ptx::umma_ss_f8_warp(dS, q, k, with_type(idS, j), acc);
+                ptx::umma_ss_f8_warp(dS, q, k, j == 2 ? idS | kE5m2 : idS, acc);
               } else {
                 const uint64_t q = ptx::smem_desc(rows + (ch * (C::kRow / 16) + 2 * ks) * (NQ * 16), NQ * 16, 128, 0);
-                ptx::umma_ss_f8_warp(dS, k, q, with_type(idS, j), acc);
+                ptx::umma_ss_f8_warp(dS, k, q, j == 2 ? idS | kE5m2 : idS, acc);
               }
               acc = 1;
             }
@@ -1419,7 +1446,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       const int slot = acquire(fill);
       ptx::tc_fence_after();
       if (ok) {
-        const uint32_t weights = sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kTerms * C::kPTerm;
+        const uint32_t weights = sbase + C::kP + (C::kPBufs == 2 ? sb : 0) * C::kWTerms * C::kPTerm;
         const uint32_t dO = tmem + (uint32_t)(2 * C::kSCols + (C::kPairs == 2 ? sb * D : 0));
         if constexpr (C::kQueryMajor) {
 #pragma unroll
@@ -1427,9 +1454,9 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
             const uint64_t v = ptx::smem_desc(sbase + slot * C::kSlotBytes + ks * 32 * C::kRow, kPagedTile * C::kRow,
                                               8 * C::kRow, C::kSwizzle);
 #pragma unroll
-            for (int j = 0; j < C::kTerms; ++j) {
+            for (int j = 0; j < C::kWTerms; ++j) {
               const uint64_t w = ptx::smem_desc(weights + j * C::kPTerm + ks * 32, 16, 1024, 2);
-              ptx::umma_ss_f8_warp(dO, w, v, with_type(idPV, j), first && ks == 0 && j == 0 ? 0u : 1u);
+              ptx::umma_ss_f8_warp(dO, w, v, idPV, first && ks == 0 && j == 0 ? 0u : 1u);
             }
           }
         } else {
@@ -1442,9 +1469,9 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
                   sbase + slot * C::kSlotBytes + ch * (kPagedTile * C::kRow) + ks * 32 * C::kRow, 0, 8 * C::kRow,
                   C::kSwizzle);
 #pragma unroll
-              for (int j = 0; j < C::kTerms; ++j) {
+              for (int j = 0; j < C::kWTerms; ++j) {
                 const uint64_t w = ptx::smem_desc(weights + j * C::kPTerm + ks * 32 * 16, 128, 2048, 0);
-                ptx::umma_ss_f8_warp(dO + (uint32_t)(ch * NQ), v, w, with_type(idPV, j), first && ks == 0 && j == 0 ? 0u : 1u);
+                ptx::umma_ss_f8_warp(dO + (uint32_t)(ch * NQ), v, w, idPV, first && ks == 0 && j == 0 ? 0u : 1u);
               }
             }
         }
@@ -1485,7 +1512,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     __syncwarp();
   } else if (warp == kWarpScale) {
     // ============================================================ scales ===
-    // Ahead of the softmax: per tile and page, a * sm_scale * log2 e, log2 b and 1 / b.
+    // Ahead of the softmax: per tile and page, a * sm_scale * log2 e, log2 b and 2^-13 / b.
     // Four tiles' loads at a time: lane 8 i + k looks after page k of the i-th.
     const int pages = kPagedTile >> p.block_shift;
     float4* const scales = reinterpret_cast<float4*>(smem + C::kScales);
@@ -1520,15 +1547,15 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
         const int j = j0 + (lane >> 3), page = lane & 7;
         const int at = (seg.tile + j) * kPagedTile + (page << p.block_shift);
         // Pages that are not there: zero scores and values, and a V scale too small to move a maximum.
-        float4 sc = make_float4(0.f, -100.f, 1.f / kPagedLeastScale, 0.f);
+        float4 sc = make_float4(0.f, -100.f, kPagedSumUnit / kPagedLeastScale, 0.f);
         if (j < seg.n && page < pages && at < seg.hi && at + (1 << p.block_shift) > seg.lo) {
           const int id = read_input(p.block_table + (long long)seg.b * p.table_stride + (at >> p.block_shift));
           if (id >= 0 && id < p.num_blocks) {
             const float a = read_input(p.k_scale + (long long)id * p.heads_kv + seg.h);
             const float given = read_input(p.v_scale + (long long)id * p.heads_kv + seg.h);
             const float b = fmaxf(given, kPagedLeastScale);
-            // A scale of NaN goes on in the exponent, which is masked; 1 / b is not, and stays a number.
-            sc = make_float4(a * p.scale_log2, given != given ? given : __log2f(b), 1.f / b, 0.f);
+            // A scale of NaN goes on in the exponent, which is masked; b is not, and stays a number.
+            sc = make_float4(a * p.scale_log2, given != given ? given : __log2f(b), kPagedSumUnit / b, 0.f);
           }
         }
         const int take = min(4, seg.n - j0);
