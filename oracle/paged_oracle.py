@@ -93,18 +93,20 @@ def attend(q, k_codes, v_codes, k_scale, v_scale, table, lens, cu, block, causal
     bounds on what the kernels' documented roundings may move them by (before o is rounded
     to its type):
 
-    * a weight p * v_scale is rounded to fp16 (2^-12 covers half a step of 11 bits) and held in
-      two e4m3 terms: 2^-8 of itself (half a step of four bits, twice) plus 2^-16 of the row's largest (e4m3's spacing 2^-9 below 2^-6, halved, with
-      the largest at 2^6);
-    * a query value in two terms (three for fp16): exact, or off by 2^-10 / 224 of the largest
-      of the tile's, taken here as the largest of the request's rows;
-    * fp32 products and sums: 2^-21 of the sum of magnitudes."""
+    * a weight p * v_scale is rounded to 11 bits, 2^-11 of itself, and held in terms of 8 bits that add up to
+      that, or to 2^-17 with the row's largest at 2^13 or more: 2^-30 of the row's largest, or the weight itself
+      where it is smaller;
+    * a query value in two terms (bf16) or three (fp16): exact, or off by 2^-10 (2^-17) where its row's largest
+      lies above 224;
+    * fp32 products and sums: 2^-21 of the sum of magnitudes in a score; in o 2^-19, and 2^-23 for each of the
+      three products of 32 tokens that are added up one after another."""
     total, heads, dim = q.shape
     group = heads // k_codes.shape[1]
     sm_scale = dim ** -0.5 if sm_scale is None else sm_scale
     o = torch.zeros((total, heads, dim), dtype=torch.float64)
     lse = torch.zeros((heads, total), dtype=torch.float64)
     o_bound, lse_bound = torch.zeros_like(o), torch.zeros_like(lse)
+    lost = 2.0 ** (-17 if q.dtype is torch.float16 else -10) / 224
     q = q.double()
     for b in range(len(lens)):
         n, rows = lens[b], range(cu[b], cu[b + 1])
@@ -115,7 +117,6 @@ def attend(q, k_codes, v_codes, k_scale, v_scale, table, lens, cu, block, causal
             vc = v_codes[ids, hk].reshape(-1, dim)[:n]
             ks = k_scale[ids, hk].repeat_interleave(block)[:n]
             vs = v_scale[ids, hk].repeat_interleave(block)[:n]
-            biggest = q[cu[b]:cu[b + 1]].abs().max().item() if len(rows) else 0.0
             for r in rows:
                 place = n - len(rows) + r - cu[b]
                 hi = min(place + 1, n) if causal else n
@@ -128,10 +129,12 @@ def attend(q, k_codes, v_codes, k_scale, v_scale, table, lens, cu, block, causal
                 lse[h, r] = torch.logsumexp(s, 0)
                 p = torch.exp(s - lse[h, r])
                 o[r, h] = p @ v
-                off = sm_scale * (k.abs().sum(1) * (biggest * 2.0 ** -10 / 224) + (k.abs() @ q[r, h].abs()) * 2.0 ** -21)
+                biggest = q[r, h].abs().max()
+                off = sm_scale * (k.abs().sum(1) * (biggest * lost) + (k.abs() @ q[r, h].abs()) * 2.0 ** -21)
                 off = off.max().item() + 2.0 ** -20 * (1 + abs(lse[h, r].item()))
                 lse_bound[h, r] = off
-                mass = p @ v.abs()
-                o_bound[r, h] = mass * (2.0 ** -8 + 2.0 ** -12 + 2 * off + 2.0 ** -19) \
-                    + 2.0 ** -16 * (p * vs[lo:hi]).max() * vc[lo:hi].abs().sum(0)
+                w = p * vs[lo:hi]
+                floor = torch.minimum(w, 2.0 ** -30 * w.max()) @ vc[lo:hi].abs()
+                steps = 3 * -(-(hi - lo) // 32)
+                o_bound[r, h] = (p @ v.abs()) * (2.0 ** -11 + 2 * off + 2.0 ** -19 + steps * 2.0 ** -23) + floor
     return o, lse, o_bound, lse_bound
