@@ -1,12 +1,14 @@
-"""Builds libapex_attn.so in-tree (next to the apex_attn package) with nvcc for sm_100a, and the
+"""Builds libapex_attn.so in-tree (next to the apex_attn package) with nvcc for sm_100a, and then the
 Python module _calls.so beside it with g++.
 
-Usage: python apex-tune-results_b200/build.py [--verbose]
+Usage: python apex-tune-results_b200/build.py [--verbose] [--force] [--strict]
 Each source is compiled to an object under _build/ (side by side, and only when it or a
 header changed), then linked. The library links the CUDA runtime statically and resolves
 cuTensorMapEncodeTiled through cudaGetDriverEntryPoint, so it needs no -lcuda and loads on
-a machine without a GPU. _calls.so uses the headers of the installed torch and links to its
-libraries.
+a machine without a GPU; nvcc is all that it needs. _calls.so, a shorter way for the host
+from Python to some of the library's calls, uses the headers of the installed torch and links to
+its libraries. Where it cannot be built (no torch, no headers, no C++ compiler) the package does
+without, so that is a warning, and an error with --strict only.
 """
 from __future__ import annotations
 
@@ -17,6 +19,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -61,15 +64,28 @@ def up_to_date() -> bool:
     return newer(OUT, inputs)
 
 
+def torch_dir() -> str:
+    spec = importlib.util.find_spec("torch")
+    if spec is None or spec.origin is None:
+        raise RuntimeError("torch is not installed")
+    return os.path.dirname(spec.origin)
+
+
+def cxx11_abi() -> int:
+    """The C++ library ABI that the installed torch was compiled with."""
+    import torch
+    return int(torch.compiled_with_cxx11_abi())
+
+
 def calls_command(out: str) -> list[str]:
-    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
-    include = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+    torch = torch_dir()
+    include = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"),
                sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include"),
                os.path.join(ROOT, "include")]
     libs = ["torch_python", "torch", "torch_cpu", "torch_cuda", "c10", "c10_cuda"]
     return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-            "-D_GLIBCXX_USE_CXX11_ABI=1", *("-I" + p for p in include), "-o", out, CALLS_SOURCE,
-            "-L" + os.path.join(torch_dir, "lib"), *("-l" + name for name in libs)]
+            f"-D_GLIBCXX_USE_CXX11_ABI={cxx11_abi()}", *("-I" + p for p in include), "-o", out, CALLS_SOURCE,
+            "-L" + os.path.join(torch, "lib"), *("-l" + name for name in libs)]
 
 
 def build_calls(force: bool = False) -> str:
@@ -83,8 +99,21 @@ def build_calls(force: bool = False) -> str:
     return CALLS_OUT
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    build_calls(force)
+def build(force: bool = False, verbose: bool = False, strict: bool = False) -> str:
+    """Builds both; returns the library's path. Without _calls.so: RuntimeError if `strict`, else a warning."""
+    build_library(force, verbose)
+    try:
+        build_calls(force)
+    except (RuntimeError, ImportError, OSError) as e:
+        if os.path.exists(CALLS_OUT):  # of other sources: it may not fit the library
+            os.remove(CALLS_OUT)
+        if strict:
+            raise RuntimeError(f"_calls.so was not built: {e}") from e
+        warnings.warn(f"_calls.so was not built ({e}): the paged cache's calls take the longer way through Python")
+    return OUT
+
+
+def build_library(force: bool = False, verbose: bool = False) -> str:
     if not force and up_to_date():
         return OUT
     os.makedirs(OBJ, exist_ok=True)
@@ -119,5 +148,6 @@ if __name__ == "__main__":
     ap = argparse.ArgumentParser()
     ap.add_argument("--verbose", action="store_true")
     ap.add_argument("--force", action="store_true")
+    ap.add_argument("--strict", action="store_true")
     a = ap.parse_args()
-    print(build(force=a.force, verbose=a.verbose))
+    print(build(force=a.force, verbose=a.verbose, strict=a.strict))
