@@ -25,7 +25,10 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import importlib.util
 import math
+import sysconfig
+import warnings
 from typing import NamedTuple
 
 import torch
@@ -46,14 +49,28 @@ _INT_MAX = 2 ** 31 - 1
 _calls = None
 
 
-def _load_calls():
-    """The native module with the library's addresses set, or False where it was not built."""
-    global _calls
-    lib = _lib.load()
+def _import_calls():
+    """The native module, or False where it was not built. One that was built for another torch or
+    Python knows their objects by another layout: False too, with a warning."""
+    if importlib.util.find_spec("._calls", __package__) is None:
+        return False
+    here = f"torch {torch.__version__} {sysconfig.get_config_var('SOABI')}"
     try:
         from . import _calls as module
-    except ImportError:
-        module = False
+        built_for = getattr(module, "built_for", "an unknown version")
+    except ImportError as e:
+        built_for = f"another version ({e})"
+    if built_for == here:
+        return module
+    warnings.warn(f"apex_attn._calls was built for {built_for} and is left out with {here}: build it again")
+    return False
+
+
+def _load_calls():
+    """The native module with the library's addresses set, or False."""
+    global _calls
+    lib = _lib.load()
+    module = _import_calls()
     if module:
         module.init(*(ctypes.cast(getattr(lib, "apex_attn_" + name), ctypes.c_void_p).value for name in (
             "kv_plan", "kv_release", "kv_append", "fwd_paged_workspace_bytes", "fwd_paged")))

@@ -15,6 +15,7 @@ from __future__ import annotations
 import argparse
 import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -71,6 +72,26 @@ def torch_dir() -> str:
     return os.path.dirname(spec.origin)
 
 
+def calls_key() -> str:
+    """What _calls.so is compiled against: it uses the insides of torch's tensors and Python's objects, so
+    it is only good for these very versions. Compiled in, and compared when it is loaded."""
+    with open(os.path.join(torch_dir(), "version.py")) as f:
+        version = re.search(r"^__version__\s*=\s*['\"]([^'\"]+)['\"]", f.read(), re.MULTILINE)
+    if version is None:
+        raise RuntimeError("the installed torch names no version")
+    return f"torch {version.group(1)} {sysconfig.get_config_var('SOABI')}"
+
+
+def cxx() -> str:
+    return os.environ.get("CXX", "g++")
+
+
+def calls_stamp() -> str:
+    """The key and the compiler's version: with another of either the module is built anew."""
+    proc = subprocess.run([cxx(), "--version"], capture_output=True, text=True)
+    return f"{calls_key()}\n{cxx()}: {proc.stdout.splitlines()[0] if proc.stdout else ''}\n"
+
+
 def cxx11_abi() -> int:
     """The C++ library ABI that the installed torch was compiled with."""
     import torch
@@ -83,19 +104,27 @@ def calls_command(out: str) -> list[str]:
                sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include"),
                os.path.join(ROOT, "include")]
     libs = ["torch_python", "torch", "torch_cpu", "torch_cuda", "c10", "c10_cuda"]
-    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+    return [cxx(), "-O2", f'-DAPEX_CALLS_KEY="{calls_key()}"', "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
             f"-D_GLIBCXX_USE_CXX11_ABI={cxx11_abi()}", *("-I" + p for p in include), "-o", out, CALLS_SOURCE,
             "-L" + os.path.join(torch, "lib"), *("-l" + name for name in libs)]
 
 
 def build_calls(force: bool = False) -> str:
-    if force or not newer(CALLS_OUT, [CALLS_SOURCE, API, __file__]):
+    stamp, at = calls_stamp(), os.path.join(OBJ, "_calls.stamp")
+    same = False
+    if os.path.exists(at):
+        with open(at) as f:
+            same = f.read() == stamp
+    if force or not same or not newer(CALLS_OUT, [CALLS_SOURCE, API, __file__]):
         tmp = CALLS_OUT + ".tmp"
         proc = subprocess.run(calls_command(tmp), capture_output=True, text=True)
         if proc.returncode != 0:
             sys.stderr.write(proc.stdout + proc.stderr)
             raise RuntimeError("g++ failed building _calls.so")
         os.replace(tmp, CALLS_OUT)
+        os.makedirs(OBJ, exist_ok=True)
+        with open(at, "w") as f:
+            f.write(stamp)
     return CALLS_OUT
 
 

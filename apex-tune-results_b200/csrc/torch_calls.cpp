@@ -375,4 +375,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nul
 
 }  // namespace
 
-extern "C" __attribute__((visibility("default"))) PyObject* PyInit__calls(void) { return PyModule_Create(&module); }
+#ifndef APEX_CALLS_KEY
+#error "APEX_CALLS_KEY names the torch and Python versions that this is compiled against"
+#endif
+
+extern "C" __attribute__((visibility("default"))) PyObject* PyInit__calls(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m != nullptr && PyModule_AddStringConstant(m, "built_for", APEX_CALLS_KEY) < 0) Py_CLEAR(m);
+  return m;
+}

@@ -54,3 +54,49 @@ def test_the_module_takes_its_abi_from_torch(build, monkeypatch):
     assert f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}" in build.calls_command("x.so")
     monkeypatch.setattr(torch, "compiled_with_cxx11_abi", lambda: False)
     assert "-D_GLIBCXX_USE_CXX11_ABI=0" in build.calls_command("x.so")
+
+
+def test_the_module_is_built_again_for_another_torch_or_compiler(build, monkeypatch):
+    built = []
+    real = build.subprocess.run
+
+    def run(cmd, **kw):
+        if "--version" in cmd:
+            return real(cmd, **kw)
+        built.append(cmd)
+        open(build.CALLS_OUT + ".tmp", "w").close()
+        return real(["true"], **kw)
+
+    monkeypatch.setattr(build.subprocess, "run", run)
+    build.build_calls()
+    build.build_calls()
+    assert len(built) == 1
+    for name, value in (("calls_key", "torch 1.2.3 cpython-399"), ("cxx", "cc")):
+        monkeypatch.setattr(build, name, lambda value=value: value)
+        before = len(built)
+        build.build_calls()
+        build.build_calls()
+        assert len(built) == before + 1, name
+
+
+def test_a_module_of_another_torch_is_left_out(monkeypatch):
+    import apex_attn.paged as paged
+    module = paged._import_calls()
+    if not module:
+        pytest.skip("_calls is not built")
+    import torch
+    assert module.built_for.startswith(f"torch {torch.__version__} ")
+    monkeypatch.setattr(module, "built_for", "torch 1.2.3 cpython-399")
+    with pytest.warns(UserWarning, match="torch 1.2.3"):
+        assert paged._import_calls() is False
+    monkeypatch.delattr(module, "built_for")
+    with pytest.warns(UserWarning, match="unknown"):
+        assert paged._import_calls() is False
+
+
+def test_the_built_module_is_the_one_for_this_torch(build):
+    import apex_attn.paged as paged
+    module = paged._import_calls()
+    if not module:
+        pytest.skip("_calls is not built")
+    assert module.built_for == build.calls_key()
