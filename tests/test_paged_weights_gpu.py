@@ -119,3 +119,27 @@ def test_one_loud_block_of_values(n, share, dim, heads_q, heads_kv, q_len, dtype
         p = problem(n, share, tail, 5, dim, heads_kv, heads_q, q_len, dtype, loud_block=True)
         check(p, 1)
         check(p, 296)
+
+
+@pytest.mark.parametrize("copies", [1, 296])
+@pytest.mark.parametrize("exponent", [-100, 0, 112, 118])
+@pytest.mark.parametrize("dim,heads_q,heads_kv,q_len,dtype", [(64, 4, 1, 1, "bf16"), (128, 8, 1, 5, "bf16")])
+def test_the_smallest_and_largest_scales_of_values(dim, heads_q, heads_kv, q_len, dtype, exponent, copies):
+    """Row sums hold 1 / scale of every token: 2^100 each for 200k tokens, or 2^-118 each for some. Held to the
+    bound above, and the logsumexp to 2^-16 (200k terms of fp32 sums in parts of 128 and up: 2^-20 each way)."""
+    from apex_attn import custom_attention_paged_forward
+    n = 200000 if exponent < 0 else 900
+    p = problem(n, 0.3, "spread", 5, dim, heads_kv, heads_q, q_len, dtype, block=128)
+    p["vs"] = torch.full_like(p["vs"], 2.0 ** exponent)
+    if exponent > 100:  # sums of magnitudes stay below the type's largest
+        p["v"] = (p["v"].float() / 64).to(E4M3)
+    check(p, copies)
+    table = torch.arange(p["k"].shape[0], dtype=torch.int32, device="cuda")[None]
+    _, lse = custom_attention_paged_forward(p["q"], p["k"], p["v"], p["ks"], p["vs"], table, ints([n]),
+                                            ints([0, q_len]), q_len, return_lse=True)
+    k = (p["k"].double() * p["ks"].double()[..., None, None]).transpose(0, 1).flatten(1, 2)[0, :n]
+    s = torch.einsum("thd,nd->htn", p["q"].double(), k) / math.sqrt(dim)
+    s = s.masked_fill(torch.arange(n, device="cuda") > torch.arange(n - q_len, n, device="cuda")[:, None], -torch.inf)
+    want = torch.logsumexp(s, -1)
+    # scores: 2^-13 of 0.8 in each of 128 places at 1/8, as in the bound above
+    assert ((lse.double() - want).abs() <= 2.0 ** -16 + 2.0 ** -13 * 0.8 * dim / math.sqrt(dim)).all()
