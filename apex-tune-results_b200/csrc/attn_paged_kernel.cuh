@@ -30,8 +30,8 @@
 // maximum is only moved when some p' would pass 2^15.75 (one vote per tile), which is rare after
 // a row's first tile.
 // More rows, in tiles of 64 or 128, are the M side themselves ("query-major"): S = Q K^T, O = P V, a
-// thread owns part of a row, and a maximum takes one exchange between warps. (Measured: two
-// 32-row token-major tiles for 33 to 96 rows are 10 to 60 % slower than one of 64 or 128.)
+// thread owns part of a row, and a maximum takes one exchange between warps. (Measured: 32 requests of
+// 40 rows take 31.8 us in tiles of 64, 43.6 in two token-major tiles of 32, 38.4 in tiles of 128.)
 //
 // m_i tracks the maximum of x_ij + log2 b_j, kept 2^13 below p's top so that small weights stay
 // above e5m2's floor: the largest weight of a row is held at 2^13 .. 2^15.75 (e5m2's largest is
@@ -45,8 +45,7 @@
 // Lengths are read on the device only.
 //
 // Warps: 4 to 16 softmax (32 rows of TMEM each), then TMA producer, MMA issuer, scales and work
-// list, and a fourth: token-major it splits the next segment's query rows, with
-// 64-row tiles it issues P V. The scales' warp alone walks the work list and publishes the segments
+// list, and a fourth that token-major splits the next segment's query rows. The scales' warp alone walks the work list and publishes the segments
 // in shared memory: a warp on its own takes some 4 cycles per dependent instruction, and all
 // warps walking cost each of them about 2 us at the start and 1 us per segment.
 //
@@ -138,11 +137,6 @@ struct PagedCfg {
   // leaves four ring slots; a query-major tile's are too many for one warp, and the softmax
   // warps split them between segments.
   static constexpr bool kSelfSplit = kQueryMajor;
-  // 64-row tiles: one warp issues S and another P V. The waits and the issue of a tile's products
-  // take a warp some 2500 cycles, the products themselves 1000, and the softmax of half a
-  // tile's rows no longer covers that (32 requests of 40 rows, fp16: 33.7 -> 31.6 us; with 128
-  // rows it does, and two warps make 3 x 1024 new tokens 562 us instead of 520).
-  static constexpr bool kTwoIssuers = NQ == 64;
   static constexpr int kQBufs = !kSelfSplit && slots(2, kPBufs) >= 4 ? 2 : 1;
   static constexpr int kNS = slots(kQBufs, kPBufs) > 12 ? 12 : slots(kQBufs, kPBufs);  // ring slots
   static_assert(kNS > kLead, "the ring needs K(j + kLead) beside V(j)");
@@ -709,7 +703,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       ptx::mbar_init(bar(C::kSegFull + s), 1);
       ptx::mbar_init(bar(C::kSegEmpty + s), C::kSoftWarps + 3);  // softmax, producer, MMA, query rows
     }
-    ptx::mbar_init(bar(C::kDrain), C::kTwoIssuers ? 2 : 1);  // warps that issue products
+    ptx::mbar_init(bar(C::kDrain), 1);
     *abort_flag = 0;
     for (int k = 0; k < 8; ++k) reinterpret_cast<unsigned*>(smem + C::kBad)[k] = 0;
     ptx::fence_mbar_init();
@@ -1388,7 +1382,7 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       }
     }
     __syncwarp();
-  } else if (warp == kWarpMma || (C::kTwoIssuers && warp == kWarpQ)) {
+  } else if (warp == kWarpMma) {
     // =============================================================== MMA ===
     // 8 bits, fp32 sums, M = 128. S: both operands K-major. P V: V is always MN-major; the weights
     // are MN-major as the B operand (token-major), K-major as the A operand (query-major).
@@ -1485,25 +1479,15 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
       // Places in the ring as the producer fills it.
       auto k_at = [&](int j) { return fills + j + max(0, j - C::kLead); };
       auto v_at = [&](int j) { return fills + j + min(seg.n, j + 1 + C::kLead); };
-      if (C::kTwoIssuers && warp == kWarpQ) {
+      wait(C::kQFull + (n & 1), (uint32_t)(n >> 1));
+      if (!C::kQueryMajor && seg.n == 0 && lane == 0) ptx::mbar_arrive(bar(C::kQEmpty + n % C::kQBufs));
 #pragma unroll 1
-        for (int j = 0; j < seg.n; ++j) issue_PV(v_at(j), j < C::kPairs);
-      } else {
-        wait(C::kQFull + (n & 1), (uint32_t)(n >> 1));
-        if (C::kTwoIssuers) {
+      for (int j = 0; j < min(seg.n, C::kLead); ++j) issue_S(k_at(j), j + 1 == seg.n);
 #pragma unroll 1
-          for (int j = 0; j < seg.n; ++j) issue_S(k_at(j), false);
-        } else {
-          if (!C::kQueryMajor && seg.n == 0 && lane == 0) ptx::mbar_arrive(bar(C::kQEmpty + n % C::kQBufs));
-#pragma unroll 1
-          for (int j = 0; j < min(seg.n, C::kLead); ++j) issue_S(k_at(j), j + 1 == seg.n);
-#pragma unroll 1
-          for (int j = 0; j < seg.n; ++j) {
-            const int next = j + C::kLead;
-            if (next < seg.n) issue_S(k_at(next), next + 1 == seg.n);
-            issue_PV(v_at(j), j < C::kPairs);
-          }
-        }
+      for (int j = 0; j < seg.n; ++j) {
+        const int next = j + C::kLead;
+        if (next < seg.n) issue_S(k_at(next), next + 1 == seg.n);
+        issue_PV(v_at(j), j < C::kPairs);
       }
       fills += 2 * seg.n;
     }
