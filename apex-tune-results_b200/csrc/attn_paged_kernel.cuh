@@ -49,10 +49,10 @@
 // in shared memory: a warp on its own takes some 4 cycles per dependent instruction, and all
 // warps walking cost each of them about 2 us at the start and 1 us per segment.
 //
-// Bound: a decode step by the cache's bytes (48 requests of up to 8191 tokens, 410 MB: 73 us, 5.6
-// TB/s; about 7 us of them pass before the first scores are there, 4 in the joining kernel);
-// calls with many new tokens by the softmax warps' issue (3 x 1024 tokens on 5k to 16k: 520 us, 838
-// TFLOP/s; schedulers busy 48 %, tensor pipe 28 %).
+// Bound: a decode step by the cache's bytes (48 requests of up to 8191 tokens, 410 MB: 76 us a call,
+// 5.4 TB/s; some 7 us of them pass before the first scores are there, 4 in the joining kernel);
+// calls with many new tokens by the softmax warps' issue (3 x 1024 tokens on 5k to 16k: 657 us a
+// call, 663 TFLOP/s; schedulers busy 52 %, tensor pipe 34 %).
 #pragma once
 
 #include "attn_fwd_kernel.cuh"
@@ -240,7 +240,7 @@ __device__ __forceinline__ int paged_qtiles(const PagedParams& p, const PagedReq
 // A CTA that begins an item spends about as long on it as on this many tiles: units of an item
 // are these and then its tiles, at least one (an item that sees nothing still has rows to
 // write). Without them the CTAs that got short requests finished last: 48 requests of 129 to
-// 8191 tokens take 88 us instead of 73, and three of 1024 new tokens each 565 instead of 520.
+// 8191 tokens take 102 us instead of 77, and three of 1024 new tokens each 695 instead of 665.
 template <int NQ>
 constexpr int kPagedItemUnits = NQ <= 32 ? 4 : 8;
 
@@ -1296,8 +1296,8 @@ __global__ void __launch_bounds__(PagedCfg<T, D, NQ>::kThreads, PagedCfg<T, D, N
     // The next K tile, V tile or both, from the block ids in lanes 0 .. pages - 1 and V's in lanes
     // 16 on. One wait, one announcement and one run of copies for both, where the ring is long enough
     // for the next K not to wait for a free V place: apart, a fill of four blocks took this warp
-    // 1150 cycles, and the card's memory brings one in 700. (Measured with five slots: 83 -> 76 us
-    // for 48 ragged requests; with three, 32 requests of 40 wide rows, it would be 87 -> 125.)
+    // 1150 cycles, and the card's memory brings one in 700. (Measured with five slots: 83 -> 77 us
+    // for 48 ragged requests; with three, 32 requests of 40 rows at d = 256, it would be 48 -> 52.)
     auto fill = [&](bool k, bool v, int ids) {  // `seg`'s head
       const bool second = lane >= 16;
       const uint32_t mine = fills + (k && v && second ? 1 : 0);

@@ -270,8 +270,8 @@ struct Elem<__half> {
 // 2048 values (16 tokens of 128) stays in registers between the pass for the maximum and the
 // one for the codes; a longer one is read again, from the L2.
 // Bound: DRAM for prompts (2 bytes read, 1 written per value): 25k tokens of 8 heads of 128 in
-// 29.5 us, 5.2 TB/s of 6.6; with 80 registers and three quarters of the warps it took 36 us, with
-// eight warps per CTA 30.4. Latency for a decode step: 3.3 us.
+// 31 us a call, 5.0 TB/s of 6.6. Of that 29.5 on the device, where it took 36 with 80 registers and
+// three quarters of the warps, and 30.4 with eight warps per CTA. Latency for a decode step: 4.9 us a call.
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * kAppendWarps, 8) kv_append_kernel(const AppendParams p) {
   constexpr int kPerRow = D / 8;   // 8 values (16 bytes of input) per lane and step

@@ -275,7 +275,8 @@ int launch_paged(const apex::PagedParams& p, const CUtensorMap& mk, const CUtens
   if (rc != APEX_ATTN_OK) return rc;
   const int grid = C::kCtas * std::min(num_sms, kMaxSms);
   // Both may be set up while the last CTAs of the kernel before them run; they wait for its end
-  // before they read or write anything (measured: about 1 us per call).
+  // before they read or write anything (measured: one short request 14.4 -> 11.9 us a call, 48 requests
+  // 80 -> 77; calls of 3 x 1024 new tokens lose 1 %).
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
