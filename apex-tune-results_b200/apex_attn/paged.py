@@ -310,7 +310,7 @@ def custom_attention_paged_forward(q, k_cache, v_cache, k_scale, v_scale, block_
 
     Precision: scores, maxima and sums are fp32. A softmax weight (times its block's V scale) is held
     to 2^-11 of itself, or to 2^-30 of the row's largest; a value of q exactly, or to 2^-17 (bf16) or
-    2^-24 (fp16) of its row's largest.
+    2^-24 (fp16) of its row's largest. Long sums of one sign come out low, by 2.6e-4 for 131072 tokens.
 
     Scales are not negative; V scales below 2^-100 count as 2^-100. A code or scale of NaN, or an
     infinite or NaN value of q, makes the rows that see it NaN and no others. Table entries

@@ -458,7 +458,8 @@ int apex_attn_kv_append(const apex_attn_kv_append_args* args, void* stream);
  * token (NaN codes too) changes no bit of the result. Scores, softmax statistics and sums are
  * fp32. A softmax weight (times its block's V scale) is held to 2^-11 of itself, or to 2^-30 of the
  * row's largest where that is more; a value of q exactly, or to 2^-17 (bf16) or 2^-24 (fp16) of its
- * row's largest. Scales are not negative; V scales below 2^-100 count as 2^-100. A code or scale of NaN,
+ * row's largest; long sums of one sign come out low, by 2.6e-4 for 131072 tokens where one CTA has
+ * them all. Scales are not negative; V scales below 2^-100 count as 2^-100. A code or scale of NaN,
  * or a value of q that is not finite, gives NaN to the rows that see it and to no others.
  * Offsets that fall or overlap give wrong rows, but nothing outside q and o is touched.
  * Refused: rows of o that overlap one another (APEX_ATTN_ERR_BAD_LAYOUT); above 2^30 query rows

@@ -143,3 +143,20 @@ def test_the_smallest_and_largest_scales_of_values(dim, heads_q, heads_kv, q_len
     want = torch.logsumexp(s, -1)
     # scores: 2^-13 of 0.8 in each of 128 places at 1/8, as in the bound above
     assert ((lse.double() - want).abs() <= 2.0 ** -16 + 2.0 ** -13 * 0.8 * dim / math.sqrt(dim)).all()
+
+
+@pytest.mark.parametrize("dim,heads_q,q_len,dtype", [(128, 4, 1, "fp16"), (128, 16, 8, "fp16"), (256, 16, 7, "bf16")])
+def test_long_sums_of_one_sign(dim, heads_q, q_len, dtype):
+    """131072 tokens with V of one sign, every item whole: three products for each 32 tokens, each sum cut by less
+    than 2^-23 of itself, and weights off by 2^-11 of themselves."""
+    from apex_attn import custom_attention_paged_forward
+    n = 131072
+    p = problem(n, 0.001, "spread", 5, dim, 1, heads_q, q_len, dtype, block=128)
+    p["v"] = p["v"].float().abs().to(E4M3)
+    o = custom_attention_paged_forward(p["q"].repeat(296, 1, 1), p["k"], p["v"], p["ks"], p["vs"],
+                                       torch.arange(n // 128, dtype=torch.int32, device="cuda").repeat(296, 1),
+                                       ints([n] * 296), ints([q_len * i for i in range(297)]), q_len)
+    want, _ = exact(p)
+    eps = torch.finfo(o.dtype).eps / 2
+    off = ((o.double().view(296, *want.shape) - want) / want).abs().max().item()
+    assert off <= 3 * n // 32 * 2.0 ** -23 + 2.0 ** -11 + eps
